@@ -1,5 +1,6 @@
-"""ctypes binding of libcutt.so: the four plan functions of include/cutt.h and
-the hooks of include/cutt_ext.h, with the same names and argument order.
+"""ctypes binding of libcutt.so: the four plan functions of include/cutt.h, the row
+operators of include/cutt_rows.h and the hooks of include/cutt_ext.h, with the same names
+and argument order.
 
 Device buffers are passed as integer addresses (e.g. ``tensor.data_ptr()``),
 streams as integer ``hipStream_t`` values (e.g.
@@ -22,6 +23,11 @@ _RESULT_NAMES = ["CUTT_SUCCESS", "CUTT_INVALID_PLAN", "CUTT_INVALID_PARAMETER", 
 
 METHOD_TRIVIAL, METHOD_PACKED, METHOD_PACKEDSPLIT, METHOD_TILED, METHOD_TILEDCOPY = 1, 2, 3, 4, 5
 METHOD_NAMES = {0: "Unknown", 1: "Trivial", 2: "Packed", 3: "PackedSplit", 4: "Tiled", 5: "TiledCopy"}
+
+
+# element types of rows that are summed (cuttRowType)
+CUTT_F32, CUTT_F16, CUTT_BF16 = 0, 1, 2
+CUTT_MAX_EXPERTS = 1024
 
 
 class CuttError(RuntimeError):
@@ -159,6 +165,20 @@ def lib():
     l.cuttModelCacheLinesCont.restype = None
     l.cuttModelShTransactions.argtypes = [ctypes.c_int] * 4 + [ip, ctypes.c_int, ip]
     l.cuttModelShTransactions.restype = None
+    i, z, ll = ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong
+    for name, args, result in (
+            ("cuttExpertRows", [i] * 4, ll),
+            ("cuttExpertSortWorkspace", [i] * 3, z),
+            ("cuttExpertSort", [i] * 6 + [z, vp] + [vp] * 6 + [z], i),
+            ("cuttExpertDispatch", [i] * 4 + [z, vp, vp, vp, vp, ll, vp, ll], i),
+            ("cuttExpertDispatchBackward", [i] * 5 + [vp, vp, vp, ll, vp, ll], i),
+            ("cuttExpertCombine", [i] * 5 + [vp, vp, vp, vp, ll, vp, ll], i),
+            ("cuttExpertCombineBackward", [i] * 5 + [vp] * 4 + [vp, ll] * 3 + [vp], i),
+            ("cuttPageTables", [i] * 5 + [vp] * 9, i),
+            ("cuttPageStore", [i] * 3 + [z, i, i] + [vp] * 4 + [llp, vp, vp, llp], i),
+            ("cuttPageLoad", [i] * 3 + [z, i, i] + [vp] * 4 + [llp, vp, vp, llp], i)):
+        f = getattr(l, name)
+        f.argtypes, f.restype = args, result
     _lib = l
     return l
 
@@ -206,6 +226,67 @@ def cuttExecuteNoAlloc(rank, dim, permutation, sizeofType, stream, idata, odata)
 
 def cuttDestroy(handle):
     return lib().cuttDestroy(ctypes.c_uint(handle))
+
+
+# The row operators (include/cutt_rows.h): device buffers are integer addresses (0 or None: NULL), the functions return the
+# result code.
+def cuttExpertRows(tokens, choices, experts, align):
+    """Rows that suffice for any choice of experts; -1 for arguments out of range."""
+    return lib().cuttExpertRows(tokens, choices, experts, align)
+
+
+def cuttExpertSortWorkspace(tokens, choices, experts):
+    """Bytes of workspace that cuttExpertSort needs."""
+    return lib().cuttExpertSortWorkspace(tokens, choices, experts)
+
+
+def cuttExpertSort(tokens, choices, firstExpert, experts, align, rows, sizeofId, stream, ids, counts, offsets, position, source,
+                   workspace=0, workspaceBytes=0):
+    return lib().cuttExpertSort(tokens, choices, firstExpert, experts, align, rows, sizeofId, stream, ids, counts, offsets, position,
+                                source, workspace, workspaceBytes)
+
+
+def cuttExpertDispatch(tokens, choices, rows, width, sizeofType, stream, position, source, x, xStride, y, yStride):
+    return lib().cuttExpertDispatch(tokens, choices, rows, width, sizeofType, stream, position, source, x, xStride, y, yStride)
+
+
+def cuttExpertDispatchBackward(tokens, choices, rows, width, type, stream, position, dy, dyStride, dx, dxStride):
+    return lib().cuttExpertDispatchBackward(tokens, choices, rows, width, type, stream, position, dy, dyStride, dx, dxStride)
+
+
+def cuttExpertCombine(tokens, choices, rows, width, type, stream, position, weights, y, yStride, out, outStride):
+    return lib().cuttExpertCombine(tokens, choices, rows, width, type, stream, position, weights, y, yStride, out, outStride)
+
+
+def cuttExpertCombineBackward(tokens, choices, rows, width, type, stream, position, source, weights, y, yStride, dout, doutStride, dy,
+                              dyStride, dweights):
+    return lib().cuttExpertCombineBackward(tokens, choices, rows, width, type, stream, position, source, weights, y, yStride, dout,
+                                           doutStride, dy, dyStride, dweights)
+
+
+def cuttPageTables(requests, pageSize, tableWidth, freeCount, tokens, stream, cached, added, freePages, tables, starts, used, slots,
+                   positions):
+    return lib().cuttPageTables(requests, pageSize, tableWidth, freeCount, tokens, stream, cached, added, freePages, tables, starts, used,
+                                slots, positions)
+
+
+def _strides(v, n):
+    """n strides as the C functions take them (an array of that kind is passed on as it is)."""
+    if v is None:
+        return v
+    if len(v) != n:
+        raise ValueError("%d strides wanted, got %d" % (n, len(v)))
+    return v if isinstance(v, ctypes.Array) else (ctypes.c_longlong * n)(*v)
+
+
+def cuttPageStore(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides):
+    return lib().cuttPageStore(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, _strides(rowStrides, 2), kCache,
+                               vCache, _strides(cacheStrides, 3))
+
+
+def cuttPageLoad(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides):
+    return lib().cuttPageLoad(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, _strides(rowStrides, 2), kCache,
+                              vCache, _strides(cacheStrides, 3))
 
 
 def get_plan_info(handle):

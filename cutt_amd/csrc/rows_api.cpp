@@ -1,0 +1,281 @@
+/*
+ * rows_api.cpp - the exported row operators (cutt_rows.h): argument checks, then one call into the
+ * kernels' layer (row_layer.h).  Pure host C++; nothing here allocates or throws.
+ */
+#include <climits>
+#include <cstdint>
+
+#include "../../include/cutt_rows.h"
+#include "row_layer.h"
+
+namespace {
+
+typedef unsigned __int128 Wide;
+
+// Byte ranges beyond this are no device buffer's (and keep the kernels' 64-bit offsets exact).
+constexpr Wide kMaxBytes = (Wide)1 << 62;
+
+// A device buffer as a call's arguments describe it: from its first to its last byte.
+struct Span {
+  uintptr_t at = 0;
+  Wide bytes = 0;
+};
+
+bool overlap(const Span& a, const Span& b) {
+  return a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes;
+}
+
+bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// `count` contiguous values of `size` bytes.
+bool values(const void* p, unsigned long long count, size_t size, Span& s) {
+  s = {(uintptr_t)p, (Wide)count * size};
+  return count == 0 || (p && aligned(p, size) && s.bytes <= kMaxBytes);
+}
+
+// Extents in elements along each of n strided axes over `width` contiguous elements.
+bool strided(const void* p, int n, const unsigned long long* extent, const long long* stride, long long least, unsigned long long width,
+             size_t size, Span& s) {
+  s = {(uintptr_t)p, 0};
+  Wide last = 0;
+  for (int i = 0; i < n; i++)
+    if (extent[i] == 0) return true;
+  if (width == 0) return true;
+  if (!p || !aligned(p, size)) return false;
+  for (int i = 0; i < n; i++) {
+    if (extent[i] == 1) continue;
+    if (stride[i] < least || stride[i] < 0) return false;
+    last += (Wide)(extent[i] - 1) * (Wide)stride[i];
+    if (last > kMaxBytes) return false;
+  }
+  s.bytes = (last + width) * size;
+  return s.bytes <= kMaxBytes;
+}
+
+bool rowsOf(const void* p, unsigned long long count, long long stride, unsigned long long width, size_t size, Span& s) {
+  return strided(p, 1, &count, &stride, (long long)width, width, size, s);
+}
+
+size_t sizeOf(cuttRowType type) { return type == CUTT_F32 ? 4 : type == CUTT_F16 || type == CUTT_BF16 ? 2 : 0; }
+
+bool opaqueSize(size_t s) { return s == 1 || s == 2 || s == 4 || s == 8; }
+
+cuttResult launched(int e) { return e == 0 ? CUTT_SUCCESS : CUTT_INTERNAL_ERROR; }
+
+// The sizes that the calls on sorted rows share.
+bool rowSizes(int tokens, int choices, int rows, int width) {
+  return tokens >= 0 && choices >= 1 && rows >= 0 && width >= 1 && (long long)tokens * choices <= INT_MAX;
+}
+
+cuttHipExpertArgs rowArgs(int tokens, int choices, int rows, int width, const int* position, const int* source, const float* weights) {
+  cuttHipExpertArgs a;
+  a.tokens = (uint32_t)tokens;
+  a.choices = (uint32_t)choices;
+  a.rows = (uint32_t)rows;
+  a.width = (uint32_t)width;
+  a.position = position;
+  a.source = source;
+  a.weights = weights;
+  return a;
+}
+
+// The weighted sum of every token's rows, which the gradient of dispatch is too.
+cuttResult sumRows(int tokens, int choices, int rows, int width, cuttRowType type, hipStream_t stream, const int* position,
+                   const float* weights, bool weighted, const void* y, long long yStride, void* out, long long outStride) {
+  const size_t size = sizeOf(type);
+  if (!size || !rowSizes(tokens, choices, rows, width)) return CUTT_INVALID_PARAMETER;
+  const unsigned long long n = (unsigned long long)tokens * choices;
+  Span p, w, from, to;
+  if (!values(position, n, 4, p) || !values(weights, weighted ? n : 0, 4, w) || !rowsOf(y, rows, yStride, width, size, from) ||
+      !rowsOf(out, tokens, outStride, width, size, to))
+    return CUTT_INVALID_PARAMETER;
+  if (overlap(to, from) || overlap(to, p) || overlap(to, w)) return CUTT_INVALID_PARAMETER;
+  if (tokens == 0) return CUTT_SUCCESS;
+  const cuttHipExpertArgs a = rowArgs(tokens, choices, rows, width, position, nullptr, weighted ? weights : nullptr);
+  return launched(cuttHipCombine(&a, (int)type, y, (uint64_t)yStride, out, (uint64_t)outStride, stream));
+}
+
+cuttResult movePages(bool load, int tokens, int heads, int width, size_t sizeofType, int pages, int pageSize, hipStream_t stream,
+                     const long long* slots, const void* k, const void* v, const long long* rowStrides, const void* kCache, const void* vCache,
+                     const long long* cacheStrides) {
+  if (tokens < 0 || heads < 1 || width < 1 || !opaqueSize(sizeofType) || pages < 0 || pageSize < 1 || !rowStrides || !cacheStrides)
+    return CUTT_INVALID_PARAMETER;
+  if ((v == nullptr) != (vCache == nullptr)) return CUTT_INVALID_PARAMETER;
+  const long long least[2] = {load ? width : 0, load ? 0 : width};  // of the rows' strides, of the caches'
+  const unsigned long long rowExtent[2] = {(unsigned long long)tokens, (unsigned long long)heads};
+  const unsigned long long cacheExtent[3] = {(unsigned long long)pages, (unsigned long long)pageSize, (unsigned long long)heads};
+  Span s, row[2], cache[2];
+  if (!values(slots, tokens, 8, s)) return CUTT_INVALID_PARAMETER;
+  const void* const rowsAt[2] = {k, v};
+  const void* const cacheAt[2] = {kCache, vCache};
+  const int tensors = v ? 2 : 1;
+  for (int i = 0; i < tensors; i++)
+    if (!strided(rowsAt[i], 2, rowExtent, rowStrides, least[0], width, sizeofType, row[i]) ||
+        !strided(cacheAt[i], 3, cacheExtent, cacheStrides, least[1], width, sizeofType, cache[i]))
+      return CUTT_INVALID_PARAMETER;
+  for (int i = 0; i < tensors; i++) {
+    for (int j = 0; j < tensors; j++)
+      if (overlap(row[i], cache[j])) return CUTT_INVALID_PARAMETER;
+    if (overlap(load ? row[i] : cache[i], s)) return CUTT_INVALID_PARAMETER;
+  }
+  if (tokens == 0 || (!load && pages == 0)) return CUTT_SUCCESS;
+  cuttHipPageArgs a;
+  a.tokens = (uint32_t)tokens;
+  a.heads = (uint32_t)heads;
+  a.width = (uint32_t)width;
+  a.elemSize = (uint32_t)sizeofType;
+  a.pages = (uint32_t)pages;
+  a.pageSize = (uint32_t)pageSize;
+  a.slots = (const int64_t*)slots;
+  for (int i = 0; i < 2; i++) {
+    a.rows[i] = const_cast<void*>(rowsAt[i]);
+    a.cache[i] = const_cast<void*>(cacheAt[i]);
+  }
+  // (the stride of an axis with one entry is never used: it may be anything)
+  a.tokenStride = tokens > 1 ? (uint64_t)rowStrides[0] : 0;
+  a.headStride = heads > 1 ? (uint64_t)rowStrides[1] : 0;
+  a.pageStride = pages > 1 ? (uint64_t)cacheStrides[0] : 0;
+  a.slotStride = pageSize > 1 ? (uint64_t)cacheStrides[1] : 0;
+  a.cacheHeadStride = heads > 1 ? (uint64_t)cacheStrides[2] : 0;
+  a.load = load;
+  return launched(cuttHipPageMove(&a, stream));
+}
+
+}  // namespace
+
+extern "C" long long cuttExpertRows(int tokens, int choices, int experts, int align) {
+  if (tokens < 0 || choices < 1 || experts < 1 || experts > CUTT_MAX_EXPERTS || align < 1) return -1;
+  const long long n = (long long)tokens * choices;
+  if (n > INT_MAX) return -1;
+  const long long rows = n + (n < experts ? n : experts) * (long long)(align - 1);
+  return rows > INT_MAX ? -1 : rows;
+}
+
+extern "C" size_t cuttExpertSortWorkspace(int tokens, int choices, int experts) {
+  if (cuttExpertRows(tokens, choices, experts, 1) < 0) return 0;
+  return cuttHipSortWorkspace((uint32_t)tokens * (uint32_t)choices, (uint32_t)experts);
+}
+
+extern "C" cuttResult cuttExpertSort(int tokens, int choices, int firstExpert, int experts, int align, int rows, size_t sizeofId,
+                                     hipStream_t stream, const void* ids, int* counts, int* offsets, int* position, int* source, void* workspace,
+                                     size_t workspaceBytes) {
+  if (cuttExpertRows(tokens, choices, experts, align) < 0 || rows < 0 || (sizeofId != 4 && sizeofId != 8)) return CUTT_INVALID_PARAMETER;
+  const unsigned long long n = (unsigned long long)tokens * choices;
+  const size_t space = cuttExpertSortWorkspace(tokens, choices, experts);
+  if (workspaceBytes < space) return CUTT_INVALID_PARAMETER;
+  Span in, out[5];
+  if (!values(ids, n, sizeofId, in) || !values(counts, experts, 4, out[0]) || !values(offsets, (unsigned long long)experts + 1, 4, out[1]) ||
+      !values(position, n, 4, out[2]) || !values(source, rows, 4, out[3]) || !values(workspace, space / 4, 4, out[4]))
+    return CUTT_INVALID_PARAMETER;
+  for (int i = 0; i < 5; i++) {
+    if (overlap(in, out[i])) return CUTT_INVALID_PARAMETER;
+    for (int j = 0; j < i; j++)
+      if (overlap(out[i], out[j])) return CUTT_INVALID_PARAMETER;
+  }
+  cuttHipSortArgs a;
+  a.n = (uint32_t)n;
+  a.firstExpert = firstExpert;
+  a.experts = (uint32_t)experts;
+  a.align = (uint32_t)align;
+  a.rows = (uint32_t)rows;
+  a.idBytes = (uint32_t)sizeofId;
+  a.ids = ids;
+  a.counts = counts;
+  a.offsets = offsets;
+  a.position = position;
+  a.source = source;
+  a.workspace = (uint32_t*)workspace;
+  return launched(cuttHipExpertSort(&a, stream));
+}
+
+extern "C" cuttResult cuttExpertDispatch(int tokens, int choices, int rows, int width, size_t sizeofType, hipStream_t stream, const int* position,
+                                         const int* source, const void* x, long long xStride, void* y, long long yStride) {
+  if (!opaqueSize(sizeofType) || !rowSizes(tokens, choices, rows, width)) return CUTT_INVALID_PARAMETER;
+  const unsigned long long n = (unsigned long long)tokens * choices;
+  Span p, s, from, to;
+  if (!values(position, n, 4, p) || !values(source, rows, 4, s) || !rowsOf(x, tokens, xStride, width, sizeofType, from) ||
+      !rowsOf(y, rows, yStride, width, sizeofType, to))
+    return CUTT_INVALID_PARAMETER;
+  if (overlap(to, from) || overlap(to, p) || overlap(to, s)) return CUTT_INVALID_PARAMETER;
+  if (rows == 0) return CUTT_SUCCESS;
+  const cuttHipExpertArgs a = rowArgs(tokens, choices, rows, width, position, source, nullptr);
+  return launched(cuttHipDispatch(&a, (uint32_t)sizeofType, x, (uint64_t)xStride, y, (uint64_t)yStride, stream));
+}
+
+extern "C" cuttResult cuttExpertDispatchBackward(int tokens, int choices, int rows, int width, cuttRowType type, hipStream_t stream,
+                                                 const int* position, const void* dy, long long dyStride, void* dx, long long dxStride) {
+  return sumRows(tokens, choices, rows, width, type, stream, position, nullptr, false, dy, dyStride, dx, dxStride);
+}
+
+extern "C" cuttResult cuttExpertCombine(int tokens, int choices, int rows, int width, cuttRowType type, hipStream_t stream, const int* position,
+                                        const float* weights, const void* y, long long yStride, void* out, long long outStride) {
+  return sumRows(tokens, choices, rows, width, type, stream, position, weights, true, y, yStride, out, outStride);
+}
+
+extern "C" cuttResult cuttExpertCombineBackward(int tokens, int choices, int rows, int width, cuttRowType type, hipStream_t stream,
+                                                const int* position, const int* source, const float* weights, const void* y, long long yStride,
+                                                const void* dout, long long doutStride, void* dy, long long dyStride, float* dweights) {
+  const size_t size = sizeOf(type);
+  if (!size || !rowSizes(tokens, choices, rows, width)) return CUTT_INVALID_PARAMETER;
+  const unsigned long long n = (unsigned long long)tokens * choices;
+  // a buffer of no entries may be null without being left out
+  const bool wantRows = dy != nullptr || rows == 0, wantWeights = dweights != nullptr || n == 0;
+  if (!wantRows && !wantWeights) return CUTT_INVALID_PARAMETER;
+  Span p, s, w, yIn, dIn, dyOut, dwOut;
+  if (!values(position, n, 4, p) || !rowsOf(dout, tokens, doutStride, width, size, dIn)) return CUTT_INVALID_PARAMETER;
+  if (wantRows && (!values(source, rows, 4, s) || !values(weights, n, 4, w) || !rowsOf(dy, rows, dyStride, width, size, dyOut)))
+    return CUTT_INVALID_PARAMETER;
+  if (wantWeights && (!values(dweights, n, 4, dwOut) || (n && !rowsOf(y, rows, yStride, width, size, yIn)))) return CUTT_INVALID_PARAMETER;
+  const Span reads[] = {p, s, w, yIn, dIn};
+  for (const Span& r : reads)
+    if (overlap(dyOut, r) || overlap(dwOut, r)) return CUTT_INVALID_PARAMETER;
+  if (overlap(dyOut, dwOut)) return CUTT_INVALID_PARAMETER;
+  if (rows == 0 && n == 0) return CUTT_SUCCESS;
+  const cuttHipExpertArgs a = rowArgs(tokens, choices, rows, width, position, source, weights);
+  return launched(cuttHipCombineBackward(&a, (int)type, y, (uint64_t)yStride, dout, (uint64_t)doutStride, rows ? dy : nullptr, (uint64_t)dyStride,
+                                         n ? dweights : nullptr, stream));
+}
+
+extern "C" cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCount, int tokens, hipStream_t stream, const int* cached,
+                                     const int* added, const int* freePages, int* tables, int* starts, int* used, long long* slots, int* positions) {
+  if (requests < 0 || pageSize < 1 || tableWidth < 1 || freeCount < 0 || tokens < 0) return CUTT_INVALID_PARAMETER;
+  const unsigned long long n = (unsigned long long)requests;
+  Span in[3], out[5];
+  if (!values(cached, n, 4, in[0]) || !values(added, n, 4, in[1]) || !values(freePages, freeCount, 4, in[2]) ||
+      !values(tables, n * (unsigned long long)tableWidth, 4, out[0]) || !values(starts, n + 1, 4, out[1]) || !values(used, 1, 4, out[2]) ||
+      !values(slots, tokens, 8, out[3]) || !values(positions, positions ? tokens : 0, 4, out[4]))
+    return CUTT_INVALID_PARAMETER;
+  for (int i = 0; i < 5; i++) {
+    for (int j = 0; j < 3; j++)
+      if (overlap(out[i], in[j])) return CUTT_INVALID_PARAMETER;
+    for (int j = 0; j < i; j++)
+      if (overlap(out[i], out[j])) return CUTT_INVALID_PARAMETER;
+  }
+  cuttHipTablesArgs a;
+  a.requests = (uint32_t)requests;
+  a.pageSize = (uint32_t)pageSize;
+  a.tableWidth = (uint32_t)tableWidth;
+  a.freeCount = (uint32_t)freeCount;
+  a.tokens = (uint32_t)tokens;
+  a.cached = cached;
+  a.added = added;
+  a.freePages = freePages;
+  a.tables = tables;
+  a.starts = starts;
+  a.used = used;
+  a.slots = (int64_t*)slots;
+  a.positions = positions;
+  return launched(cuttHipPageTables(&a, stream));
+}
+
+extern "C" cuttResult cuttPageStore(int tokens, int heads, int width, size_t sizeofType, int pages, int pageSize, hipStream_t stream,
+                                    const long long* slots, const void* k, const void* v, const long long* rowStrides, void* kCache, void* vCache,
+                                    const long long* cacheStrides) {
+  return movePages(false, tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides);
+}
+
+extern "C" cuttResult cuttPageLoad(int tokens, int heads, int width, size_t sizeofType, int pages, int pageSize, hipStream_t stream,
+                                   const long long* slots, void* k, void* v, const long long* rowStrides, const void* kCache, const void* vCache,
+                                   const long long* cacheStrides) {
+  return movePages(true, tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides);
+}
