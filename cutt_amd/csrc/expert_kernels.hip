@@ -79,78 +79,217 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
 }
 
 // ---------------------------------------------------------------------------
-// Rows to experts and back, one workgroup per row.
+// Rows to experts and back.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kRowThreads = 256;
+constexpr uint32_t kRowThreads = 256, kRowWaves = kRowThreads / 64;
 constexpr uint32_t kMaxBlocks = 1u << 22;  // (workgroups x lanes have to fit 32 bits)
 
-__device__ __forceinline__ bool rowAt(const cuttHipExpertArgs& a, uint64_t choice, uint32_t& row) {
-  row = (uint32_t)a.position[choice];
-  return row < a.rows;
-}
+// Rows without a source, which hold zeros.  Workgroup `block` of `blocks` looks at kEmptyRows rows at a time; a wavefront clears a row.
+constexpr uint32_t kEmptyRows = 16;
 
-template <typename T>
-__device__ void clearEmptyRows(const cuttHipExpertArgs& a, T* y, uint64_t stride, uint64_t first, uint64_t step) {
-  for (uint64_t r = first; r < a.rows; r += step) {
-    if (a.source[r] >= 0) continue;
-    for (uint32_t c = threadIdx.x; c < a.width; c += kRowThreads) y[r * stride + c] = T(0);
+template <typename T, int N>
+__device__ __forceinline__ void clearEmptyRows(const cuttHipExpertArgs& a, T* y, uint64_t stride, uint32_t block, uint32_t blocks) {
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  Pack<T, N> zero = {};
+  for (uint64_t first = (uint64_t)block * kEmptyRows; first < a.rows; first += (uint64_t)blocks * kEmptyRows) {
+    const uint64_t mine = first + (lane & (kEmptyRows - 1));
+    uint64_t empty = __ballot(lane < kEmptyRows && mine < a.rows && a.source[mine] < 0);
+    for (uint32_t n = 0; empty; n++) {
+      const uint32_t r = __builtin_ctzll(empty);
+      empty &= empty - 1;
+      if (n % kRowWaves != wave) continue;
+      T* const row = y + (first + r) * stride;
+      for (uint32_t c = lane * N; c < a.width; c += 64 * N) zero.store(row + min(c, a.width - N));
+    }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void dispatchKernel(cuttHipExpertArgs a, const T* x, uint64_t xStride, T* y, uint64_t yStride) {
-  for (uint64_t t = blockIdx.x; t < a.tokens; t += gridDim.x)
-    for (uint32_t k = 0; k < a.choices; k++) {
-      uint32_t row;
-      if (!rowAt(a, t * a.choices + k, row)) continue;
-      for (uint32_t c = threadIdx.x; c < a.width; c += kRowThreads) y[row * yStride + c] = x[t * xStride + c];
-    }
-  clearEmptyRows(a, y, yStride, blockIdx.x, gridDim.x);
-}
+// B choices of a token from `first` on: their rows and weights.  Lane i loads choice i, so that one load brings them all; row(i) and weight(i)
+// broadcast.  All lanes of the wavefront have to take part in making one and in the broadcasts, so the loops around them
+// are the same for the whole wavefront: lanes beyond a row's end read its last vector again and are kept from storing.
+// An absent row's number is that of a row that is there: the loads of all B can then go out back to back,
+// without branches, and what an absent one brings is not used.
+template <int B>
+struct Choices {
+  uint32_t laneRow;
+  float laneWeight;
+  uint32_t there;  // bit i: choice i has a row
 
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void combineKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, T* out, uint64_t outStride) {
-  for (uint64_t t = blockIdx.x; t < a.tokens; t += gridDim.x)
-    for (uint32_t c = threadIdx.x; c < a.width; c += kRowThreads) {
-      float sum = 0;
-      for (uint32_t k = 0; k < a.choices; k++) {
-        uint32_t row;
-        if (!rowAt(a, t * a.choices + k, row)) continue;
-        const float v = (float)y[row * yStride + c];
-        sum += a.weights ? a.weights[t * a.choices + k] * v : v;
+  __device__ __forceinline__ Choices(const cuttHipExpertArgs& a, uint32_t token, uint32_t first) {
+    const uint32_t i = threadIdx.x & (B - 1);
+    const uint64_t at = (uint64_t)token * a.choices + min(first + i, a.choices - 1);
+    laneRow = (uint32_t)a.position[at];
+    laneWeight = 1.0f;
+    if (a.weights) laneWeight = a.weights[at];
+    const bool ok = first + i < a.choices && laneRow < a.rows;
+    there = (uint32_t)__ballot(ok) & ((1u << B) - 1);
+    const uint32_t some = __builtin_amdgcn_readlane(laneRow, there ? __builtin_ctz(there) : 0);
+    if (!ok) laneRow = some, laneWeight = 0.0f;
+  }
+  __device__ __forceinline__ bool has(int i) const { return there >> i & 1; }
+  __device__ __forceinline__ uint64_t row(int i) const { return (uint32_t)__builtin_amdgcn_readlane(laneRow, i); }
+  __device__ __forceinline__ float weight(int i) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(laneWeight), i)); }
+};
+
+// The workgroup's wavefronts share a row's columns: wavefront w takes the columns w * 64 * N, (w + kRowWaves) * 64 * N, ...
+__device__ __forceinline__ uint32_t waveOfGroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// A workgroup reads a token's row once and stores it to every row that the token goes to; the last workgroups clear the empty rows.
+// Rows are bytes here: any element size, any alignment.
+template <int N>
+__global__ __launch_bounds__(kRowThreads) void dispatchKernel(cuttHipExpertArgs a, const uint8_t* x, uint64_t xStride, uint8_t* y, uint64_t yStride,
+                                                              uint32_t tokenBlocks) {
+  constexpr int U = N == 1 ? 1 : 2;  // vectors a lane keeps
+  if (blockIdx.x >= tokenBlocks) {
+    clearEmptyRows<uint8_t, N>(a, y, yStride, blockIdx.x - tokenBlocks, gridDim.x - tokenBlocks);
+    return;
+  }
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t t = blockIdx.x; t < a.tokens; t += tokenBlocks) {
+    const uint8_t* const from = x + t * xStride;
+    const Choices<8> begin(a, t, 0);
+    for (uint32_t col = waveOfGroup() * 64 * N; col < a.width; col += kRowThreads * N * U) {
+      Pack<uint8_t, N> v[U];
+      uint32_t at[U];
+      bool mine[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const uint32_t base = col + u * kRowThreads * N + lane * N;
+        mine[u] = base < a.width;
+        at[u] = min(base, a.width - N);
+        v[u].load(from + at[u]);
       }
-      out[t * outStride + c] = (T)sum;
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
-                                                                     T* dy, uint64_t dyStride, float* dweights) {
-  __shared__ float part[kRowThreads];
-  for (uint64_t t = blockIdx.x; t < a.tokens; t += gridDim.x)
-    for (uint32_t k = 0; k < a.choices; k++) {
-      uint32_t row;
-      const bool there = rowAt(a, t * a.choices + k, row);
-      float sum = 0;
-      if (there)
-        for (uint32_t c = threadIdx.x; c < a.width; c += kRowThreads) {
-          const float g = (float)dout[t * doutStride + c];
-          if (dweights) sum += g * (float)y[row * yStride + c];
-          if (dy) dy[row * dyStride + c] = (T)(a.weights[t * a.choices + k] * g);
+      auto put = [&](const Choices<8>& ch) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          if (!ch.has(i)) continue;
+          uint8_t* const to = y + ch.row(i) * yStride;
+#pragma unroll
+          for (int u = 0; u < U; u++)
+            if (mine[u]) v[u].store(to + at[u]);
         }
-      if (!dweights) continue;
-      part[threadIdx.x] = sum;
-      for (uint32_t n = kRowThreads / 2; n; n /= 2) {
-        __syncthreads();
-        if (threadIdx.x < n) part[threadIdx.x] += part[threadIdx.x + n];
+      };
+      put(begin);
+      for (uint32_t first = 8; first < a.choices; first += 8) put(Choices<8>(a, t, first));
+    }
+  }
+}
+
+// A workgroup sums a token's rows, 16 bytes of each per lane.
+template <typename T, int N, int B>
+__global__ __launch_bounds__(kRowThreads) void combineKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, T* out, uint64_t outStride) {
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const Choices<B> begin(a, t, 0);
+    for (uint32_t col = waveOfGroup() * 64 * N; col < a.width; col += kRowThreads * N) {
+      const uint32_t base = col + lane * N, c = min(base, a.width - N);
+      float sum[N] = {};
+      auto add = [&](const Choices<B>& ch) __attribute__((always_inline)) {
+        if (!ch.there) return;
+        Pack<T, N> v[B];
+#pragma unroll
+        for (int i = 0; i < B; i++) v[i].load(y + ch.row(i) * yStride + c);
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+          v[i].zeroUnless(ch.has(i));
+          const float w = ch.weight(i);
+#pragma unroll
+          for (int e = 0; e < N; e++) sum[e] = fmaf(w, (float)v[i].get(e), sum[e]);
+        }
+      };
+      add(begin);
+      for (uint32_t first = B; first < a.choices; first += B) add(Choices<B>(a, t, first));
+      Pack<T, N> o;
+#pragma unroll
+      for (int e = 0; e < N; e++) o.set(e, (T)sum[e]);
+      if (base < a.width) o.store(out + t * outStride + c);
+    }
+  }
+}
+
+// Sums of B values over the wavefront: afterwards lane l holds the sum of value l / (64 / B).  Each step halves what a lane still holds.
+template <int B>
+__device__ __forceinline__ float sumOverWave(float (&v)[B]) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t half = 32;
+#pragma unroll
+  for (int n = B / 2; n >= 1; n /= 2, half /= 2) {
+    const bool upper = lane & half;
+#pragma unroll
+    for (int i = 0; i < n; i++) {
+      const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+      v[i] = keep + __shfl_xor(give, half);
+    }
+  }
+  float sum = v[0];
+  for (; half >= 1; half /= 2) sum += __shfl_xor(sum, half);
+  return sum;
+}
+
+// A workgroup takes a token: its gradient row is multiplied into the rows it came from, and with them.  The last workgroups clear the empty rows.
+template <typename T, int N, int B, bool ROWS, bool WEIGHTS>
+__global__ __launch_bounds__(kRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
+                                                                     T* dy, uint64_t dyStride, float* dweights, uint32_t tokenBlocks) {
+  __shared__ float part[kRowWaves][B];
+  if (ROWS && blockIdx.x >= tokenBlocks) {
+    clearEmptyRows<T, N>(a, dy, dyStride, blockIdx.x - tokenBlocks, gridDim.x - tokenBlocks);
+    return;
+  }
+  const uint32_t wave = waveOfGroup(), lane = threadIdx.x & 63;
+  for (uint32_t t = blockIdx.x; t < a.tokens; t += tokenBlocks)
+    for (uint32_t first = 0; first < a.choices; first += B) {
+      const Choices<B> ch(a, t, first);
+      float dot[B] = {};
+      for (uint32_t col = waveOfGroup() * 64 * N; ch.there && col < a.width; col += kRowThreads * N) {
+        const uint32_t base = col + lane * N, c = min(base, a.width - N);
+        Pack<T, N> g, v[B];
+        g.load(dout + t * doutStride + c);
+        if (WEIGHTS)
+#pragma unroll
+          for (int i = 0; i < B; i++) v[i].load(y + ch.row(i) * yStride + c);
+        Pack<T, N> once = g;
+        if (WEIGHTS && c != base)  // columns that the vector before it, or its row's last vector, has already counted
+#pragma unroll
+          for (int e = 0; e < N; e++)
+            if (c + e < base) {
+              once.set(e, T(0));
+#pragma unroll
+              for (int i = 0; i < B; i++) v[i].set(e, T(0));
+            }
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+          if (WEIGHTS)
+#pragma unroll
+            for (int e = 0; e < N; e++) dot[i] = fmaf((float)once.get(e), (float)v[i].get(e), dot[i]);
+          if (ROWS && ch.has(i)) {
+            const float w = ch.weight(i);
+            T* const to = dy + ch.row(i) * dyStride + c;
+            Pack<T, N> o;
+#pragma unroll
+            for (int e = 0; e < N; e++) o.set(e, (T)(w * (float)g.get(e)));
+            if (base < a.width) o.store(to);
+          }
+        }
       }
-      if (threadIdx.x == 0) dweights[t * a.choices + k] = part[0];
+      if (!WEIGHTS) continue;
+#pragma unroll
+      for (int i = 0; i < B; i++) dot[i] = ch.has(i) ? dot[i] : 0.0f;
+      const float sum = sumOverWave(dot);
+      if (lane % (64 / B) == 0) part[wave][lane / (64 / B)] = sum;
+      __syncthreads();
+      if (threadIdx.x < B && first + threadIdx.x < a.choices) {
+        float all = 0;
+        for (uint32_t w = 0; w < kRowWaves; w++) all += part[w][threadIdx.x];
+        dweights[(uint64_t)t * a.choices + first + threadIdx.x] = all;
+      }
       __syncthreads();
     }
-  if (dy) clearEmptyRows(a, dy, dyStride, blockIdx.x, gridDim.x);
 }
 
-uint32_t blocksFor(uint64_t n) { return (uint32_t)(n < 1 ? 1 : n < kMaxBlocks ? n : kMaxBlocks); }
+constexpr uint64_t kMaxPiece = 1u << 30;
+
+uint32_t blocksFor(uint64_t n) { return (uint32_t)(n < kMaxBlocks ? n : kMaxBlocks); }
+uint32_t emptyBlocks(uint32_t rows) { return blocksFor((rows + (uint64_t)kEmptyRows - 1) / kEmptyRows); }
 
 }  // namespace
 
@@ -163,27 +302,53 @@ extern "C" int cuttHipExpertSort(const cuttHipSortArgs* a, void* stream) {
 }
 
 extern "C" int cuttHipDispatch(const cuttHipExpertArgs* a, uint32_t elemSize, const void* x, uint64_t xStride, void* y, uint64_t yStride, void* stream) {
-  const dim3 grid(blocksFor(a->tokens > a->rows ? a->tokens : a->rows));
-  switch (elemSize) {
-    case 1: return launchRows(dispatchKernel<uint8_t>, grid, kRowThreads, 0, stream, *a, (const uint8_t*)x, xStride, (uint8_t*)y, yStride);
-    case 2: return launchRows(dispatchKernel<uint16_t>, grid, kRowThreads, 0, stream, *a, (const uint16_t*)x, xStride, (uint16_t*)y, yStride);
-    case 4: return launchRows(dispatchKernel<uint32_t>, grid, kRowThreads, 0, stream, *a, (const uint32_t*)x, xStride, (uint32_t*)y, yStride);
-    default: return launchRows(dispatchKernel<uint64_t>, grid, kRowThreads, 0, stream, *a, (const uint64_t*)x, xStride, (uint64_t*)y, yStride);
+  const uint64_t bytes = (uint64_t)a->width * elemSize;
+  const uint32_t tokenBlocks = blocksFor(a->tokens);
+  const dim3 grid(tokenBlocks + emptyBlocks(a->rows));
+  // (a launch's offsets in a row have 32 bits: longer rows go piece by piece)
+  for (uint64_t at = 0; at < bytes; at += kMaxPiece) {
+    cuttHipExpertArgs b = *a;
+    b.width = (uint32_t)(bytes - at < kMaxPiece ? bytes - at : kMaxPiece);
+    auto kernel = b.width >= 16 ? dispatchKernel<16> : dispatchKernel<1>;
+    if (int e = launchRows(kernel, grid, kRowThreads, 0, stream, b, (const uint8_t*)x + at, xStride * elemSize, (uint8_t*)y + at, yStride * elemSize, tokenBlocks))
+      return e;
   }
+  return 0;
 }
 
 namespace {
 
+// Calls f with the elements per vector and the choices taken at once as constants.
+template <typename T, typename F>
+int byShape(const cuttHipExpertArgs* a, F f) {
+  constexpr int N = 16 / sizeof(T);
+  if (a->width < N) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  const std::integral_constant<int, N> n;
+  if (a->choices > 4) return f(n, std::integral_constant<int, 8>{});
+  if (a->choices > 2) return f(n, std::integral_constant<int, 4>{});
+  if (a->choices > 1) return f(n, std::integral_constant<int, 2>{});
+  return f(n, std::integral_constant<int, 1>{});
+}
+
 template <typename T>
 int combine(const cuttHipExpertArgs* a, const void* y, uint64_t yStride, void* out, uint64_t outStride, void* stream) {
-  return launchRows(combineKernel<T>, blocksFor(a->tokens), kRowThreads, 0, stream, *a, (const T*)y, yStride, (T*)out, outStride);
+  return byShape<T>(a, [&](auto n, auto b) {
+    return launchRows(combineKernel<T, n, b>, blocksFor(a->tokens), kRowThreads, 0, stream, *a, (const T*)y, yStride, (T*)out, outStride);
+  });
 }
 
 template <typename T>
 int combineBackward(const cuttHipExpertArgs* a, const void* y, uint64_t yStride, const void* dout, uint64_t doutStride, void* dy, uint64_t dyStride,
                     float* dweights, void* stream) {
-  return launchRows(combineBackwardKernel<T>, blocksFor(a->tokens > a->rows ? a->tokens : a->rows), kRowThreads, 0, stream, *a, (const T*)y, yStride,
-                (const T*)dout, doutStride, (T*)dy, dyStride, dweights);
+  const uint32_t tokenBlocks = blocksFor(a->tokens);
+  return byShape<T>(a, [&](auto n, auto b) {
+    auto go = [&](auto kernel, uint32_t blocks) {
+      return launchRows(kernel, tokenBlocks + blocks, kRowThreads, 0, stream, *a, (const T*)y, yStride, (const T*)dout, doutStride, (T*)dy, dyStride, dweights, tokenBlocks);
+    };
+    if (!dy) return go(combineBackwardKernel<T, n, b, false, true>, 0);
+    if (!dweights) return go(combineBackwardKernel<T, n, b, true, false>, emptyBlocks(a->rows));
+    return go(combineBackwardKernel<T, n, b, true, true>, emptyBlocks(a->rows));
+  });
 }
 
 }  // namespace
