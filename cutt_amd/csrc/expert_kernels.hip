@@ -10,9 +10,21 @@ using namespace cutt;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Sort: one workgroup counts, adds up and places.
+// Sort.  A stable counting sort: each workgroup places a stretch of neighbouring choices.  It needs to know how many choices each expert has in
+// all and before the stretch.  Few choices: every workgroup counts all of them (COUNTED = false, one launch).  Many: a first
+// launch counts stretch by stretch into the workspace, [stretch][expert], and a workgroup adds the columns up.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr uint32_t kSortItems = 4;  // choices that a lane places at a time
+constexpr uint32_t kSortPart = kSortThreads * kSortItems;
+constexpr uint32_t kSortGroups = 256;       // at most
+constexpr uint32_t kCountAll = 16384;       // choices that every workgroup counts for itself
+
+struct SortPlan {
+  uint32_t stretch;  // choices per workgroup, a multiple of kSortPart
+  uint32_t groups;
+  bool counted;
+};
 
 // The expert of choice i among the `experts`, or `experts` if it is none of them.
 template <typename Id>
@@ -21,7 +33,20 @@ __device__ __forceinline__ uint32_t expertOf(const cuttHipSortArgs& a, uint32_t 
   return e < a.experts ? (uint32_t)e : a.experts;
 }
 
-// Lanes of the wavefront whose key is this lane's.
+template <typename Id>
+__global__ __launch_bounds__(kSortThreads) void expertCountKernel(cuttHipSortArgs a, uint32_t stretch) {
+  extern __shared__ uint32_t count[];  // [experts + 1]
+  const uint32_t E = a.experts;
+  for (uint32_t e = threadIdx.x; e <= E; e += kSortThreads) count[e] = 0;
+  __syncthreads();
+  const uint32_t from = blockIdx.x * stretch, to = min(from + stretch, a.n);
+#pragma unroll 4
+  for (uint32_t i = from + threadIdx.x; i < to; i += kSortThreads) atomicAdd(&count[expertOf<Id>(a, i)], 1u);
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < E; e += kSortThreads) a.workspace[(uint64_t)blockIdx.x * E + e] = count[e];
+}
+
+// Lanes of the wavefront whose key is this lane's; keys have `bits` bits.
 __device__ __forceinline__ uint64_t sameKey(uint32_t key, uint32_t bits) {
   uint64_t same = ~0ull;
   for (uint32_t b = 0; b < bits; b++) {
@@ -32,50 +57,147 @@ __device__ __forceinline__ uint64_t sameKey(uint32_t key, uint32_t bits) {
   return same;
 }
 
-template <typename Id>
-__global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs a) {
+template <typename Id, bool COUNTED>
+__global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs a, uint32_t stretch) {
   extern __shared__ uint32_t lds[];
-  uint32_t* const next = lds;                     // [experts + 1] row of an expert's next choice
-  uint32_t* const seen = lds + a.experts + 1;     // [waves][experts + 1]
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = a.experts;
-  for (uint32_t i = tid; i <= E; i += kSortThreads) next[i] = 0;
-  __syncthreads();
-  for (uint32_t i = tid; i < a.n; i += kSortThreads) atomicAdd(&next[expertOf<Id>(a, i)], 1u);
-  __syncthreads();
-  if (tid == 0) {
-    uint32_t at = 0;
-    for (uint32_t e = 0; e < E; e++) {
-      const uint32_t c = next[e];
-      a.counts[e] = (int32_t)c;
-      a.offsets[e] = (int32_t)at;
-      next[e] = at;
-      at += (c + a.align - 1) / a.align * a.align;
+  const uint32_t E = a.experts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t* const next = lds;                    // [E + 1] choices before the stretch, then the row of an expert's next choice
+  uint32_t* const all = next + E + 1;            // [E + 1] choices in all, then the row behind an expert's last choice
+  uint32_t* const start = all + E + 1;           // [E + 1] an expert's first row
+  uint32_t* const seen = start + E + 1;          // [waves][E + 1]
+  __shared__ uint32_t waveSum[kSortWaves];
+  const uint32_t from = blockIdx.x * stretch, to = min(from + stretch, a.n);
+
+  if constexpr (COUNTED) {
+    // The threads share the table: thread tid adds up every `share`-th stretch of expert tid % E (E <= kSortThreads), or experts
+    // tid, tid + kSortThreads of all.
+    for (uint32_t e = tid; e <= E; e += kSortThreads) next[e] = all[e] = 0;
+    __syncthreads();
+    const uint32_t share = E <= kSortThreads ? kSortThreads / E : 1, part = tid / E;
+    if (part < share || share == 1)
+      for (uint32_t e = share == 1 ? tid : tid - part * E; e < E; e += kSortThreads) {
+        uint32_t before = 0, sum = 0;
+#pragma unroll 8
+        for (uint32_t g = share == 1 ? 0 : part; g < gridDim.x; g += share) {
+          const uint32_t c = a.workspace[(uint64_t)g * E + e];
+          sum += c;
+          before += g < blockIdx.x ? c : 0;
+        }
+        atomicAdd(&next[e], before);
+        atomicAdd(&all[e], sum);
+      }
+  } else {
+    for (uint32_t e = tid; e <= E; e += kSortThreads) next[e] = all[e] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = tid; i < a.n; i += kSortThreads) {
+      const uint32_t e = expertOf<Id>(a, i);
+      atomicAdd(&all[e], 1u);
+      if (i < from) atomicAdd(&next[e], 1u);
     }
-    a.offsets[E] = (int32_t)at;
   }
-  for (uint32_t r = tid; r < a.rows; r += kSortThreads) a.source[r] = -1;
+  __syncthreads();
+
+  // Experts' first rows: thread tid adds up experts 2 tid and 2 tid + 1 (CUTT_MAX_EXPERTS = 2 * kSortThreads).
+  {
+    uint32_t padded[2], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const uint32_t e = 2 * tid + j;
+      padded[j] = e < E ? (all[e] + a.align - 1) / a.align * a.align : 0;
+      sum += padded[j];
+    }
+    uint32_t upTo = sum;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) {
+      const uint32_t x = __shfl_up(upTo, d);
+      if (lane >= d) upTo += x;
+    }
+    if (lane == 63) waveSum[wave] = upTo;
+    __syncthreads();
+    uint32_t at = upTo - sum;
+    for (uint32_t w = 0; w < wave; w++) at += waveSum[w];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const uint32_t e = 2 * tid + j;
+      if (e <= E) start[e] = at;
+      if (e < E) {
+        const uint32_t c = all[e];
+        if (blockIdx.x == 0) a.counts[e] = (int32_t)c;
+        all[e] = at + c;
+        next[e] += at;
+      }
+      if (e <= E && blockIdx.x == 0) a.offsets[e] = (int32_t)at;
+      at += padded[j];
+    }
+    if (2 * tid + 2 == E) {  // (the sum behind the last expert falls to nobody's pair when E = 2 * kSortThreads)
+      start[E] = at;
+      if (blockIdx.x == 0) a.offsets[E] = (int32_t)at;
+    }
+  }
+  __syncthreads();
+
+  // Rows without a choice: behind every expert's last one, and behind all experts.
+  for (uint32_t e = blockIdx.x * kSortWaves + wave; e < E; e += gridDim.x * kSortWaves)
+    for (uint64_t r = (uint64_t)all[e] + lane; r < start[e + 1] && r < a.rows; r += 64) a.source[r] = -1;
+  for (uint64_t r = (uint64_t)start[E] + blockIdx.x * kSortThreads + tid; r < a.rows; r += (uint64_t)gridDim.x * kSortThreads) a.source[r] = -1;
+
+  // The stretch, part by part.  A wavefront's choices of a part are neighbours, so that an expert's rows follow the order of the
+  // wavefronts, in a wavefront that of its steps, and in a step that of the lanes.
   const uint32_t bits = 32 - __builtin_clz(E);
-  for (uint32_t base = 0; base < a.n; base += kSortThreads) {
+  uint32_t* const mine = seen + wave * (E + 1);
+  for (uint64_t part = from; part < to; part += kSortPart) {
+    for (uint32_t e = lane; e <= E; e += 64) mine[e] = 0;
+    __builtin_amdgcn_wave_barrier();
+    uint32_t expert[kSortItems], rank[kSortItems];
+#pragma unroll
+    for (uint32_t j = 0; j < kSortItems; j++) {
+      const uint64_t i = part + (wave * kSortItems + j) * 64 + lane;
+      expert[j] = i < to ? expertOf<Id>(a, (uint32_t)i) : E;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kSortItems; j++) {
+      const uint64_t same = sameKey(expert[j], bits);
+      const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+      const uint32_t before = mine[expert[j]];  // (the wavefront's lanes all read, then one lane per expert writes)
+      __builtin_amdgcn_wave_barrier();
+      rank[j] = before + below;
+      if (below == 0) mine[expert[j]] = before + __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+    }
     __syncthreads();
-    for (uint32_t i = tid; i < kSortWaves * (E + 1); i += kSortThreads) seen[i] = 0;
+    for (uint32_t e = tid; e < E; e += kSortThreads) {
+      uint32_t at = next[e];
+#pragma unroll
+      for (uint32_t w = 0; w < kSortWaves; w++) {
+        const uint32_t c = seen[w * (E + 1) + e];
+        seen[w * (E + 1) + e] = at;
+        at += c;
+      }
+      next[e] = at;
+    }
     __syncthreads();
-    const uint32_t i = base + tid;
-    const uint32_t e = i < a.n ? expertOf<Id>(a, i) : E;
-    const uint64_t same = sameKey(e, bits);
-    const uint32_t rank = __popcll(same & ((1ull << lane) - 1));
-    if (rank == 0) seen[wave * (E + 1) + e] = __popcll(same);
-    __syncthreads();
-    uint32_t row = next[e] + rank;
-    for (uint32_t w = 0; w < wave; w++) row += seen[w * (E + 1) + e];
-    if (i < a.n) {
-      const bool there = e < E && row < a.rows;
+#pragma unroll
+    for (uint32_t j = 0; j < kSortItems; j++) {
+      const uint64_t i = part + (wave * kSortItems + j) * 64 + lane;
+      if (i >= to) continue;
+      const uint32_t row = mine[expert[j]] + rank[j];
+      const bool there = expert[j] < E && row < a.rows;
       a.position[i] = there ? (int32_t)row : -1;
       if (there) a.source[row] = (int32_t)i;
     }
     __syncthreads();
-    for (uint32_t x = tid; x < E; x += kSortThreads)
-      for (uint32_t w = 0; w < kSortWaves; w++) next[x] += seen[w * (E + 1) + x];
   }
+}
+
+SortPlan planSort(uint32_t n) {
+  SortPlan p;
+  const uint64_t parts = n ? ((uint64_t)n + kSortPart - 1) / kSortPart : 1;
+  p.counted = n > kCountAll;
+  const uint64_t perGroup = (parts + kSortGroups - 1) / kSortGroups;
+  p.stretch = (uint32_t)(perGroup * kSortPart);
+  p.groups = (uint32_t)((parts + perGroup - 1) / perGroup);
+  return p;
 }
 
 // ---------------------------------------------------------------------------
@@ -293,12 +415,26 @@ uint32_t emptyBlocks(uint32_t rows) { return blocksFor((rows + (uint64_t)kEmptyR
 
 }  // namespace
 
-extern "C" size_t cuttHipSortWorkspace(uint32_t, uint32_t) { return 0; }
+extern "C" size_t cuttHipSortWorkspace(uint32_t n, uint32_t experts) {
+  const SortPlan p = planSort(n);
+  return p.counted ? (size_t)p.groups * experts * 4 : 0;
+}
+
+namespace {
+
+template <typename Id>
+int sortBy(const cuttHipSortArgs* a, void* stream) {
+  const SortPlan p = planSort(a->n);
+  const size_t perExpert = (size_t)(a->experts + 1) * 4, lds = (3 + kSortWaves) * perExpert;
+  if (!p.counted) return launchRows(expertSortKernel<Id, false>, p.groups, kSortThreads, lds, stream, *a, p.stretch);
+  if (int e = launchRows(expertCountKernel<Id>, p.groups, kSortThreads, perExpert, stream, *a, p.stretch)) return e;
+  return launchRows(expertSortKernel<Id, true>, p.groups, kSortThreads, lds, stream, *a, p.stretch);
+}
+
+}  // namespace
 
 extern "C" int cuttHipExpertSort(const cuttHipSortArgs* a, void* stream) {
-  const size_t lds = (size_t)(kSortWaves + 1) * (a->experts + 1) * 4;
-  return a->idBytes == 8 ? launchRows(expertSortKernel<int64_t>, 1, kSortThreads, lds, stream, *a)
-                         : launchRows(expertSortKernel<int32_t>, 1, kSortThreads, lds, stream, *a);
+  return a->idBytes == 8 ? sortBy<int64_t>(a, stream) : sortBy<int32_t>(a, stream);
 }
 
 extern "C" int cuttHipDispatch(const cuttHipExpertArgs* a, uint32_t elemSize, const void* x, uint64_t xStride, void* y, uint64_t yStride, void* stream) {

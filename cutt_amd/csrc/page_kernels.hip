@@ -9,45 +9,171 @@ using namespace cutt;
 
 namespace {
 
-constexpr uint32_t kThreads = 256, kMaxBlocks = 1u << 22;
+constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 
 // Sums of lengths stop at 2^31 - 1.  (Capping a sum of such numbers is associative, so the order of a scan does not matter.)
 __device__ __forceinline__ uint32_t capped(uint32_t a, uint32_t b) { return min(a + b, 0x7fffffffu); }
 
 __device__ __forceinline__ uint32_t pagesFor(uint32_t tokens, uint32_t pageSize) { return (tokens + pageSize - 1) / pageSize; }
 
-// One thread goes through the requests.
-__global__ void pageTablesKernel(cuttHipTablesArgs a) {
-  uint32_t start = 0, taken = 0;
-  for (uint32_t b = 0; b < a.requests; b++) {
-    const uint32_t cached = max(a.cached[b], 0), added = max(a.added[b], 0);
-    const uint32_t owned = pagesFor(cached, a.pageSize), want = pagesFor(capped(cached, added), a.pageSize);
-    a.starts[b] = (int32_t)start;
-    for (uint32_t j = owned; j < want && j < a.tableWidth; j++) {
-      const uint64_t at = (uint64_t)taken + (j - owned);
-      a.tables[(uint64_t)b * a.tableWidth + j] = at < a.freeCount ? a.freePages[at] : -1;
-    }
-    start = capped(start, added);
-    taken = capped(taken, want - owned);
+// What the tables need to know of a request.
+struct Request {
+  uint32_t cached, added, owned, need;
+  __device__ __forceinline__ Request(const cuttHipTablesArgs& a, uint32_t b) {
+    cached = max(a.cached[b], 0);
+    added = max(a.added[b], 0);
+    owned = min(pagesFor(cached, a.pageSize), a.tableWidth);
+    need = min(pagesFor(capped(cached, added), a.pageSize), a.tableWidth) - owned;
   }
-  a.starts[a.requests] = (int32_t)start;
-  a.used[0] = (int32_t)taken;
+};
+
+// ---------------------------------------------------------------------------
+// Page tables.  A workgroup scans the lengths of up to kScan requests: how many new tokens and new pages there are before each.
+// Tokens and pages then find their request by a search in LDS.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kPerThread = 8, kScan = kThreads * kPerThread;
+
+struct Scan {
+  uint32_t tokens[kScan + 1];  // before request i of the scan; behind the last one, all
+  uint32_t pages[kScan + 1];
+  uint32_t waveTokens[kWaves], wavePages[kWaves];
+};
+
+// Fills s for the requests first .. first + n - 1, whose predecessors have the given numbers of tokens and pages.  All threads of the workgroup.
+__device__ __forceinline__ void scanRequests(const cuttHipTablesArgs& a, uint32_t first, uint32_t n, uint32_t tokensBefore, uint32_t pagesBefore, Scan& s) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t each = (n + kThreads - 1) / kThreads, from = threadIdx.x * each;  // consecutive requests of this thread
+  uint32_t tokens[kPerThread], pages[kPerThread], allTokens = 0, allPages = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kPerThread; i++) {
+    tokens[i] = pages[i] = 0;
+    if (i < each && from + i < n) {
+      const Request r(a, first + from + i);
+      tokens[i] = r.added;
+      pages[i] = r.need;
+    }
+    allTokens = capped(allTokens, tokens[i]);
+    allPages = capped(allPages, pages[i]);
+  }
+  uint32_t upToTokens = allTokens, upToPages = allPages;  // inclusive over the wavefront
+#pragma unroll
+  for (uint32_t d = 1; d < 64; d *= 2) {
+    const uint32_t t = __shfl_up(upToTokens, d), p = __shfl_up(upToPages, d);
+    if (lane >= d) {
+      upToTokens = capped(upToTokens, t);
+      upToPages = capped(upToPages, p);
+    }
+  }
+  if (lane == 63) {
+    s.waveTokens[wave] = upToTokens;
+    s.wavePages[wave] = upToPages;
+  }
+  uint32_t t = __shfl_up(upToTokens, 1), p = __shfl_up(upToPages, 1);
+  if (lane == 0) t = p = 0;
+  __syncthreads();
+  for (uint32_t w = 0; w < wave; w++) {
+    t = capped(t, s.waveTokens[w]);
+    p = capped(p, s.wavePages[w]);
+  }
+  t = capped(t, tokensBefore);
+  p = capped(p, pagesBefore);
+#pragma unroll
+  for (uint32_t i = 0; i < kPerThread; i++) {
+    if (i < each && from + i < n) {
+      s.tokens[from + i] = t;
+      s.pages[from + i] = p;
+    }
+    t = capped(t, tokens[i]);
+    p = capped(p, pages[i]);
+  }
+  if (threadIdx.x == kThreads - 1) {  // (its requests are the last ones, or there are none behind the last)
+    s.tokens[n] = t;
+    s.pages[n] = p;
+  }
+  __syncthreads();
+}
+
+// The last request whose number is not above x; sums[0] <= x < sums[n].
+__device__ __forceinline__ uint32_t requestOf(const uint32_t* sums, uint32_t n, uint32_t x) {
+  uint32_t lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (sums[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int32_t freePage(const cuttHipTablesArgs& a, uint32_t at) { return at < a.freeCount ? a.freePages[at] : -1; }
+
+// Writes the new entries of the scanned requests' tables; `thread` of `threads` takes every `threads`-th page.
+__device__ __forceinline__ void assignPages(const cuttHipTablesArgs& a, uint32_t first, uint32_t n, const Scan& s, uint32_t thread, uint32_t threads) {
+  for (uint64_t at = (uint64_t)s.pages[0] + thread; at < s.pages[n]; at += threads) {
+    const uint32_t i = requestOf(s.pages, n, (uint32_t)at), b = first + i;
+    const uint32_t j = Request(a, b).owned + ((uint32_t)at - s.pages[i]);
+    if (j < a.tableWidth) a.tables[(uint64_t)b * a.tableWidth + j] = freePage(a, (uint32_t)at);  // (always, unless sums were capped)
+  }
+}
+
+// The requests are few enough for one scan: every workgroup makes it for itself and takes its share of the tokens and the pages.  A new token's page
+// comes from the free list, not from the table, whose new entries another workgroup may still have to write.
+__global__ __launch_bounds__(kThreads) void pageTablesKernel(cuttHipTablesArgs a) {
+  __shared__ Scan s;
+  const uint32_t n = a.requests, thread = blockIdx.x * kThreads + threadIdx.x, threads = gridDim.x * kThreads;
+  scanRequests(a, 0, n, 0, 0, s);
+  if (blockIdx.x == 0) {
+    for (uint32_t b = threadIdx.x; b <= n; b += kThreads) a.starts[b] = (int32_t)s.tokens[b];
+    if (threadIdx.x == 0) a.used[0] = (int32_t)s.pages[n];
+  }
+  for (uint64_t i = thread; i < a.tokens; i += threads) {
+    int64_t slot = -1;
+    int32_t position = -1;
+    if (i < s.tokens[n]) {
+      const uint32_t b = requestOf(s.tokens, n, (uint32_t)i);
+      const Request r(a, b);
+      const uint32_t p = capped(r.cached, (uint32_t)i - s.tokens[b]), j = p / a.pageSize;
+      position = (int32_t)p;
+      if (j < a.tableWidth) {
+        const int32_t page = j < r.owned ? a.tables[(uint64_t)b * a.tableWidth + j] : freePage(a, capped(s.pages[b], j - r.owned));
+        if (page >= 0) slot = (int64_t)page * a.pageSize + (p - j * a.pageSize);
+      }
+    }
+    a.slots[i] = slot;
+    if (a.positions) a.positions[i] = position;
+  }
+  assignPages(a, 0, n, s, thread, threads);
+}
+
+// Any number of requests: one workgroup scans them part by part and writes the tables, a second launch looks the tokens up.
+__global__ __launch_bounds__(kThreads) void pageTablesLongKernel(cuttHipTablesArgs a) {
+  __shared__ Scan s;
+  uint32_t tokens = 0, pages = 0;
+  for (uint32_t first = 0; first < a.requests; first += kScan) {
+    const uint32_t n = min(a.requests - first, kScan);
+    scanRequests(a, first, n, tokens, pages, s);
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) a.starts[first + i] = (int32_t)s.tokens[i];
+    assignPages(a, first, n, s, threadIdx.x, kThreads);
+    tokens = s.tokens[n];
+    pages = s.pages[n];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    a.starts[a.requests] = (int32_t)tokens;
+    a.used[0] = (int32_t)pages;
+  }
 }
 
 __global__ __launch_bounds__(kThreads) void pageSlotsKernel(cuttHipTablesArgs a) {
+  const uint32_t* const starts = reinterpret_cast<const uint32_t*>(a.starts);
+  const uint32_t all = starts[a.requests];
   for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < a.tokens; i += (uint64_t)gridDim.x * kThreads) {
     int64_t slot = -1;
     int32_t position = -1;
-    if (i < (uint32_t)a.starts[a.requests]) {
-      uint32_t lo = 0, hi = a.requests;  // starts[lo] <= i < starts[hi]
-      while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if ((uint32_t)a.starts[mid] <= i) lo = mid;
-        else hi = mid;
-      }
-      const uint32_t p = capped(max(a.cached[lo], 0), (uint32_t)i - (uint32_t)a.starts[lo]), j = p / a.pageSize;
+    if (i < all) {
+      const uint32_t b = requestOf(starts, a.requests, (uint32_t)i);
+      const uint32_t p = capped(max(a.cached[b], 0), (uint32_t)i - starts[b]), j = p / a.pageSize;
       position = (int32_t)p;
-      const int32_t page = j < a.tableWidth ? a.tables[(uint64_t)lo * a.tableWidth + j] : -1;
+      const int32_t page = j < a.tableWidth ? a.tables[(uint64_t)b * a.tableWidth + j] : -1;
       if (page >= 0) slot = (int64_t)page * a.pageSize + (p - j * a.pageSize);
     }
     a.slots[i] = slot;
@@ -55,41 +181,128 @@ __global__ __launch_bounds__(kThreads) void pageSlotsKernel(cuttHipTablesArgs a)
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void pageMoveKernel(cuttHipPageArgs a) {
-  const uint64_t perToken = (uint64_t)a.heads * a.width;
-  T* const rows = (T*)a.rows[blockIdx.y];
-  T* const cache = (T*)a.cache[blockIdx.y];
-  for (uint64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    const int64_t slot = a.slots[t];
-    const bool there = slot >= 0 && slot < (int64_t)a.pages * a.pageSize;
-    if (!there && !a.load) continue;
-    const uint64_t at = there ? slot / a.pageSize * a.pageStride + slot % a.pageSize * a.slotStride : 0;
-    for (uint64_t i = threadIdx.x; i < perToken; i += kThreads) {
-      const uint64_t h = i / a.width, c = i % a.width;
-      T& row = rows[t * a.tokenStride + h * a.headStride + c];
-      T* const cell = cache + (at + h * a.cacheHeadStride + c);
-      if (!a.load) *cell = row;
-      else row = there ? *cell : T(0);
+// ---------------------------------------------------------------------------
+// Rows to their slots and back.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kMaxBlocks = 1u << 20;
+constexpr int kPerLane = 4;  // vectors a lane keeps in flight
+
+struct PageMove {
+  uint32_t tokens, rowBytes;
+  uint32_t heads, vecs;                 // vectors per row
+  uint32_t groupTokens, groupItems;     // a workgroup's tokens at a time, and their vectors
+  cuttHipDivisor byVecs, byInner;       // inner: what runs faster of a group's tokens and heads
+  uint32_t pages, pageSize;
+  int wideSlots;                        // pages * pageSize is 2^31 or more
+  cuttHipDivisor byPage;
+  const int64_t* slots;
+  uint8_t* rows[2];
+  uint8_t* cache[2];
+  uint64_t tokenStride, headStride, pageStride, slotStride, cacheHeadStride;  // in bytes
+};
+
+// A workgroup takes a few tokens' rows of all heads at a time, N bytes per lane.  TOKENS_INNER: neighbouring lanes go from a row to the next
+// token's of the same head, else to the next head's.
+template <int N, bool LOAD, bool TOKENS_INNER>
+__global__ __launch_bounds__(kThreads) void pageMoveKernel(PageMove a) {
+  uint8_t* const rows = a.rows[blockIdx.y];
+  uint8_t* const cache = a.cache[blockIdx.y];
+  const uint64_t allSlots = (uint64_t)a.pages * a.pageSize;
+  for (uint64_t group = (uint64_t)blockIdx.x * a.groupTokens; group < a.tokens; group += (uint64_t)gridDim.x * a.groupTokens)
+    for (uint32_t item = threadIdx.x; item < a.groupItems; item += kThreads * kPerLane) {
+      Pack<uint8_t, N> v[kPerLane];
+      uint8_t *row[kPerLane], *cell[kPerLane];
+      bool mine[kPerLane], there[kPerLane];
+      int64_t slot[kPerLane];
+      uint32_t head[kPerLane], at[kPerLane];
+#pragma unroll
+      for (int u = 0; u < kPerLane; u++) {
+        const uint32_t i = min(item + u * kThreads, a.groupItems - 1), q = divide(i, a.byVecs), outer = divide(q, a.byInner);
+        const uint32_t inner = q - outer * (TOKENS_INNER ? a.groupTokens : a.heads);
+        head[u] = TOKENS_INNER ? outer : inner;
+        const uint64_t token = group + (TOKENS_INNER ? inner : outer);
+        mine[u] = item + u * kThreads < a.groupItems && token < a.tokens;
+        at[u] = min((i - q * a.vecs) * N, a.rowBytes - N);
+        const uint64_t t = min(token, (uint64_t)a.tokens - 1);
+        slot[u] = a.slots[t];
+        row[u] = rows + (t * a.tokenStride + head[u] * a.headStride + at[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kPerLane; u++) {
+        there[u] = (uint64_t)slot[u] < allSlots;
+        const uint64_t s = there[u] ? slot[u] : 0;
+        const uint64_t page = a.wideSlots ? s / a.pageSize : divide((uint32_t)s, a.byPage);
+        cell[u] = cache + (page * a.pageStride + (s - page * a.pageSize) * a.slotStride + head[u] * a.cacheHeadStride + at[u]);
+        if (LOAD) {
+          v[u] = {};
+          if (mine[u] && there[u]) v[u].load(cell[u]);
+        } else {
+          v[u].load(row[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kPerLane; u++) {
+        if (LOAD) {
+          if (mine[u]) v[u].store(row[u]);
+        } else {
+          if (mine[u] && there[u]) v[u].store(cell[u]);
+        }
+      }
     }
-  }
+}
+
+template <int N>
+int movePages(const PageMove& a, bool load, bool tokensInner, dim3 grid, void* stream) {
+  auto kernel = load ? (tokensInner ? pageMoveKernel<N, true, true> : pageMoveKernel<N, true, false>)
+                     : (tokensInner ? pageMoveKernel<N, false, true> : pageMoveKernel<N, false, false>);
+  return launchRows(kernel, grid, kThreads, 0, stream, a);
 }
 
 }  // namespace
 
 extern "C" int cuttHipPageTables(const cuttHipTablesArgs* a, void* stream) {
-  if (int e = launchRows(pageTablesKernel, 1, 1, 0, stream, *a)) return e;
+  const uint64_t most = a->tokens > a->requests ? a->tokens : a->requests;
+  const uint64_t groups = (most + kThreads - 1) / kThreads;
+  if (a->requests <= kScan)
+    return launchRows(pageTablesKernel, groups < 1 ? 1 : groups < 1024 ? groups : 1024, kThreads, 0, stream, *a);
+  if (int e = launchRows(pageTablesLongKernel, 1, kThreads, 0, stream, *a)) return e;
   if (!a->tokens) return 0;
-  const uint32_t blocks = (a->tokens + kThreads - 1) / kThreads;
-  return launchRows(pageSlotsKernel, blocks < kMaxBlocks ? blocks : kMaxBlocks, kThreads, 0, stream, *a);
+  return launchRows(pageSlotsKernel, groups < kMaxBlocks ? groups : kMaxBlocks, kThreads, 0, stream, *a);
 }
 
 extern "C" int cuttHipPageMove(const cuttHipPageArgs* a, void* stream) {
-  const dim3 grid(a->tokens < kMaxBlocks ? a->tokens : kMaxBlocks, a->rows[1] ? 2 : 1);
-  switch (a->elemSize) {
-    case 1: return launchRows(pageMoveKernel<uint8_t>, grid, kThreads, 0, stream, *a);
-    case 2: return launchRows(pageMoveKernel<uint16_t>, grid, kThreads, 0, stream, *a);
-    case 4: return launchRows(pageMoveKernel<uint32_t>, grid, kThreads, 0, stream, *a);
-    default: return launchRows(pageMoveKernel<uint64_t>, grid, kThreads, 0, stream, *a);
+  PageMove m;
+  const uint64_t size = a->elemSize;
+  m.tokens = a->tokens;
+  m.rowBytes = (uint32_t)(a->width * size);
+  m.heads = a->heads;
+  const uint32_t n = m.rowBytes >= 16 ? 16 : m.rowBytes % 4 == 0 ? 4 : 1;
+  m.vecs = (m.rowBytes + n - 1) / n;
+  const uint32_t perToken = m.vecs * m.heads;
+  m.groupTokens = kThreads * kPerLane / perToken;
+  if (m.groupTokens < 1) m.groupTokens = 1;
+  if (m.groupTokens > m.tokens) m.groupTokens = m.tokens;
+  m.groupItems = m.groupTokens * perToken;
+  const bool tokensInner = a->slotStride < a->cacheHeadStride;
+  m.byVecs = cuttHipMakeDivisor(m.vecs);
+  m.byInner = cuttHipMakeDivisor(tokensInner ? m.groupTokens : m.heads);
+  m.pages = a->pages;
+  m.pageSize = a->pageSize;
+  m.wideSlots = (uint64_t)a->pages * a->pageSize > 0x7fffffffull;
+  m.byPage = cuttHipMakeDivisor(a->pageSize);
+  m.slots = a->slots;
+  for (int i = 0; i < 2; i++) {
+    m.rows[i] = (uint8_t*)a->rows[i];
+    m.cache[i] = (uint8_t*)a->cache[i];
   }
+  m.tokenStride = a->tokenStride * size;
+  m.headStride = a->headStride * size;
+  m.pageStride = a->pageStride * size;
+  m.slotStride = a->slotStride * size;
+  m.cacheHeadStride = a->cacheHeadStride * size;
+  const uint32_t groups = (m.tokens + m.groupTokens - 1) / m.groupTokens;
+  const dim3 grid(groups < kMaxBlocks ? groups : kMaxBlocks, a->rows[1] ? 2 : 1);
+  const bool load = a->load != 0;
+  return n == 16 ? movePages<16>(m, load, tokensInner, grid, stream)
+                 : n == 4 ? movePages<4>(m, load, tokensInner, grid, stream) : movePages<1>(m, load, tokensInner, grid, stream);
 }

@@ -10,6 +10,8 @@
 #include <tuple>
 #include <type_traits>
 
+#include "hip_layer.h"
+
 namespace cutt {
 
 // Reports the launch call's own result (hipGetLastError would also report, and clear, what an earlier call of the
@@ -23,6 +25,9 @@ int launchRows(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t lds, void
   std::apply([&](auto&... v) { ((ptrs[i++] = (void*)&v), ...); }, held);
   return (int)hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, lds, (hipStream_t)stream);
 }
+
+// n / d for a divisor made by cuttHipMakeDivisor(d), n below 2^31.
+__device__ __forceinline__ uint32_t divide(uint32_t n, const cuttHipDivisor& d) { return (__umulhi(n, d.mul) + n * d.add) >> d.shift; }
 
 // N elements that lie anywhere: a vector whose accesses assume no more alignment than its element's.  16 bytes per lane are one
 // load or store instruction at any address.

@@ -57,6 +57,7 @@ typedef struct cuttHipTablesArgs {
 
 int cuttHipPageTables(const cuttHipTablesArgs* a, void* stream);
 
+/* heads * width * elemSize is below 2^31. */
 typedef struct cuttHipPageArgs {
   uint32_t tokens, heads, width, elemSize;
   uint32_t pages, pageSize;

@@ -100,6 +100,7 @@ cuttResult movePages(bool load, int tokens, int heads, int width, size_t sizeofT
                      const long long* cacheStrides) {
   if (tokens < 0 || heads < 1 || width < 1 || !opaqueSize(sizeofType) || pages < 0 || pageSize < 1 || !rowStrides || !cacheStrides)
     return CUTT_INVALID_PARAMETER;
+  if ((Wide)heads * (Wide)width * sizeofType > INT_MAX) return CUTT_INVALID_PARAMETER;
   if ((v == nullptr) != (vCache == nullptr)) return CUTT_INVALID_PARAMETER;
   const long long least[2] = {load ? width : 0, load ? 0 : width};  // of the rows' strides, of the caches'
   const unsigned long long rowExtent[2] = {(unsigned long long)tokens, (unsigned long long)heads};

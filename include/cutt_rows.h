@@ -114,8 +114,8 @@ cuttResult cuttExpertCombineBackward(int tokens, int choices, int rows, int widt
 
 /*
  * Takes pages for the new tokens of every request from a list of free ones and names the new tokens' slots.  With
- * owned = ceil(cached / pageSize) and want = ceil((cached + added) / pageSize), request b gets want - owned pages, the requests one after the
- * other from the front of freePages:
+ * owned = ceil(cached / pageSize) and want = ceil((cached + added) / pageSize), both tableWidth at most, request b gets want - owned
+ * pages, the requests one after the other from the front of freePages:
  *   tables[b, j]      for owned <= j < want: the next free page, -1 past the list's end; other entries stay
  *   starts[b]         new tokens of the requests before b; starts[requests] = all of them
  *   used[0]           pages wanted from the list; more than freeCount if it did not suffice
@@ -135,6 +135,7 @@ cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCo
  * Rows into pages: for every token t and head h, with s = slots[t],
  *   kCache[s / pageSize, s % pageSize, h, :] = k[t, h, :], the same for v.  Tokens whose slot is not in
  * 0 .. pages * pageSize - 1 are left out.  Slots that are named twice get one of the rows, not said which.
+ * A token's heads * width * sizeofType bytes are fewer than 2^31.
  *
  *   slots             [tokens], 64-bit
  *   rowStrides[2]     elements from token to token and from head to head of k and v

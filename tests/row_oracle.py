@@ -71,8 +71,8 @@ def tables(cached, added, page, free, tables, tokens):
     starts, taken, flat = [0], 0, []
     for b in range(len(cached)):
         c, n = max(int(cached[b]), 0), max(int(added[b]), 0)
-        owned, want = -(-c // page), -(-min(c + n, most) // page)
-        for j in range(owned, min(want, tables.shape[1])):
+        owned, want = (min(-(-x // page), tables.shape[1]) for x in (c, min(c + n, most)))
+        for j in range(owned, want):
             at = taken + j - owned
             tables[b, j] = free[at] if at < len(free) else -1
         taken = min(taken + want - owned, most)
