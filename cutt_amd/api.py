@@ -270,13 +270,16 @@ def cuttPageTables(requests, pageSize, tableWidth, freeCount, tokens, stream, ca
                                 slots, positions)
 
 
+_LONGS = {n: ctypes.c_longlong * n for n in (2, 3)}
+
+
 def _strides(v, n):
     """n strides as the C functions take them (an array of that kind is passed on as it is)."""
     if v is None:
         return v
     if len(v) != n:
         raise ValueError("%d strides wanted, got %d" % (n, len(v)))
-    return v if isinstance(v, ctypes.Array) else (ctypes.c_longlong * n)(*v)
+    return v if isinstance(v, ctypes.Array) else _LONGS[n](*v)
 
 
 def cuttPageStore(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides):

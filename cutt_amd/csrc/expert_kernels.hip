@@ -9,21 +9,28 @@ using namespace cutt;
 
 namespace {
 
+template <bool X>
+using Is = std::integral_constant<bool, X>;
+template <int X>
+using Number = std::integral_constant<int, X>;
+
 // ---------------------------------------------------------------------------
 // Sort.  A stable counting sort: each workgroup places a stretch of neighbouring choices.  It needs to know how many choices each expert has in
 // all and before the stretch.  Few choices: every workgroup counts all of them (COUNTED = false, one launch).  Many: a first
-// launch counts stretch by stretch into the workspace, [stretch][expert], and a workgroup adds the columns up.
+// launch counts stretch by stretch into the workspace, [stretch][experts, rounded up to 4], and a workgroup adds the columns up.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
-constexpr uint32_t kSortItems = 4;  // choices that a lane places at a time
-constexpr uint32_t kSortPart = kSortThreads * kSortItems;
+constexpr uint32_t kCountLoads = 16;
 constexpr uint32_t kSortGroups = 256;       // at most
-constexpr uint32_t kCountAll = 16384;       // choices that every workgroup counts for itself
+constexpr uint32_t kCountAll = 8192;        // choices that every workgroup counts for itself
+constexpr uint32_t kOneItem = 65536, kTwoItems = 131072;
 
 struct SortPlan {
-  uint32_t stretch;  // choices per workgroup, a multiple of kSortPart
+  uint32_t items;    // choices that a lane places at a time; a part is kSortThreads * items choices
+  uint32_t stretch;  // choices per workgroup, whole parts
   uint32_t groups;
   bool counted;
+  cuttHipDivisor byAlign;
 };
 
 // The expert of choice i among the `experts`, or `experts` if it is none of them.
@@ -43,22 +50,28 @@ __global__ __launch_bounds__(kSortThreads) void expertCountKernel(cuttHipSortArg
 #pragma unroll 4
   for (uint32_t i = from + threadIdx.x; i < to; i += kSortThreads) atomicAdd(&count[expertOf<Id>(a, i)], 1u);
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e < E; e += kSortThreads) a.workspace[(uint64_t)blockIdx.x * E + e] = count[e];
+  const uint32_t pitch = (E + 3) / 4 * 4;
+  for (uint32_t e = threadIdx.x; e < pitch; e += kSortThreads) a.workspace[(uint64_t)blockIdx.x * pitch + e] = e < E ? count[e] : 0;
 }
 
-// Lanes of the wavefront whose key is this lane's; keys have `bits` bits.
-__device__ __forceinline__ uint64_t sameKey(uint32_t key, uint32_t bits) {
-  uint64_t same = ~0ull;
-  for (uint32_t b = 0; b < bits; b++) {
-    const bool one = (key >> b) & 1;
-    const uint64_t set = __ballot(one);
-    same &= one ? set : ~set;
+// Lanes of the wavefront whose key is this lane's; keys have BITS bits.
+template <int BITS>
+__device__ __forceinline__ uint64_t sameKey(uint32_t key) {
+  uint32_t low = ~0u, high = ~0u;
+#pragma unroll
+  for (int b = 0; b < BITS; b++) {
+    const uint64_t set = __ballot((key >> b) & 1);
+    const uint32_t other = (key >> b & 1) - 1;  // all ones where this lane's bit is clear
+    low &= (uint32_t)set ^ other;
+    high &= (uint32_t)(set >> 32) ^ other;
   }
-  return same;
+  return (uint64_t)high << 32 | low;
 }
 
-template <typename Id, bool COUNTED>
-__global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs a, uint32_t stretch) {
+template <typename Id, bool COUNTED, int ITEMS, int BITS>
+__global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs a, SortPlan p) {
+  constexpr uint32_t kSortItems = ITEMS, kSortPart = kSortThreads * ITEMS;
+  const uint32_t stretch = p.stretch;
   extern __shared__ uint32_t lds[];
   const uint32_t E = a.experts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t* const next = lds;                    // [E + 1] choices before the stretch, then the row of an expert's next choice
@@ -68,28 +81,48 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
   __shared__ uint32_t waveSum[kSortWaves];
   const uint32_t from = blockIdx.x * stretch, to = min(from + stretch, a.n);
 
+  // The stretch's first part, before anything is waited for.
+  uint32_t expert[kSortItems];
+  const auto take = [&](uint64_t part) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t j = 0; j < kSortItems; j++) {
+      const uint64_t i = part + (wave * kSortItems + j) * 64 + lane;
+      expert[j] = i < to ? expertOf<Id>(a, (uint32_t)i) : E;
+    }
+  };
+  take(from);
+  for (uint32_t e = tid; e <= E; e += kSortThreads) next[e] = all[e] = 0;
+  __syncthreads();
   if constexpr (COUNTED) {
-    // The threads share the table: thread tid adds up every `share`-th stretch of expert tid % E (E <= kSortThreads), or experts
-    // tid, tid + kSortThreads of all.
-    for (uint32_t e = tid; e <= E; e += kSortThreads) next[e] = all[e] = 0;
-    __syncthreads();
-    const uint32_t share = E <= kSortThreads ? kSortThreads / E : 1, part = tid / E;
-    if (part < share || share == 1)
-      for (uint32_t e = share == 1 ? tid : tid - part * E; e < E; e += kSortThreads) {
-        uint32_t before = 0, sum = 0;
-#pragma unroll 8
-        for (uint32_t g = share == 1 ? 0 : part; g < gridDim.x; g += share) {
-          const uint32_t c = a.workspace[(uint64_t)g * E + e];
-          sum += c;
-          before += g < blockIdx.x ? c : 0;
+    // A thread adds up four neighbouring experts over every `share`-th stretch, kCountLoads loads of 16 bytes in flight.
+    const uint32_t quads = (E + 3) / 4, share = kSortThreads / quads, part = tid / quads, quad = tid - part * quads;
+    uint32_t before[4] = {}, sum[4] = {};
+    for (uint32_t first = part; part < share && first < gridDim.x; first += share * kCountLoads) {
+      Vec<uint32_t, 4> c[kCountLoads];
+#pragma unroll
+      for (uint32_t u = 0; u < kCountLoads; u++)
+        c[u] = *reinterpret_cast<const Vec<uint32_t, 4>*>(a.workspace + (uint64_t)min(first + u * share, gridDim.x - 1) * quads * 4 + quad * 4);
+#pragma unroll
+      for (uint32_t u = 0; u < kCountLoads; u++) {
+        const uint32_t g = first + u * share;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          sum[x] += g < gridDim.x ? c[u][x] : 0;
+          before[x] += g < blockIdx.x ? c[u][x] : 0;
         }
-        atomicAdd(&next[e], before);
-        atomicAdd(&all[e], sum);
       }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+      if (part < share && quad * 4 + x < E) {
+        atomicAdd(&next[quad * 4 + x], before[x]);
+        atomicAdd(&all[quad * 4 + x], sum[x]);
+      }
+  } else if (gridDim.x == 1) {
+#pragma unroll
+    for (uint32_t j = 0; j < kSortItems; j++) atomicAdd(&all[expert[j]], 1u);
   } else {
-    for (uint32_t e = tid; e <= E; e += kSortThreads) next[e] = all[e] = 0;
-    __syncthreads();
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t i = tid; i < a.n; i += kSortThreads) {
       const uint32_t e = expertOf<Id>(a, i);
       atomicAdd(&all[e], 1u);
@@ -104,15 +137,10 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const uint32_t e = 2 * tid + j;
-      padded[j] = e < E ? (all[e] + a.align - 1) / a.align * a.align : 0;
+      padded[j] = e < E ? divide(all[e] + a.align - 1, p.byAlign) * a.align : 0;
       sum += padded[j];
     }
-    uint32_t upTo = sum;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d *= 2) {
-      const uint32_t x = __shfl_up(upTo, d);
-      if (lane >= d) upTo += x;
-    }
+    const uint32_t upTo = scanOverWave(sum, [](uint32_t x, uint32_t y) { return x + y; });
     if (lane == 63) waveSum[wave] = upTo;
     __syncthreads();
     uint32_t at = upTo - sum;
@@ -144,20 +172,15 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
 
   // The stretch, part by part.  A wavefront's choices of a part are neighbours, so that an expert's rows follow the order of the
   // wavefronts, in a wavefront that of its steps, and in a step that of the lanes.
-  const uint32_t bits = 32 - __builtin_clz(E);
   uint32_t* const mine = seen + wave * (E + 1);
   for (uint64_t part = from; part < to; part += kSortPart) {
     for (uint32_t e = lane; e <= E; e += 64) mine[e] = 0;
     __builtin_amdgcn_wave_barrier();
-    uint32_t expert[kSortItems], rank[kSortItems];
+    uint32_t rank[kSortItems];
+    if (part != from) take(part);
 #pragma unroll
     for (uint32_t j = 0; j < kSortItems; j++) {
-      const uint64_t i = part + (wave * kSortItems + j) * 64 + lane;
-      expert[j] = i < to ? expertOf<Id>(a, (uint32_t)i) : E;
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < kSortItems; j++) {
-      const uint64_t same = sameKey(expert[j], bits);
+      const uint64_t same = sameKey<BITS>(expert[j]);
       const uint32_t below = __popcll(same & ((1ull << lane) - 1));
       const uint32_t before = mine[expert[j]];  // (the wavefront's lanes all read, then one lane per expert writes)
       __builtin_amdgcn_wave_barrier();
@@ -190,28 +213,31 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
   }
 }
 
-SortPlan planSort(uint32_t n) {
+SortPlan planSort(uint32_t n, uint32_t align) {
   SortPlan p;
-  const uint64_t parts = n ? ((uint64_t)n + kSortPart - 1) / kSortPart : 1;
   p.counted = n > kCountAll;
+  p.items = n <= kOneItem ? 1 : n <= kTwoItems ? 2 : 4;
+  const uint32_t part = kSortThreads * p.items;
+  const uint64_t parts = n ? ((uint64_t)n + part - 1) / part : 1;
   const uint64_t perGroup = (parts + kSortGroups - 1) / kSortGroups;
-  p.stretch = (uint32_t)(perGroup * kSortPart);
+  p.stretch = (uint32_t)(perGroup * part);
   p.groups = (uint32_t)((parts + perGroup - 1) / perGroup);
+  p.byAlign = cuttHipMakeDivisor(align);
   return p;
 }
 
 // ---------------------------------------------------------------------------
 // Rows to experts and back.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kRowThreads = 256, kRowWaves = kRowThreads / 64;
+constexpr uint32_t kMaxRowThreads = 512, kMaxRowWaves = kMaxRowThreads / 64;
 constexpr uint32_t kMaxBlocks = 1u << 22;  // (workgroups x lanes have to fit 32 bits)
 
 // Rows without a source, which hold zeros.  Workgroup `block` of `blocks` looks at kEmptyRows rows at a time; a wavefront clears a row.
 constexpr uint32_t kEmptyRows = 16;
 
-template <typename T, int N>
+template <typename T, int N, bool NT>
 __device__ __forceinline__ void clearEmptyRows(const cuttHipExpertArgs& a, T* y, uint64_t stride, uint32_t block, uint32_t blocks) {
-  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   Pack<T, N> zero = {};
   for (uint64_t first = (uint64_t)block * kEmptyRows; first < a.rows; first += (uint64_t)blocks * kEmptyRows) {
     const uint64_t mine = first + (lane & (kEmptyRows - 1));
@@ -219,9 +245,9 @@ __device__ __forceinline__ void clearEmptyRows(const cuttHipExpertArgs& a, T* y,
     for (uint32_t n = 0; empty; n++) {
       const uint32_t r = __builtin_ctzll(empty);
       empty &= empty - 1;
-      if (n % kRowWaves != wave) continue;
+      if (n % waves != wave) continue;
       T* const row = y + (first + r) * stride;
-      for (uint32_t c = lane * N; c < a.width; c += 64 * N) zero.store(row + min(c, a.width - N));
+      for (uint32_t c = lane * N; c < a.width; c += 64 * N) zero.template store<NT>(row + min(c, a.width - N));
     }
   }
 }
@@ -233,18 +259,19 @@ __device__ __forceinline__ void clearEmptyRows(const cuttHipExpertArgs& a, T* y,
 // without branches, and what an absent one brings is not used.
 template <int B>
 struct Choices {
+  static_assert(B >= 1 && B <= 8, "a power of two of lanes holds them");
   uint32_t laneRow;
   float laneWeight;
   uint32_t there;  // bit i: choice i has a row
 
   __device__ __forceinline__ Choices(const cuttHipExpertArgs& a, uint32_t token, uint32_t first) {
-    const uint32_t i = threadIdx.x & (B - 1);
+    const uint32_t i = threadIdx.x & 7;
     const uint64_t at = (uint64_t)token * a.choices + min(first + i, a.choices - 1);
     laneRow = (uint32_t)a.position[at];
     laneWeight = 1.0f;
     if (a.weights) laneWeight = a.weights[at];
-    const bool ok = first + i < a.choices && laneRow < a.rows;
-    there = (uint32_t)__ballot(ok) & ((1u << B) - 1);
+    const bool ok = i < B && first + i < a.choices && laneRow < a.rows;
+    there = (uint32_t)__ballot(ok) & 0xff;
     const uint32_t some = __builtin_amdgcn_readlane(laneRow, there ? __builtin_ctz(there) : 0);
     if (!ok) laneRow = some, laneWeight = 0.0f;
   }
@@ -253,42 +280,32 @@ struct Choices {
   __device__ __forceinline__ float weight(int i) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(laneWeight), i)); }
 };
 
-// The workgroup's wavefronts share a row's columns: wavefront w takes the columns w * 64 * N, (w + kRowWaves) * 64 * N, ...
+// The workgroup's wavefronts share a row's columns: wavefront w of W takes the columns w * 64 * N, (w + W) * 64 * N, ...
 __device__ __forceinline__ uint32_t waveOfGroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // A workgroup reads a token's row once and stores it to every row that the token goes to; the last workgroups clear the empty rows.
 // Rows are bytes here: any element size, any alignment.
-template <int N>
-__global__ __launch_bounds__(kRowThreads) void dispatchKernel(cuttHipExpertArgs a, const uint8_t* x, uint64_t xStride, uint8_t* y, uint64_t yStride,
-                                                              uint32_t tokenBlocks) {
-  constexpr int U = N == 1 ? 1 : 2;  // vectors a lane keeps
+template <int N, bool NT>
+__global__ __launch_bounds__(kMaxRowThreads) void dispatchKernel(cuttHipExpertArgs a, const uint8_t* x, uint64_t xStride, uint8_t* y, uint64_t yStride,
+                                                                 uint32_t tokenBlocks) {
   if (blockIdx.x >= tokenBlocks) {
-    clearEmptyRows<uint8_t, N>(a, y, yStride, blockIdx.x - tokenBlocks, gridDim.x - tokenBlocks);
+    clearEmptyRows<uint8_t, N, NT>(a, y, yStride, blockIdx.x - tokenBlocks, gridDim.x - tokenBlocks);
     return;
   }
   const uint32_t lane = threadIdx.x & 63;
   for (uint32_t t = blockIdx.x; t < a.tokens; t += tokenBlocks) {
     const uint8_t* const from = x + t * xStride;
     const Choices<8> begin(a, t, 0);
-    for (uint32_t col = waveOfGroup() * 64 * N; col < a.width; col += kRowThreads * N * U) {
-      Pack<uint8_t, N> v[U];
-      uint32_t at[U];
-      bool mine[U];
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const uint32_t base = col + u * kRowThreads * N + lane * N;
-        mine[u] = base < a.width;
-        at[u] = min(base, a.width - N);
-        v[u].load(from + at[u]);
-      }
+    for (uint32_t col = waveOfGroup() * 64 * N; col < a.width; col += blockDim.x * N) {
+      const uint32_t base = col + lane * N, c = min(base, a.width - N);
+      Pack<uint8_t, N> v;
+      v.load(from + c);
       auto put = [&](const Choices<8>& ch) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           if (!ch.has(i)) continue;
-          uint8_t* const to = y + ch.row(i) * yStride;
-#pragma unroll
-          for (int u = 0; u < U; u++)
-            if (mine[u]) v[u].store(to + at[u]);
+          uint8_t* const to = y + ch.row(i) * yStride + c;
+          if (base < a.width) v.template store<NT>(to);
         }
       };
       put(begin);
@@ -298,19 +315,19 @@ __global__ __launch_bounds__(kRowThreads) void dispatchKernel(cuttHipExpertArgs 
 }
 
 // A workgroup sums a token's rows, 16 bytes of each per lane.
-template <typename T, int N, int B>
-__global__ __launch_bounds__(kRowThreads) void combineKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, T* out, uint64_t outStride) {
+template <typename T, int N, int B, bool NT>
+__global__ __launch_bounds__(kMaxRowThreads) void combineKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, T* out, uint64_t outStride) {
   const uint32_t lane = threadIdx.x & 63;
   for (uint32_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
     const Choices<B> begin(a, t, 0);
-    for (uint32_t col = waveOfGroup() * 64 * N; col < a.width; col += kRowThreads * N) {
+    for (uint32_t col = waveOfGroup() * 64 * N; col < a.width; col += blockDim.x * N) {
       const uint32_t base = col + lane * N, c = min(base, a.width - N);
       float sum[N] = {};
       auto add = [&](const Choices<B>& ch) __attribute__((always_inline)) {
         if (!ch.there) return;
         Pack<T, N> v[B];
 #pragma unroll
-        for (int i = 0; i < B; i++) v[i].load(y + ch.row(i) * yStride + c);
+        for (int i = 0; i < B; i++) v[i].template load<NT>(y + ch.row(i) * yStride + c);
 #pragma unroll
         for (int i = 0; i < B; i++) {
           v[i].zeroUnless(ch.has(i));
@@ -332,6 +349,7 @@ __global__ __launch_bounds__(kRowThreads) void combineKernel(cuttHipExpertArgs a
 // Sums of B values over the wavefront: afterwards lane l holds the sum of value l / (64 / B).  Each step halves what a lane still holds.
 template <int B>
 __device__ __forceinline__ float sumOverWave(float (&v)[B]) {
+  static_assert((B & (B - 1)) == 0, "halved step by step");
   const uint32_t lane = threadIdx.x & 63;
   uint32_t half = 32;
 #pragma unroll
@@ -349,26 +367,27 @@ __device__ __forceinline__ float sumOverWave(float (&v)[B]) {
 }
 
 // A workgroup takes a token: its gradient row is multiplied into the rows it came from, and with them.  The last workgroups clear the empty rows.
-template <typename T, int N, int B, bool ROWS, bool WEIGHTS>
-__global__ __launch_bounds__(kRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
+template <typename T, int N, int B, bool ROWS, bool WEIGHTS, bool NT>
+__global__ __launch_bounds__(kMaxRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
                                                                      T* dy, uint64_t dyStride, float* dweights, uint32_t tokenBlocks) {
-  __shared__ float part[kRowWaves][B];
+  constexpr int P = B <= 1 ? 1 : B <= 2 ? 2 : B <= 4 ? 4 : 8;
+  __shared__ float part[kMaxRowWaves][P];
   if (ROWS && blockIdx.x >= tokenBlocks) {
-    clearEmptyRows<T, N>(a, dy, dyStride, blockIdx.x - tokenBlocks, gridDim.x - tokenBlocks);
+    clearEmptyRows<T, N, NT>(a, dy, dyStride, blockIdx.x - tokenBlocks, gridDim.x - tokenBlocks);
     return;
   }
   const uint32_t wave = waveOfGroup(), lane = threadIdx.x & 63;
   for (uint32_t t = blockIdx.x; t < a.tokens; t += tokenBlocks)
     for (uint32_t first = 0; first < a.choices; first += B) {
       const Choices<B> ch(a, t, first);
-      float dot[B] = {};
-      for (uint32_t col = waveOfGroup() * 64 * N; ch.there && col < a.width; col += kRowThreads * N) {
+      float dot[P] = {};
+      for (uint32_t col = waveOfGroup() * 64 * N; ch.there && col < a.width; col += blockDim.x * N) {
         const uint32_t base = col + lane * N, c = min(base, a.width - N);
         Pack<T, N> g, v[B];
-        g.load(dout + t * doutStride + c);
+        g.template load<NT>(dout + t * doutStride + c);
         if (WEIGHTS)
 #pragma unroll
-          for (int i = 0; i < B; i++) v[i].load(y + ch.row(i) * yStride + c);
+          for (int i = 0; i < B; i++) v[i].template load<NT>(y + ch.row(i) * yStride + c);
         Pack<T, N> once = g;
         if (WEIGHTS && c != base)  // columns that the vector before it, or its row's last vector, has already counted
 #pragma unroll
@@ -389,7 +408,7 @@ __global__ __launch_bounds__(kRowThreads) void combineBackwardKernel(cuttHipExpe
             Pack<T, N> o;
 #pragma unroll
             for (int e = 0; e < N; e++) o.set(e, (T)(w * (float)g.get(e)));
-            if (base < a.width) o.store(to);
+            if (base < a.width) o.template store<NT>(to);
           }
         }
       }
@@ -397,11 +416,11 @@ __global__ __launch_bounds__(kRowThreads) void combineBackwardKernel(cuttHipExpe
 #pragma unroll
       for (int i = 0; i < B; i++) dot[i] = ch.has(i) ? dot[i] : 0.0f;
       const float sum = sumOverWave(dot);
-      if (lane % (64 / B) == 0) part[wave][lane / (64 / B)] = sum;
+      if (lane % (64 / P) == 0) part[wave][lane / (64 / P)] = sum;
       __syncthreads();
       if (threadIdx.x < B && first + threadIdx.x < a.choices) {
         float all = 0;
-        for (uint32_t w = 0; w < kRowWaves; w++) all += part[w][threadIdx.x];
+        for (uint32_t w = 0; w < blockDim.x / 64; w++) all += part[w][threadIdx.x];
         dweights[(uint64_t)t * a.choices + first + threadIdx.x] = all;
       }
       __syncthreads();
@@ -416,19 +435,25 @@ uint32_t emptyBlocks(uint32_t rows) { return blocksFor((rows + (uint64_t)kEmptyR
 }  // namespace
 
 extern "C" size_t cuttHipSortWorkspace(uint32_t n, uint32_t experts) {
-  const SortPlan p = planSort(n);
-  return p.counted ? (size_t)p.groups * experts * 4 : 0;
+  const SortPlan p = planSort(n, 1);
+  return p.counted ? (size_t)p.groups * ((experts + 3) / 4 * 4) * 4 : 0;
 }
 
 namespace {
 
 template <typename Id>
 int sortBy(const cuttHipSortArgs* a, void* stream) {
-  const SortPlan p = planSort(a->n);
+  const SortPlan p = planSort(a->n, a->align);
   const size_t perExpert = (size_t)(a->experts + 1) * 4, lds = (3 + kSortWaves) * perExpert;
-  if (!p.counted) return launchRows(expertSortKernel<Id, false>, p.groups, kSortThreads, lds, stream, *a, p.stretch);
-  if (int e = launchRows(expertCountKernel<Id>, p.groups, kSortThreads, perExpert, stream, *a, p.stretch)) return e;
-  return launchRows(expertSortKernel<Id, true>, p.groups, kSortThreads, lds, stream, *a, p.stretch);
+  if (p.counted)
+    if (int e = launchRows(expertCountKernel<Id>, p.groups, kSortThreads, perExpert, stream, *a, p.stretch)) return e;
+  auto go = [&](auto counted, auto items) {  // (numbers up to `experts` itself, which stands for none of them)
+    auto kernel = a->experts < 64 ? expertSortKernel<Id, counted, items, 6>
+                                  : a->experts < 256 ? expertSortKernel<Id, counted, items, 8> : expertSortKernel<Id, counted, items, 11>;
+    return launchRows(kernel, p.groups, kSortThreads, lds, stream, *a, p);
+  };
+  if (!p.counted) return go(Is<false>{}, Number<1>{});
+  return p.items == 1 ? go(Is<true>{}, Number<1>{}) : p.items == 2 ? go(Is<true>{}, Number<2>{}) : go(Is<true>{}, Number<4>{});
 }
 
 }  // namespace
@@ -436,6 +461,18 @@ int sortBy(const cuttHipSortArgs* a, void* stream) {
 extern "C" int cuttHipExpertSort(const cuttHipSortArgs* a, void* stream) {
   return a->idBytes == 8 ? sortBy<int64_t>(a, stream) : sortBy<int32_t>(a, stream);
 }
+
+namespace {
+
+// Lanes for rows of `width` elements, N per lane: one pass over a row if kMaxRowThreads suffice.
+uint32_t rowThreads(uint32_t width, uint32_t n) {
+  const uint64_t waves = ((uint64_t)width + 64 * n - 1) / (64 * n);
+  return waves < kMaxRowWaves ? (uint32_t)waves * 64 : kMaxRowThreads;
+}
+
+bool onLines(const void* p, uint64_t strideBytes) { return ((uintptr_t)p | strideBytes) % 128 == 0; }
+
+}  // namespace
 
 extern "C" int cuttHipDispatch(const cuttHipExpertArgs* a, uint32_t elemSize, const void* x, uint64_t xStride, void* y, uint64_t yStride, void* stream) {
   const uint64_t bytes = (uint64_t)a->width * elemSize;
@@ -445,8 +482,10 @@ extern "C" int cuttHipDispatch(const cuttHipExpertArgs* a, uint32_t elemSize, co
   for (uint64_t at = 0; at < bytes; at += kMaxPiece) {
     cuttHipExpertArgs b = *a;
     b.width = (uint32_t)(bytes - at < kMaxPiece ? bytes - at : kMaxPiece);
-    auto kernel = b.width >= 16 ? dispatchKernel<16> : dispatchKernel<1>;
-    if (int e = launchRows(kernel, grid, kRowThreads, 0, stream, b, (const uint8_t*)x + at, xStride * elemSize, (uint8_t*)y + at, yStride * elemSize, tokenBlocks))
+    const bool nt = pastCaches(a->rows, bytes) && onLines(y, yStride * elemSize);
+    auto kernel = b.width < 16 ? dispatchKernel<1, false> : nt ? dispatchKernel<16, true> : dispatchKernel<16, false>;
+    if (int e = launchRows(kernel, grid, rowThreads(b.width, b.width < 16 ? 1 : 16), 0, stream, b, (const uint8_t*)x + at, xStride * elemSize, (uint8_t*)y + at,
+                           yStride * elemSize, tokenBlocks))
       return e;
   }
   return 0;
@@ -454,54 +493,89 @@ extern "C" int cuttHipDispatch(const cuttHipExpertArgs* a, uint32_t elemSize, co
 
 namespace {
 
-// Calls f with the elements per vector and the choices taken at once as constants.
-template <typename T, typename F>
-int byShape(const cuttHipExpertArgs* a, F f) {
+template <typename T, int N>
+int combine(const cuttHipExpertArgs* a, const T* y, uint64_t yStride, T* out, uint64_t outStride, bool nt, void* stream) {
+  auto go = [&](auto kernel) { return launchRows(kernel, blocksFor(a->tokens), rowThreads(a->width, N), 0, stream, *a, y, yStride, out, outStride); };
+  if constexpr (N == 1) {
+    return go(combineKernel<T, 1, 1, false>);
+  } else {
+    auto withChoices = [&](auto b) { return nt ? go(combineKernel<T, N, b, true>) : go(combineKernel<T, N, b, false>); };
+    switch (a->choices) {
+      case 1: return withChoices(Number<1>{});
+      case 2: return withChoices(Number<2>{});
+      case 3: return withChoices(Number<3>{});
+      case 4: return withChoices(Number<4>{});
+      case 5: return withChoices(Number<5>{});
+      case 6: return withChoices(Number<6>{});
+      case 7: return withChoices(Number<7>{});
+      default: return withChoices(Number<8>{});
+    }
+  }
+}
+
+template <typename T>
+int combineRows(const cuttHipExpertArgs* a, const void* y, uint64_t yStride, void* out, uint64_t outStride, void* stream) {
   constexpr int N = 16 / sizeof(T);
-  if (a->width < N) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-  const std::integral_constant<int, N> n;
-  if (a->choices > 4) return f(n, std::integral_constant<int, 8>{});
-  if (a->choices > 2) return f(n, std::integral_constant<int, 4>{});
-  if (a->choices > 1) return f(n, std::integral_constant<int, 2>{});
-  return f(n, std::integral_constant<int, 1>{});
+  const bool nt = pastCaches(a->rows, a->width * sizeof(T));
+  if (a->width < N) return combine<T, 1>(a, (const T*)y, yStride, (T*)out, outStride, false, stream);
+  return combine<T, N>(a, (const T*)y, yStride, (T*)out, outStride, nt, stream);
 }
 
-template <typename T>
-int combine(const cuttHipExpertArgs* a, const void* y, uint64_t yStride, void* out, uint64_t outStride, void* stream) {
-  return byShape<T>(a, [&](auto n, auto b) {
-    return launchRows(combineKernel<T, n, b>, blocksFor(a->tokens), kRowThreads, 0, stream, *a, (const T*)y, yStride, (T*)out, outStride);
-  });
-}
-
-template <typename T>
-int combineBackward(const cuttHipExpertArgs* a, const void* y, uint64_t yStride, const void* dout, uint64_t doutStride, void* dy, uint64_t dyStride,
-                    float* dweights, void* stream) {
+template <typename T, int N>
+int combineBackward(const cuttHipExpertArgs* a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride, T* dy, uint64_t dyStride, float* dweights,
+                    bool nt, void* stream) {
   const uint32_t tokenBlocks = blocksFor(a->tokens);
-  return byShape<T>(a, [&](auto n, auto b) {
-    auto go = [&](auto kernel, uint32_t blocks) {
-      return launchRows(kernel, tokenBlocks + blocks, kRowThreads, 0, stream, *a, (const T*)y, yStride, (const T*)dout, doutStride, (T*)dy, dyStride, dweights, tokenBlocks);
-    };
-    if (!dy) return go(combineBackwardKernel<T, n, b, false, true>, 0);
-    if (!dweights) return go(combineBackwardKernel<T, n, b, true, false>, emptyBlocks(a->rows));
-    return go(combineBackwardKernel<T, n, b, true, true>, emptyBlocks(a->rows));
-  });
+  auto go = [&](auto kernel) {
+    return launchRows(kernel, tokenBlocks + (dy ? emptyBlocks(a->rows) : 0), rowThreads(a->width, N), 0, stream, *a, y, yStride, dout, doutStride, dy, dyStride, dweights,
+                      tokenBlocks);
+  };
+  if constexpr (N == 1) {
+    if (!dy) return go(combineBackwardKernel<T, 1, 1, false, true, false>);
+    if (!dweights) return go(combineBackwardKernel<T, 1, 1, true, false, false>);
+    return go(combineBackwardKernel<T, 1, 1, true, true, false>);
+  } else {
+    if (!dy) {
+      auto withChoices = [&](auto b) { return nt ? go(combineBackwardKernel<T, N, b, false, true, true>) : go(combineBackwardKernel<T, N, b, false, true, false>); };
+      return a->choices > 4 ? withChoices(Number<8>{}) : withChoices(Number<4>{});
+    }
+    if (!dweights) return nt ? go(combineBackwardKernel<T, N, 8, true, false, true>) : go(combineBackwardKernel<T, N, 8, true, false, false>);
+    auto withChoices = [&](auto b) { return nt ? go(combineBackwardKernel<T, N, b, true, true, true>) : go(combineBackwardKernel<T, N, b, true, true, false>); };
+    switch (a->choices) {
+      case 1:
+      case 2: return withChoices(Number<2>{});
+      case 3:
+      case 4: return withChoices(Number<4>{});
+      case 5:
+      case 6: return withChoices(Number<6>{});
+      default: return withChoices(Number<8>{});
+    }
+  }
+}
+
+template <typename T>
+int combineRowsBackward(const cuttHipExpertArgs* a, const void* y, uint64_t yStride, const void* dout, uint64_t doutStride, void* dy, uint64_t dyStride,
+                        float* dweights, void* stream) {
+  constexpr int N = 16 / sizeof(T);
+  const bool nt = pastCaches(a->rows, a->width * sizeof(T));
+  if (a->width < N) return combineBackward<T, 1>(a, (const T*)y, yStride, (const T*)dout, doutStride, (T*)dy, dyStride, dweights, false, stream);
+  return combineBackward<T, N>(a, (const T*)y, yStride, (const T*)dout, doutStride, (T*)dy, dyStride, dweights, nt, stream);
 }
 
 }  // namespace
 
 extern "C" int cuttHipCombine(const cuttHipExpertArgs* a, int type, const void* y, uint64_t yStride, void* out, uint64_t outStride, void* stream) {
   switch (type) {
-    case CUTT_ROW_F32: return combine<float>(a, y, yStride, out, outStride, stream);
-    case CUTT_ROW_F16: return combine<_Float16>(a, y, yStride, out, outStride, stream);
-    default: return combine<__bf16>(a, y, yStride, out, outStride, stream);
+    case CUTT_ROW_F32: return combineRows<float>(a, y, yStride, out, outStride, stream);
+    case CUTT_ROW_F16: return combineRows<_Float16>(a, y, yStride, out, outStride, stream);
+    default: return combineRows<__bf16>(a, y, yStride, out, outStride, stream);
   }
 }
 
 extern "C" int cuttHipCombineBackward(const cuttHipExpertArgs* a, int type, const void* y, uint64_t yStride, const void* dout, uint64_t doutStride,
                                       void* dy, uint64_t dyStride, float* dweights, void* stream) {
   switch (type) {
-    case CUTT_ROW_F32: return combineBackward<float>(a, y, yStride, dout, doutStride, dy, dyStride, dweights, stream);
-    case CUTT_ROW_F16: return combineBackward<_Float16>(a, y, yStride, dout, doutStride, dy, dyStride, dweights, stream);
-    default: return combineBackward<__bf16>(a, y, yStride, dout, doutStride, dy, dyStride, dweights, stream);
+    case CUTT_ROW_F32: return combineRowsBackward<float>(a, y, yStride, dout, doutStride, dy, dyStride, dweights, stream);
+    case CUTT_ROW_F16: return combineRowsBackward<_Float16>(a, y, yStride, dout, doutStride, dy, dyStride, dweights, stream);
+    default: return combineRowsBackward<__bf16>(a, y, yStride, dout, doutStride, dy, dyStride, dweights, stream);
   }
 }

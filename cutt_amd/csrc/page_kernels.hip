@@ -36,6 +36,7 @@ constexpr uint32_t kPerThread = 8, kScan = kThreads * kPerThread;
 struct Scan {
   uint32_t tokens[kScan + 1];  // before request i of the scan; behind the last one, all
   uint32_t pages[kScan + 1];
+  uint32_t cached[kScan];
   uint32_t waveTokens[kWaves], wavePages[kWaves];
 };
 
@@ -51,19 +52,12 @@ __device__ __forceinline__ void scanRequests(const cuttHipTablesArgs& a, uint32_
       const Request r(a, first + from + i);
       tokens[i] = r.added;
       pages[i] = r.need;
+      s.cached[from + i] = r.cached;
     }
     allTokens = capped(allTokens, tokens[i]);
     allPages = capped(allPages, pages[i]);
   }
-  uint32_t upToTokens = allTokens, upToPages = allPages;  // inclusive over the wavefront
-#pragma unroll
-  for (uint32_t d = 1; d < 64; d *= 2) {
-    const uint32_t t = __shfl_up(upToTokens, d), p = __shfl_up(upToPages, d);
-    if (lane >= d) {
-      upToTokens = capped(upToTokens, t);
-      upToPages = capped(upToPages, p);
-    }
-  }
+  const uint32_t upToTokens = scanOverWave(allTokens, capped), upToPages = scanOverWave(allPages, capped);
   if (lane == 63) {
     s.waveTokens[wave] = upToTokens;
     s.wavePages[wave] = upToPages;
@@ -110,7 +104,7 @@ __device__ __forceinline__ int32_t freePage(const cuttHipTablesArgs& a, uint32_t
 __device__ __forceinline__ void assignPages(const cuttHipTablesArgs& a, uint32_t first, uint32_t n, const Scan& s, uint32_t thread, uint32_t threads) {
   for (uint64_t at = (uint64_t)s.pages[0] + thread; at < s.pages[n]; at += threads) {
     const uint32_t i = requestOf(s.pages, n, (uint32_t)at), b = first + i;
-    const uint32_t j = Request(a, b).owned + ((uint32_t)at - s.pages[i]);
+    const uint32_t j = min(pagesFor(s.cached[i], a.pageSize), a.tableWidth) + ((uint32_t)at - s.pages[i]);
     if (j < a.tableWidth) a.tables[(uint64_t)b * a.tableWidth + j] = freePage(a, (uint32_t)at);  // (always, unless sums were capped)
   }
 }
@@ -130,11 +124,11 @@ __global__ __launch_bounds__(kThreads) void pageTablesKernel(cuttHipTablesArgs a
     int32_t position = -1;
     if (i < s.tokens[n]) {
       const uint32_t b = requestOf(s.tokens, n, (uint32_t)i);
-      const Request r(a, b);
-      const uint32_t p = capped(r.cached, (uint32_t)i - s.tokens[b]), j = p / a.pageSize;
+      const uint32_t cached = s.cached[b], owned = pagesFor(cached, a.pageSize);
+      const uint32_t p = capped(cached, (uint32_t)i - s.tokens[b]), j = p / a.pageSize;
       position = (int32_t)p;
       if (j < a.tableWidth) {
-        const int32_t page = j < r.owned ? a.tables[(uint64_t)b * a.tableWidth + j] : freePage(a, capped(s.pages[b], j - r.owned));
+        const int32_t page = j < owned ? a.tables[(uint64_t)b * a.tableWidth + j] : freePage(a, capped(s.pages[b], j - owned));
         if (page >= 0) slot = (int64_t)page * a.pageSize + (p - j * a.pageSize);
       }
     }
@@ -185,7 +179,7 @@ __global__ __launch_bounds__(kThreads) void pageSlotsKernel(cuttHipTablesArgs a)
 // Rows to their slots and back.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMaxBlocks = 1u << 20;
-constexpr int kPerLane = 4;  // vectors a lane keeps in flight
+constexpr int kPerLane = 2;  // vectors a lane keeps in flight
 
 struct PageMove {
   uint32_t tokens, rowBytes;
@@ -203,7 +197,7 @@ struct PageMove {
 
 // A workgroup takes a few tokens' rows of all heads at a time, N bytes per lane.  TOKENS_INNER: neighbouring lanes go from a row to the next
 // token's of the same head, else to the next head's.
-template <int N, bool LOAD, bool TOKENS_INNER>
+template <int N, bool LOAD, bool TOKENS_INNER, bool NT>
 __global__ __launch_bounds__(kThreads) void pageMoveKernel(PageMove a) {
   uint8_t* const rows = a.rows[blockIdx.y];
   uint8_t* const cache = a.cache[blockIdx.y];
@@ -235,26 +229,26 @@ __global__ __launch_bounds__(kThreads) void pageMoveKernel(PageMove a) {
         cell[u] = cache + (page * a.pageStride + (s - page * a.pageSize) * a.slotStride + head[u] * a.cacheHeadStride + at[u]);
         if (LOAD) {
           v[u] = {};
-          if (mine[u] && there[u]) v[u].load(cell[u]);
+          if (mine[u] && there[u]) v[u].template load<NT>(cell[u]);
         } else {
-          v[u].load(row[u]);
+          v[u].template load<NT>(row[u]);
         }
       }
 #pragma unroll
       for (int u = 0; u < kPerLane; u++) {
         if (LOAD) {
-          if (mine[u]) v[u].store(row[u]);
+          if (mine[u]) v[u].template store<NT>(row[u]);
         } else {
-          if (mine[u] && there[u]) v[u].store(cell[u]);
+          if (mine[u] && there[u]) v[u].template store<NT>(cell[u]);
         }
       }
     }
 }
 
-template <int N>
+template <int N, bool NT>
 int movePages(const PageMove& a, bool load, bool tokensInner, dim3 grid, void* stream) {
-  auto kernel = load ? (tokensInner ? pageMoveKernel<N, true, true> : pageMoveKernel<N, true, false>)
-                     : (tokensInner ? pageMoveKernel<N, false, true> : pageMoveKernel<N, false, false>);
+  auto kernel = load ? (tokensInner ? pageMoveKernel<N, true, true, NT> : pageMoveKernel<N, true, false, NT>)
+                     : (tokensInner ? pageMoveKernel<N, false, true, NT> : pageMoveKernel<N, false, false, NT>);
   return launchRows(kernel, grid, kThreads, 0, stream, a);
 }
 
@@ -303,6 +297,8 @@ extern "C" int cuttHipPageMove(const cuttHipPageArgs* a, void* stream) {
   const uint32_t groups = (m.tokens + m.groupTokens - 1) / m.groupTokens;
   const dim3 grid(groups < kMaxBlocks ? groups : kMaxBlocks, a->rows[1] ? 2 : 1);
   const bool load = a->load != 0;
-  return n == 16 ? movePages<16>(m, load, tokensInner, grid, stream)
-                 : n == 4 ? movePages<4>(m, load, tokensInner, grid, stream) : movePages<1>(m, load, tokensInner, grid, stream);
+  if (n == 4) return movePages<4, false>(m, load, tokensInner, grid, stream);
+  if (n == 1) return movePages<1, false>(m, load, tokensInner, grid, stream);
+  if (pastCaches(m.tokens, (uint64_t)m.rowBytes * m.heads * (a->rows[1] ? 2 : 1))) return movePages<16, true>(m, load, tokensInner, grid, stream);
+  return movePages<16, false>(m, load, tokensInner, grid, stream);
 }

@@ -26,8 +26,30 @@ int launchRows(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t lds, void
   return (int)hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, lds, (hipStream_t)stream);
 }
 
+// Whether rows are more than the memory-side cache (256 MB) holds.  Then what is read cannot have been left there by whoever wrote it, nor what is
+// written be found there, and accesses past the caches are faster; below it they cost the next kernel more than they give.
+// 16384 tokens, 8 choices, 4096 bfloat16: dispatch (537 MB per 8192 tokens) 103 us past the caches, 117 us through them; dispatch and a combine that reads its rows
+// right after it, 134 MB: 60 us past, 52 us through; 537 MB: 202 and 205 us.
+inline bool pastCaches(uint64_t rows, uint64_t rowBytes) { return rows * rowBytes > ((uint64_t)256 << 20); }
+
 // n / d for a divisor made by cuttHipMakeDivisor(d), n below 2^31.
 __device__ __forceinline__ uint32_t divide(uint32_t n, const cuttHipDivisor& d) { return (__umulhi(n, d.mul) + n * d.add) >> d.shift; }
+
+// x of the lanes up to this one combined by an associative f whose neutral element is 0, for the lanes of a wavefront (all of them
+// take part).  Data move between lanes in the vector unit: four steps inside rows of 16 lanes, then the last lane of a row to the
+// next row and the last lane of the lower half to the upper half.
+template <typename F>
+__device__ __forceinline__ uint32_t scanOverWave(uint32_t x, F f) {
+#define CUTT_STEP(ctrl, rows) x = f(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false))
+  CUTT_STEP(0x111, 0xf);  // row_shr:1
+  CUTT_STEP(0x112, 0xf);
+  CUTT_STEP(0x114, 0xf);
+  CUTT_STEP(0x118, 0xf);
+  CUTT_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+  CUTT_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef CUTT_STEP
+  return x;
+}
 
 // N elements that lie anywhere: a vector whose accesses assume no more alignment than its element's.  16 bytes per lane are one
 // load or store instruction at any address.
@@ -42,8 +64,19 @@ using Vec = typename VecOf<T, N>::type;
 template <typename T, int N>
 struct Pack {
   Vec<T, N> v;
-  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const Vec<T, N>*>(p); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Vec<T, N>*>(p) = v; }
+  // NT: past the caches (non-temporal), for what is used once
+  template <bool NT = false>
+  __device__ __forceinline__ void load(const T* p) {
+    const Vec<T, N>* const q = reinterpret_cast<const Vec<T, N>*>(p);
+    if constexpr (NT) v = __builtin_nontemporal_load(q);
+    else v = *q;
+  }
+  template <bool NT = false>
+  __device__ __forceinline__ void store(T* p) const {
+    Vec<T, N>* const q = reinterpret_cast<Vec<T, N>*>(p);
+    if constexpr (NT) __builtin_nontemporal_store(v, q);
+    else *q = v;
+  }
   __device__ __forceinline__ T get(int i) const { return v[i]; }
   __device__ __forceinline__ void set(int i, T x) { v[i] = x; }
   // zeros unless `keep`
@@ -55,7 +88,9 @@ struct Pack {
 template <typename T>
 struct Pack<T, 1> {
   T v;
+  template <bool NT = false>
   __device__ __forceinline__ void load(const T* p) { v = *p; }
+  template <bool NT = false>
   __device__ __forceinline__ void store(T* p) const { *p = v; }
   __device__ __forceinline__ T get(int) const { return v; }
   __device__ __forceinline__ void set(int, T x) { v = x; }
