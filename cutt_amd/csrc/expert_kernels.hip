@@ -2,6 +2,8 @@
  * expert_kernels.hip - rows sorted by expert and back (cutt_rows.h): the stable counting sort of a router's
  * choices, the move of the tokens' rows to their experts, the weighted sum back, and the gradients of both.
  */
+#include <algorithm>
+
 #include "row_device.h"
 #include "row_layer.h"
 
@@ -22,7 +24,8 @@ using Number = std::integral_constant<int, X>;
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr uint32_t kCountLoads = 16;
 constexpr uint32_t kSortGroups = 256;       // at most
-constexpr uint32_t kCountAll = 8192;        // choices that every workgroup counts for itself
+constexpr uint32_t kCountAll = 4096;        // choices that every workgroup counts for itself
+constexpr uint32_t kRowsPerGroup = 1024, kRowGroups = 16;
 constexpr uint32_t kOneItem = 65536, kTwoItems = 131072;
 
 struct SortPlan {
@@ -42,13 +45,16 @@ __device__ __forceinline__ uint32_t expertOf(const cuttHipSortArgs& a, uint32_t 
 
 template <typename Id>
 __global__ __launch_bounds__(kSortThreads) void expertCountKernel(cuttHipSortArgs a, uint32_t stretch) {
-  extern __shared__ uint32_t count[];  // [experts + 1]
+  extern __shared__ uint32_t count[];  // [experts]
   const uint32_t E = a.experts;
-  for (uint32_t e = threadIdx.x; e <= E; e += kSortThreads) count[e] = 0;
+  for (uint32_t e = threadIdx.x; e < E; e += kSortThreads) count[e] = 0;
   __syncthreads();
   const uint32_t from = blockIdx.x * stretch, to = min(from + stretch, a.n);
 #pragma unroll 4
-  for (uint32_t i = from + threadIdx.x; i < to; i += kSortThreads) atomicAdd(&count[expertOf<Id>(a, i)], 1u);
+  for (uint32_t i = from + threadIdx.x; i < to; i += kSortThreads) {
+    const uint32_t e = expertOf<Id>(a, i);
+    if (e < E) atomicAdd(&count[e], 1u);
+  }
   __syncthreads();
   const uint32_t pitch = (E + 3) / 4 * 4;
   for (uint32_t e = threadIdx.x; e < pitch; e += kSortThreads) a.workspace[(uint64_t)blockIdx.x * pitch + e] = e < E ? count[e] : 0;
@@ -120,13 +126,14 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
       }
   } else if (gridDim.x == 1) {
 #pragma unroll
-    for (uint32_t j = 0; j < kSortItems; j++) atomicAdd(&all[expert[j]], 1u);
+    for (uint32_t j = 0; j < kSortItems; j++)
+      if (expert[j] < E) atomicAdd(&all[expert[j]], 1u);
   } else {
 #pragma unroll 8
     for (uint32_t i = tid; i < a.n; i += kSortThreads) {
       const uint32_t e = expertOf<Id>(a, i);
-      atomicAdd(&all[e], 1u);
-      if (i < from) atomicAdd(&next[e], 1u);
+      if (e < E) atomicAdd(&all[e], 1u);
+      if (e < E && i < from) atomicAdd(&next[e], 1u);
     }
   }
   __syncthreads();
@@ -213,7 +220,7 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
   }
 }
 
-SortPlan planSort(uint32_t n, uint32_t align) {
+SortPlan planSort(uint32_t n, uint32_t align, uint32_t rows) {
   SortPlan p;
   p.counted = n > kCountAll;
   p.items = n <= kOneItem ? 1 : n <= kTwoItems ? 2 : 4;
@@ -222,6 +229,7 @@ SortPlan planSort(uint32_t n, uint32_t align) {
   const uint64_t perGroup = (parts + kSortGroups - 1) / kSortGroups;
   p.stretch = (uint32_t)(perGroup * part);
   p.groups = (uint32_t)((parts + perGroup - 1) / perGroup);
+  if (!p.counted) p.groups = std::max(p.groups, std::min(rows / kRowsPerGroup, kRowGroups));  // (more, for the rows without a choice)
   p.byAlign = cuttHipMakeDivisor(align);
   return p;
 }
@@ -435,7 +443,7 @@ uint32_t emptyBlocks(uint32_t rows) { return blocksFor((rows + (uint64_t)kEmptyR
 }  // namespace
 
 extern "C" size_t cuttHipSortWorkspace(uint32_t n, uint32_t experts) {
-  const SortPlan p = planSort(n, 1);
+  const SortPlan p = planSort(n, 1, 0);
   return p.counted ? (size_t)p.groups * ((experts + 3) / 4 * 4) * 4 : 0;
 }
 
@@ -443,7 +451,7 @@ namespace {
 
 template <typename Id>
 int sortBy(const cuttHipSortArgs* a, void* stream) {
-  const SortPlan p = planSort(a->n, a->align);
+  const SortPlan p = planSort(a->n, a->align, a->rows);
   const size_t perExpert = (size_t)(a->experts + 1) * 4, lds = (3 + kSortWaves) * perExpert;
   if (p.counted)
     if (int e = launchRows(expertCountKernel<Id>, p.groups, kSortThreads, perExpert, stream, *a, p.stretch)) return e;
