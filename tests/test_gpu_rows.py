@@ -141,7 +141,8 @@ def on_gpu(a):
 # tokens, choices, experts, align, width, dropped, lead, gap
 ROWS = [(1, 1, 1, 1, 1, 0, 0, 0), (3, 2, 4, 4, 7, 0, 1, 0), (5, 1, 3, 1, 8, 0, 0, 8), (16, 8, 16, 8, 64, 0.2, 0, 0), (33, 3, 7, 16, 63, 0, 3, 2),
         (9, 9, 9, 2, 130, 0.5, 0, 6), (70, 4, 8, 16, 257, 0.1, 1, 1), (12, 17, 30, 1, 512, 0, 8, 8), (4, 6, 5, 64, 2050, 0, 0, 0),
-        (2, 2, 4, 1, 5001, 0.3, 0, 3), (6, 3, 4, 32, 9000, 1.0, 0, 0), (130, 2, 3, 1, 33, 0, 0, 0), (0, 2, 4, 4, 16, 0, 0, 0), (600, 8, 16, 16, 96, 0, 0, 0)]
+        (2, 2, 4, 1, 5001, 0.3, 0, 3), (6, 3, 4, 32, 9000, 1.0, 0, 0), (130, 2, 3, 1, 33, 0, 0, 0), (0, 2, 4, 4, 16, 0, 0, 0), (600, 8, 16, 16, 96, 0, 0, 0),
+        (40, 5, 9, 2, 200, 0.1, 0, 0), (41, 6, 9, 1, 203, 0.3, 5, 0), (42, 7, 9, 4, 1029, 0.1, 0, 3), (10, 24, 40, 1, 77, 0.1, 0, 0)]
 
 
 @pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.int32, torch.int64])
@@ -351,6 +352,70 @@ def test_rows_far_apart():
     assert cutt.cuttExpertCombineBackward(2, 1, 3, 40, 1, st(), ptr(p), ptr(s), ptr(w), 0, 0, ptr(dout), 40, ptr(rows), far, 0) == 0
     for r, want in ((0, 2.0), (1, 0.0), (2, 2.0)):
         assert bool((rows[r * far:r * far + 40] == want).all())
+
+
+@pytest.mark.parametrize("tokens,choices,width", [(4200, 8, 4096), (4100, 8, 4111), (5500, 6, 4108), (8300, 4, 4096), (17000, 2, 4096)])
+def test_rows_beyond_the_memory_side_cache(tokens, choices, width):
+    """More than 256 MB of rows; whole numbers, so that every sum is exact and comparisons are bit for bit."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(tokens)
+    experts, align = 64, 16
+    ids = torch.randint(0, experts + 2, (tokens, choices), generator=g, device="cuda", dtype=torch.int32)  # (some choices are nobody's)
+    rows = cutt.cuttExpertRows(tokens, choices, experts, align)
+    assert rows * width * 2 > 256 << 20
+    counts, offsets, position, source = run_sort(ids, 0, experts, align, rows)
+    p, s = on_gpu(position.reshape(tokens, choices)), on_gpu(source)
+
+    def whole(*shape):
+        return torch.randint(-8, 9, shape, generator=g, device="cuda", dtype=torch.int8).bfloat16()
+
+    x, w = whole(tokens, width), whole(tokens, choices).float()
+    y = torch.full((rows, width), float("nan"), dtype=torch.bfloat16, device="cuda")
+    assert cutt.cuttExpertDispatch(tokens, choices, rows, width, 2, st(), ptr(p), ptr(s), ptr(x), width, ptr(y), width) == 0
+    token = torch.div(s, choices, rounding_mode="floor").clamp(min=0).long()
+    assert torch.equal(y, x[token].masked_fill_((s < 0)[:, None], 0))
+    y = torch.where((s < 0)[:, None], float("nan"), whole(rows, width))
+    out, dx = torch.empty_like(x), torch.empty_like(x)
+    assert cutt.cuttExpertCombine(tokens, choices, rows, width, 2, st(), ptr(p), ptr(w), ptr(y), width, ptr(out), width) == 0
+    assert cutt.cuttExpertDispatchBackward(tokens, choices, rows, width, 2, st(), ptr(p), ptr(y), width, ptr(dx), width) == 0
+    want, plain = torch.zeros(tokens, width, device="cuda"), torch.zeros(tokens, width, device="cuda")
+    dw = torch.empty_like(w)
+    want_dw = torch.empty_like(w)
+    for k in range(choices):
+        there = (p[:, k] >= 0)[:, None]
+        row = torch.where(there, y[p[:, k].clamp(min=0).long()].float(), 0.0)
+        want += torch.where(there, w[:, k:k + 1] * row, 0.0)
+        plain += row
+        want_dw[:, k] = (row * x.float()).sum(1)
+    assert torch.equal(out, want.bfloat16()) and torch.equal(dx, plain.bfloat16())
+    dy = torch.full_like(y, float("nan"))
+    assert cutt.cuttExpertCombineBackward(tokens, choices, rows, width, 2, st(), ptr(p), ptr(s), ptr(w), ptr(y), width, ptr(x), width, ptr(dy), width,
+                                          ptr(dw)) == 0
+    scale = torch.where(s >= 0, w.view(-1)[s.clamp(min=0).long()], 0.0)
+    assert torch.equal(dy, (x[token].float() * scale[:, None]).bfloat16()) and torch.equal(dw, want_dw)
+
+
+@pytest.mark.parametrize("layout", ["slot", "head"])
+def test_pages_beyond_the_memory_side_cache(layout):
+    tokens, heads, width, page = 70000, 8, 128, 64
+    pages = 1200
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:tokens]
+    slots[::7] = -1
+    rows = torch.randint(-9, 10, (2, tokens, heads, width), generator=g, device="cuda", dtype=torch.int16)
+    caches = torch.full((2, pages, page, heads, width) if layout == "slot" else (2, pages, heads, page, width), MARK, dtype=torch.int16, device="cuda")
+    at = caches if layout == "slot" else caches.transpose(2, 3)
+    assert cutt.cuttPageStore(tokens, heads, width, 2, pages, page, st(), ptr(slots), ptr(rows[0]), ptr(rows[1]), rows.stride()[1:3], ptr(caches[0]),
+                              ptr(caches[1]), at.stride()[1:4]) == 0
+    there = (slots >= 0).nonzero()[:, 0]
+    want = torch.full((2, pages * page, heads, width), MARK, dtype=torch.int16, device="cuda")
+    want[:, slots[there]] = rows[:, there]
+    assert torch.equal(at.reshape(want.shape), want)
+    back = torch.empty(2, heads, tokens, width, dtype=torch.int16, device="cuda")
+    assert cutt.cuttPageLoad(tokens, heads, width, 2, pages, page, st(), ptr(slots), ptr(back[0]), ptr(back[1]), (back.stride(2), back.stride(1)),
+                             ptr(caches[0]), ptr(caches[1]), at.stride()[1:4]) == 0
+    assert torch.equal(back.transpose(1, 2), rows.masked_fill((slots < 0)[None, :, None, None], 0))
 
 
 # ---- pages ------------------------------------------------------------------------
