@@ -238,7 +238,8 @@ SortPlan planSort(uint32_t n, uint32_t align, uint32_t rows) {
 // Rows to experts and back.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMaxRowThreads = 512, kMaxRowWaves = kMaxRowThreads / 64;
-constexpr uint32_t kMaxBlocks = 1u << 22;  // (workgroups x lanes have to fit 32 bits)
+constexpr uint32_t kMaxBlocks = 1u << 21;  // of tokens, and of empty rows: all lanes of a launch have to be fewer than 2^32
+static_assert(2ull * kMaxBlocks * kMaxRowThreads <= CUTT_HIP_MAX_GRID_LANES, "a larger grid would be cut without an error");
 
 // Rows without a source, which hold zeros.  Workgroup `block` of `blocks` looks at kEmptyRows rows at a time; a wavefront clears a row.
 constexpr uint32_t kEmptyRows = 16;

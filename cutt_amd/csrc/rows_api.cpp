@@ -44,7 +44,7 @@ bool strided(const void* p, int n, const unsigned long long* extent, const long 
   if (!p || !aligned(p, size)) return false;
   for (int i = 0; i < n; i++) {
     if (extent[i] == 1) continue;
-    if (stride[i] < least || stride[i] < 0) return false;
+    if (stride[i] < least) return false;
     last += (Wide)(extent[i] - 1) * (Wide)stride[i];
     if (last > kMaxBytes) return false;
   }
@@ -52,7 +52,10 @@ bool strided(const void* p, int n, const unsigned long long* extent, const long 
   return s.bytes <= kMaxBytes;
 }
 
-bool rowsOf(const void* p, unsigned long long count, long long stride, unsigned long long width, size_t size, Span& s) {
+bool rowsRead(const void* p, unsigned long long count, long long stride, unsigned long long width, size_t size, Span& s) {
+  return strided(p, 1, &count, &stride, 0, width, size, s);
+}
+bool rowsWritten(const void* p, unsigned long long count, long long stride, unsigned long long width, size_t size, Span& s) {
   return strided(p, 1, &count, &stride, (long long)width, width, size, s);
 }
 
@@ -86,8 +89,8 @@ cuttResult sumRows(int tokens, int choices, int rows, int width, cuttRowType typ
   if (!size || !rowSizes(tokens, choices, rows, width)) return CUTT_INVALID_PARAMETER;
   const unsigned long long n = (unsigned long long)tokens * choices;
   Span p, w, from, to;
-  if (!values(position, n, 4, p) || !values(weights, weighted ? n : 0, 4, w) || !rowsOf(y, rows, yStride, width, size, from) ||
-      !rowsOf(out, tokens, outStride, width, size, to))
+  if (!values(position, n, 4, p) || !values(weights, weighted ? n : 0, 4, w) || !rowsRead(y, rows, yStride, width, size, from) ||
+      !rowsWritten(out, tokens, outStride, width, size, to))
     return CUTT_INVALID_PARAMETER;
   if (overlap(to, from) || overlap(to, p) || overlap(to, w)) return CUTT_INVALID_PARAMETER;
   if (tokens == 0) return CUTT_SUCCESS;
@@ -194,8 +197,8 @@ extern "C" cuttResult cuttExpertDispatch(int tokens, int choices, int rows, int 
   if (!opaqueSize(sizeofType) || !rowSizes(tokens, choices, rows, width)) return CUTT_INVALID_PARAMETER;
   const unsigned long long n = (unsigned long long)tokens * choices;
   Span p, s, from, to;
-  if (!values(position, n, 4, p) || !values(source, rows, 4, s) || !rowsOf(x, tokens, xStride, width, sizeofType, from) ||
-      !rowsOf(y, rows, yStride, width, sizeofType, to))
+  if (!values(position, n, 4, p) || !values(source, rows, 4, s) || !rowsRead(x, tokens, xStride, width, sizeofType, from) ||
+      !rowsWritten(y, rows, yStride, width, sizeofType, to))
     return CUTT_INVALID_PARAMETER;
   if (overlap(to, from) || overlap(to, p) || overlap(to, s)) return CUTT_INVALID_PARAMETER;
   if (rows == 0) return CUTT_SUCCESS;
@@ -223,10 +226,10 @@ extern "C" cuttResult cuttExpertCombineBackward(int tokens, int choices, int row
   const bool wantRows = dy != nullptr || rows == 0, wantWeights = dweights != nullptr || n == 0;
   if (!wantRows && !wantWeights) return CUTT_INVALID_PARAMETER;
   Span p, s, w, yIn, dIn, dyOut, dwOut;
-  if (!values(position, n, 4, p) || !rowsOf(dout, tokens, doutStride, width, size, dIn)) return CUTT_INVALID_PARAMETER;
-  if (wantRows && (!values(source, rows, 4, s) || !values(weights, n, 4, w) || !rowsOf(dy, rows, dyStride, width, size, dyOut)))
+  if (!values(position, n, 4, p) || !rowsRead(dout, tokens, doutStride, width, size, dIn)) return CUTT_INVALID_PARAMETER;
+  if (wantRows && (!values(source, rows, 4, s) || !values(weights, n, 4, w) || !rowsWritten(dy, rows, dyStride, width, size, dyOut)))
     return CUTT_INVALID_PARAMETER;
-  if (wantWeights && (!values(dweights, n, 4, dwOut) || (n && !rowsOf(y, rows, yStride, width, size, yIn)))) return CUTT_INVALID_PARAMETER;
+  if (wantWeights && (!values(dweights, n, 4, dwOut) || (n && !rowsRead(y, rows, yStride, width, size, yIn)))) return CUTT_INVALID_PARAMETER;
   const Span reads[] = {p, s, w, yIn, dIn};
   for (const Span& r : reads)
     if (overlap(dyOut, r) || overlap(dwOut, r)) return CUTT_INVALID_PARAMETER;

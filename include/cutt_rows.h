@@ -4,8 +4,8 @@
  * knows when it plans; the reference has no counterpart.
  *
  * Conventions:
- *   - a row is `width` contiguous elements; row strides are in elements; the last argument group of a
- *     call names device buffers, integers in them are 32-bit unless said otherwise;
+ *   - a row is `width` contiguous elements; row strides are in elements, `width` and more for what is written, 0 and more for
+ *     what is read; integers in device buffers are 32-bit unless said otherwise;
  *   - rows that only move are opaque (sizeofType 1, 2, 4 or 8 bytes per element) and keep their bits;
  *     rows that are summed have a cuttRowType, are summed in 32 bits and rounded once, to nearest even;
  *   - every call only launches kernels on `stream`, on the current device: it allocates nothing, keeps nothing,
@@ -142,7 +142,7 @@ cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCo
  *   cacheStrides[3]   elements from page to page, slot to slot and head to head of the caches; any order of the three
  *                     ([pages, pageSize, heads, width], [pages, heads, pageSize, width], ...)
  *   v, vCache         NULL both: only k moves
- * The strides are host arrays, read during the call.  What is written needs strides of width and more, what is read of 0 and more.
+ * The strides are host arrays, read during the call.
  */
 cuttResult cuttPageStore(int tokens, int heads, int width, size_t sizeofType, int pages, int pageSize, hipStream_t stream,
                          const long long* slots, const void* k, const void* v, const long long* rowStrides, void* kCache,

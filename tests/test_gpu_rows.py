@@ -280,6 +280,46 @@ def test_positions_out_of_range_count_as_absent():
     dy.check_surroundings()
 
 
+def test_one_row_for_all():
+    """Rows that are read may lie on top of each other (stride 0, as an expanded gradient has it)."""
+    rng = np.random.default_rng(8)
+    position, source, rows = routing(rng, 9, 2, 4, 4, 0.2)
+    p, s = on_gpu(position), on_gpu(source)
+    w = on_gpu(rng.integers(-4, 5, (9, 2)).astype(np.float32))
+    one, y = on_gpu(rng.integers(-9, 10, (1, 21)).astype(np.float32)), on_gpu(rng.integers(-9, 10, (rows, 21)).astype(np.float32))
+    all_of_it = np.repeat(f64(one), 9, 0)
+    out, dy, dw = torch.empty(rows, 21, device="cuda"), torch.empty_like(y), torch.empty_like(w)
+    assert cutt.cuttExpertDispatch(9, 2, rows, 21, 4, st(), ptr(p), ptr(s), ptr(one), 0, ptr(out), 21) == 0
+    assert np.array_equal(f64(out), row_oracle.dispatch(all_of_it, position, source, np.zeros((rows, 21))))
+    assert cutt.cuttExpertCombineBackward(9, 2, rows, 21, 0, st(), ptr(p), ptr(s), ptr(w), ptr(y), 21, ptr(one), 0, ptr(dy), 21, ptr(dw)) == 0
+    want_dy, want_dw, _ = row_oracle.combine_backward(f64(y), all_of_it, position, source, f64(w), np.zeros((rows, 21)))
+    assert np.array_equal(f64(dy), want_dy) and np.array_equal(f64(dw), want_dw)
+    back = torch.empty(9, 21, device="cuda")
+    assert cutt.cuttExpertCombine(9, 2, rows, 21, 0, st(), ptr(p), ptr(w), ptr(one), 0, ptr(back), 21) == 0
+    assert np.array_equal(f64(back), row_oracle.combine(np.repeat(f64(one), rows, 0), position, f64(w))[0])
+
+
+def test_more_tokens_than_workgroups():
+    tokens = 2 ** 21 + 77  # a launch has 2^21 workgroups for tokens at most
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    rows = tokens + 5
+    source = torch.randperm(rows, generator=g, device="cuda").int()
+    source = torch.where(source < tokens, source, -1)
+    position = torch.empty(tokens, 1, dtype=torch.int32, device="cuda")
+    there = (source >= 0).nonzero()[:, 0]
+    position[source[there].long(), 0] = there.int()
+    x = torch.randint(-9, 10, (tokens, 9), generator=g, device="cuda").half()
+    w = torch.randint(-4, 5, (tokens, 1), generator=g, device="cuda").float()
+    y, out, dy, dw = torch.empty(rows, 9, dtype=torch.half, device="cuda"), torch.empty_like(x), torch.empty(rows, 9, dtype=torch.half, device="cuda"), torch.empty_like(w)
+    assert cutt.cuttExpertDispatch(tokens, 1, rows, 9, 2, st(), ptr(position), ptr(source), ptr(x), 9, ptr(y), 9) == 0
+    assert torch.equal(y, x[source.clamp(min=0).long()].masked_fill_((source < 0)[:, None], 0))
+    assert cutt.cuttExpertCombine(tokens, 1, rows, 9, 1, st(), ptr(position), ptr(w), ptr(y), 9, ptr(out), 9) == 0
+    assert torch.equal(out, (x.float() * w).half())
+    assert cutt.cuttExpertCombineBackward(tokens, 1, rows, 9, 1, st(), ptr(position), ptr(source), ptr(w), ptr(y), 9, ptr(x), 9, ptr(dy), 9, ptr(dw)) == 0
+    assert torch.equal(dy, (y.float() * w[source.clamp(min=0).long()]).half()) and torch.equal(dw, (x.float() ** 2).sum(1, keepdim=True))
+
+
 def test_combine_without_rows():
     p = on_gpu(np.zeros((3, 2), dtype=np.int32))
     w, out, dw = (torch.full(s, float(MARK), device="cuda") for s in ((3, 2), (3, 8), (3, 2)))
@@ -459,6 +499,12 @@ def test_tables_many_requests():
     rng = np.random.default_rng(9)
     cached, added = rng.integers(0, 50, 20000), rng.integers(0, 3, 20000)
     check_tables(cached, added, 8, 7, rng.permutation(40000), int(added.sum()) + 5)
+
+
+def test_tables_more_tokens_than_lanes():
+    rng = np.random.default_rng(10)
+    cached, added = rng.integers(0, 700, 300), rng.integers(800, 1100, 300)
+    check_tables(cached, added, 16, 120, rng.permutation(40000), int(added.sum()))
 
 
 def test_tables_edges():

@@ -78,7 +78,7 @@ DISPATCH = dict(tokens=4, choices=2, rows=8, width=16, size=2, stream=0, positio
 
 
 @pytest.mark.parametrize("change", [dict(tokens=-1), dict(choices=0), dict(rows=-1), dict(width=0), dict(size=3), dict(size=16), dict(size=0),
-                                    dict(position=0), dict(source=0), dict(x=0), dict(y=0), dict(x=C + 1), dict(y=D + 1), dict(xs=15), dict(ys=15),
+                                    dict(position=0), dict(source=0), dict(x=0), dict(y=0), dict(x=C + 1), dict(y=D + 1), dict(xs=-1), dict(ys=15),
                                     dict(xs=-16), dict(y=C), dict(y=C + 120), dict(y=A), dict(position=A + 2), dict(xs=2 ** 62), dict(tokens=2 ** 30)])
 def test_dispatch_refuses(cutt, change):
     assert cutt.cuttExpertDispatch(*{**DISPATCH, **change}.values()) == BAD
@@ -97,7 +97,7 @@ COMBINE = dict(tokens=4, choices=2, rows=8, width=16, type=2, stream=0, position
 
 
 @pytest.mark.parametrize("change", [dict(tokens=-1), dict(choices=0), dict(rows=-1), dict(width=0), dict(type=3), dict(type=-1), dict(position=0),
-                                    dict(weights=0), dict(weights=B + 2), dict(y=0), dict(out=0), dict(out=D + 1), dict(ys=15), dict(outs=1),
+                                    dict(weights=0), dict(weights=B + 2), dict(y=0), dict(out=0), dict(out=D + 1), dict(ys=-1), dict(outs=1),
                                     dict(out=C + 8 * 32 - 2), dict(out=B), dict(out=A)])
 def test_combine_refuses(cutt, change):
     assert cutt.cuttExpertCombine(*{**COMBINE, **change}.values()) == BAD
@@ -111,8 +111,8 @@ BACKWARD = dict(tokens=4, choices=2, rows=8, width=16, type=2, stream=0, positio
 
 
 @pytest.mark.parametrize("change", [dict(tokens=-1), dict(type=3), dict(width=0), dict(position=0), dict(source=0), dict(weights=0), dict(y=0),
-                                    dict(dout=0), dict(dy=0, dweights=0), dict(dy=D), dict(dy=E), dict(dy=G), dict(dweights=G + 1), dict(ys=1),
-                                    dict(douts=1), dict(dys=1), dict(dweights=C), dict(dy=F + 1)])
+                                    dict(dout=0), dict(dy=0, dweights=0), dict(dy=D), dict(dy=E), dict(dy=G), dict(dweights=G + 1), dict(ys=-1),
+                                    dict(douts=-16), dict(dys=1), dict(dweights=C), dict(dy=F + 1)])
 def test_combine_backward_refuses(cutt, change):
     assert cutt.cuttExpertCombineBackward(*{**BACKWARD, **change}.values()) == BAD
 
