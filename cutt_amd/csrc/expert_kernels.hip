@@ -304,11 +304,13 @@ __global__ __launch_bounds__(kMaxRowThreads) void dispatchKernel(cuttHipExpertAr
   const uint32_t lane = threadIdx.x & 63;
   for (uint32_t t = blockIdx.x; t < a.tokens; t += tokenBlocks) {
     const uint8_t* const from = x + t * xStride;
+    uint32_t col = waveOfGroup() * 64 * N;
+    if (col >= a.width) continue;
+    Pack<uint8_t, N> v;  // (asked for before the choices are waited for)
+    v.load(from + min(col + lane * N, a.width - N));
     const Choices<8> begin(a, t, 0);
-    for (uint32_t col = waveOfGroup() * 64 * N; col < a.width; col += blockDim.x * N) {
+    for (;;) {
       const uint32_t base = col + lane * N, c = min(base, a.width - N);
-      Pack<uint8_t, N> v;
-      v.load(from + c);
       auto put = [&](const Choices<8>& ch) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -319,6 +321,9 @@ __global__ __launch_bounds__(kMaxRowThreads) void dispatchKernel(cuttHipExpertAr
       };
       put(begin);
       for (uint32_t first = 8; first < a.choices; first += 8) put(Choices<8>(a, t, first));
+      col += blockDim.x * N;
+      if (col >= a.width) break;
+      v.load(from + min(col + lane * N, a.width - N));
     }
   }
 }
