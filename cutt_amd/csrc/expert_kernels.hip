@@ -1,6 +1,9 @@
 /*
  * expert_kernels.hip - rows sorted by expert and back (cutt_rows.h): the stable counting sort of a router's
  * choices, the move of the tokens' rows to their experts, the weighted sum back, and the gradients of both.
+ *
+ * Times in the comments: MI355X, back to back in a graph, the buffers of several calls in rotation unless they say "the same buffers"; a launch
+ * of an empty kernel takes about 2.2 us there, a copy of 512 MB runs at 5.3 - 5.6 TB/s.
  */
 #include <algorithm>
 
@@ -17,15 +20,27 @@ template <int X>
 using Number = std::integral_constant<int, X>;
 
 // ---------------------------------------------------------------------------
-// Sort.  A stable counting sort: each workgroup places a stretch of neighbouring choices.  It needs to know how many choices each expert has in
-// all and before the stretch.  Few choices: every workgroup counts all of them (COUNTED = false, one launch).  Many: a first
-// launch counts stretch by stretch into the workspace, [stretch][experts, rounded up to 4], and a workgroup adds the columns up.
+// Sort.  A stable counting sort: each workgroup places a stretch of neighbouring choices, choice a of expert e in row
+//   first row of e + choices of e before the stretch + choices of e in the stretch before a.
+// It needs to know how many choices each expert has in all and before the stretch.  Few choices: every workgroup counts all of them (COUNTED =
+// false, one launch).  Many: a first launch counts stretch by stretch into the workspace, [stretch][experts, rounded up to 4], and a
+// workgroup adds the columns up.  Whole numbers only: the order of the LDS atomics does not show.
+//
+// Bound by launches and latencies, not by its bytes (262144 choices are 4 MB, under 1 us): the choices, the table, the scan over the
+// experts and the scattered 4-byte stores of `source` wait for each other.  512 choices 3.8 us, 4096 5.4, 65536 8.1, 262144 10.9, 1048576
+// 19 (128 or 256 experts, two launches from the third on).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
-constexpr uint32_t kCountLoads = 16;
-constexpr uint32_t kSortGroups = 256;       // at most
-constexpr uint32_t kCountAll = 4096;        // choices that every workgroup counts for itself
+constexpr uint32_t kCountLoads = 16;   // a workgroup's loads of the table go out at once: 262144 choices 25.9 -> 11.3 us against 8 loads of 4 bytes
+constexpr uint32_t kSortGroups = 256;  // at most: beyond, stretches get longer and the table does not grow
+// Choices that every workgroup counts for itself.  8192 choices, 256 experts: 7.1 us so, 7.9 with the table, but 17.0 and 7.7 where all are one expert's
+// and their LDS atomics follow each other.
+constexpr uint32_t kCountAll = 4096;
+// More workgroups for the rows that stay empty: 512 choices, 128 experts' segments in multiples of 64 rows, 5.2 us with one workgroup, 3.8 with 8.
 constexpr uint32_t kRowsPerGroup = 1024, kRowGroups = 16;
+// Choices that a lane places at a time: one up to the first number, two up to the second, four beyond.  More per lane are more steps in turn (512
+// choices: 5.2 us with one, 6.5 with two, 8.3 with four), fewer a longer table (262144 choices: 11.5 us with two, 10.9 with four; 65536: 8.4 with
+// one, 8.7 with two).
 constexpr uint32_t kOneItem = 65536, kTwoItems = 131072;
 
 struct SortPlan {
@@ -235,13 +250,17 @@ SortPlan planSort(uint32_t n, uint32_t align, uint32_t rows) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows to experts and back.
+// Rows to experts and back.  Sums of a few products per element of a row: all of it is bound by memory.  Every row is read once and written once (HBM
+// bytes by the counters equal to the algorithm's within 1 %), 16 bytes per lane at any alignment.  A workgroup takes a token and has a
+// lane for every vector of its row, up to 512: combine of 2048 x 8 rows of 4096 bfloat16 31.4 us with 512 lanes, 32.1 with 256, of 16 x 8 rows of 8192
+// 4.7 and 5.7.  Neighbouring tokens to the workgroups of one XCD: 208 -> 218 us for combine of 16384 x 8 rows, so the workgroups keep their order.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMaxRowThreads = 512, kMaxRowWaves = kMaxRowThreads / 64;
 constexpr uint32_t kMaxBlocks = 1u << 21;  // of tokens, and of empty rows: all lanes of a launch have to be fewer than 2^32
 static_assert(2ull * kMaxBlocks * kMaxRowThreads <= CUTT_HIP_MAX_GRID_LANES, "a larger grid would be cut without an error");
 
-// Rows without a source, which hold zeros.  Workgroup `block` of `blocks` looks at kEmptyRows rows at a time; a wavefront clears a row.
+// Rows without a source, which hold zeros.  Workgroup `block` of `blocks` looks at kEmptyRows rows at a time; a wavefront clears a row.  16384 x 8 rows of 512
+// bfloat16, none empty: 34.1 us with 4 rows, 30.5 with 16, 31.6 with 32; 256 rows of 8320 not empty, 4096 wide: 13.1, 14.0, 15.0.
 constexpr uint32_t kEmptyRows = 16;
 
 template <typename T, int N, bool NT>
@@ -293,7 +312,9 @@ struct Choices {
 __device__ __forceinline__ uint32_t waveOfGroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // A workgroup reads a token's row once and stores it to every row that the token goes to; the last workgroups clear the empty rows.
-// Rows are bytes here: any element size, any alignment.
+// Rows are bytes here: any element size, any alignment.  (Row by row of y instead, a token's row would be read once per choice.)
+// 16384 x 8 rows of 4096 bfloat16 and 8064 empty ones (1275 MB): 249 us, 216 with x left in the memory-side cache by whoever made it; rows
+// that follow each other instead of the experts' order take the same time.
 template <int N, bool NT>
 __global__ __launch_bounds__(kMaxRowThreads) void dispatchKernel(cuttHipExpertArgs a, const uint8_t* x, uint64_t xStride, uint8_t* y, uint64_t yStride,
                                                                  uint32_t tokenBlocks) {
@@ -328,7 +349,9 @@ __global__ __launch_bounds__(kMaxRowThreads) void dispatchKernel(cuttHipExpertAr
   }
 }
 
-// A workgroup sums a token's rows, 16 bytes of each per lane.
+// A workgroup sums a token's rows, 16 bytes of each per lane, in 32 bits and in the order of the choices, with one rounding at the end.
+// The loads of all choices are in flight together.  16384 x 8 rows of 4096 bfloat16 (1209 MB): 208 us, 5.8 TB/s; the gradient of dispatch
+// of 8191 x 4 rows of 2050 floats (336 MB) 55 us.
 template <typename T, int N, int B, bool NT>
 __global__ __launch_bounds__(kMaxRowThreads) void combineKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, T* out, uint64_t outStride) {
   const uint32_t lane = threadIdx.x & 63;
@@ -381,6 +404,9 @@ __device__ __forceinline__ float sumOverWave(float (&v)[B]) {
 }
 
 // A workgroup takes a token: its gradient row is multiplied into the rows it came from, and with them.  The last workgroups clear the empty rows.
+// The dot products are summed in 32 bits: a lane's columns, the lanes of a wavefront pairwise, the wavefronts in turn, always in the same order.
+// 8192 x 8 rows of 4096 bfloat16 (1142 MB): 219 us, 5.2 TB/s, as much read as written; a wavefront per token, without LDS: 241 us; four choices at a
+// time for less registers (six instead of four waves per SIMD): 232.
 template <typename T, int N, int B, bool ROWS, bool WEIGHTS, bool NT>
 __global__ __launch_bounds__(kMaxRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
                                                                      T* dy, uint64_t dyStride, float* dweights, uint32_t tokenBlocks) {
@@ -402,28 +428,33 @@ __global__ __launch_bounds__(kMaxRowThreads) void combineBackwardKernel(cuttHipE
         if (WEIGHTS)
 #pragma unroll
           for (int i = 0; i < B; i++) v[i].template load<NT>(y + ch.row(i) * yStride + c);
-        Pack<T, N> once = g;
-        if (WEIGHTS && c != base)  // columns that the vector before it, or its row's last vector, has already counted
+        float grad[N];
 #pragma unroll
-          for (int e = 0; e < N; e++)
-            if (c + e < base) {
-              once.set(e, T(0));
+        for (int e = 0; e < N; e++) grad[e] = (float)g.get(e);
+        if (ROWS)
 #pragma unroll
-              for (int i = 0; i < B; i++) v[i].set(e, T(0));
+          for (int i = 0; i < B; i++)
+            if (ch.has(i)) {
+              const float w = ch.weight(i);
+              T* const to = dy + ch.row(i) * dyStride + c;
+              Pack<T, N> o;
+#pragma unroll
+              for (int e = 0; e < N; e++) o.set(e, (T)(w * grad[e]));
+              if (base < a.width) o.template store<NT>(to);
             }
+        if (WEIGHTS) {
+          if (c != base)  // columns that the vector before it, or its row's last vector, has already counted
 #pragma unroll
-        for (int i = 0; i < B; i++) {
-          if (WEIGHTS)
+            for (int e = 0; e < N; e++)
+              if (c + e < base) {
+                grad[e] = 0;
 #pragma unroll
-            for (int e = 0; e < N; e++) dot[i] = fmaf((float)once.get(e), (float)v[i].get(e), dot[i]);
-          if (ROWS && ch.has(i)) {
-            const float w = ch.weight(i);
-            T* const to = dy + ch.row(i) * dyStride + c;
-            Pack<T, N> o;
+                for (int i = 0; i < B; i++) v[i].set(e, T(0));
+              }
 #pragma unroll
-            for (int e = 0; e < N; e++) o.set(e, (T)(w * (float)g.get(e)));
-            if (base < a.width) o.template store<NT>(to);
-          }
+          for (int i = 0; i < B; i++)
+#pragma unroll
+            for (int e = 0; e < N; e++) dot[i] = fmaf(grad[e], (float)v[i].get(e), dot[i]);
         }
       }
       if (!WEIGHTS) continue;
