@@ -9,6 +9,7 @@ the library is missing the import of :func:`lib` fails.
 """
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -175,8 +176,8 @@ def lib():
             ("cuttExpertCombine", [i] * 5 + [vp, vp, vp, vp, ll, vp, ll], i),
             ("cuttExpertCombineBackward", [i] * 5 + [vp] * 4 + [vp, ll] * 3 + [vp], i),
             ("cuttPageTables", [i] * 5 + [vp] * 9, i),
-            ("cuttPageStore", [i] * 3 + [z, i, i] + [vp] * 4 + [llp, vp, vp, llp], i),
-            ("cuttPageLoad", [i] * 3 + [z, i, i] + [vp] * 4 + [llp, vp, vp, llp], i)):
+            ("cuttPageStore", [i] * 3 + [z, i, i] + [vp] * 8, i),
+            ("cuttPageLoad", [i] * 3 + [z, i, i] + [vp] * 8, i)):
         f = getattr(l, name)
         f.argtypes, f.restype = args, result
     _lib = l
@@ -270,16 +271,16 @@ def cuttPageTables(requests, pageSize, tableWidth, freeCount, tokens, stream, ca
                                 slots, positions)
 
 
-_LONGS = {n: ctypes.c_longlong * n for n in (2, 3)}
+_PACK = {n: struct.Struct("%dq" % n).pack for n in (2, 3)}
 
 
 def _strides(v, n):
-    """n strides as the C functions take them (an array of that kind is passed on as it is)."""
+    """n strides as the C functions take them: 64-bit integers, which they read during the call."""
     if v is None:
         return v
     if len(v) != n:
         raise ValueError("%d strides wanted, got %d" % (n, len(v)))
-    return v if isinstance(v, ctypes.Array) else _LONGS[n](*v)
+    return _PACK[n](*v)
 
 
 def cuttPageStore(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides):
