@@ -15,28 +15,33 @@ typedef unsigned __int128 Wide;
 // Byte ranges beyond this are no device buffer's (and keep the kernels' 64-bit offsets exact).
 constexpr Wide kMaxBytes = (Wide)1 << 62;
 
-// A device buffer as a call's arguments describe it: from its first to its last byte.
+// A device buffer as a call's arguments describe it: from its first to its last byte, and of rows the bytes per row and from row to row.
 struct Span {
   uintptr_t at = 0;
   Wide bytes = 0;
+  Wide row = 0, pitch = 0;
 };
 
 bool overlap(const Span& a, const Span& b) {
-  return a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes;
+  if (!a.bytes || !b.bytes || a.at >= b.at + b.bytes || b.at >= a.at + a.bytes) return false;
+  // Rows side by side in the rows of one larger buffer: equal pitches, and neither row reaches the other's columns.
+  if (a.pitch == 0 || a.pitch != b.pitch) return true;
+  const Wide apart = (b.at >= a.at ? b.at - a.at : a.pitch - (a.at - b.at) % a.pitch) % a.pitch;  // from a's columns to b's
+  return !(apart >= a.row && apart + b.row <= a.pitch);
 }
 
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 // `count` contiguous values of `size` bytes.
 bool values(const void* p, unsigned long long count, size_t size, Span& s) {
-  s = {(uintptr_t)p, (Wide)count * size};
+  s = {(uintptr_t)p, (Wide)count * size, 0, 0};
   return count == 0 || (p && aligned(p, size) && s.bytes <= kMaxBytes);
 }
 
 // Extents in elements along each of n strided axes over `width` contiguous elements.
 bool strided(const void* p, int n, const unsigned long long* extent, const long long* stride, long long least, unsigned long long width,
              size_t size, Span& s) {
-  s = {(uintptr_t)p, 0};
+  s = {(uintptr_t)p, 0, 0, 0};
   Wide last = 0;
   for (int i = 0; i < n; i++)
     if (extent[i] == 0) return true;
@@ -49,6 +54,10 @@ bool strided(const void* p, int n, const unsigned long long* extent, const long 
     if (last > kMaxBytes) return false;
   }
   s.bytes = (last + width) * size;
+  if (n == 1 && extent[0] > 1) {
+    s.row = (Wide)width * size;
+    s.pitch = (Wide)stride[0] * size;
+  }
   return s.bytes <= kMaxBytes;
 }
 
@@ -234,10 +243,11 @@ extern "C" cuttResult cuttExpertCombineBackward(int tokens, int choices, int row
   for (const Span& r : reads)
     if (overlap(dyOut, r) || overlap(dwOut, r)) return CUTT_INVALID_PARAMETER;
   if (overlap(dyOut, dwOut)) return CUTT_INVALID_PARAMETER;
-  if (rows == 0 && n == 0) return CUTT_SUCCESS;
+  const bool anyRows = rows != 0 && dy, anyWeights = n != 0 && dweights;
+  if (!anyRows && !anyWeights) return CUTT_SUCCESS;
   const cuttHipExpertArgs a = rowArgs(tokens, choices, rows, width, position, source, weights);
-  return launched(cuttHipCombineBackward(&a, (int)type, y, (uint64_t)yStride, dout, (uint64_t)doutStride, rows ? dy : nullptr, (uint64_t)dyStride,
-                                         n ? dweights : nullptr, stream));
+  return launched(cuttHipCombineBackward(&a, (int)type, y, (uint64_t)yStride, dout, (uint64_t)doutStride, anyRows ? dy : nullptr, (uint64_t)dyStride,
+                                         anyWeights ? dweights : nullptr, stream));
 }
 
 extern "C" cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCount, int tokens, hipStream_t stream, const int* cached,

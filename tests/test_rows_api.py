@@ -90,6 +90,9 @@ def test_nothing_to_do_is_no_error(cutt):
     assert cutt.cuttExpertCombine(0, 2, 8, 16, 0, 0, 0, 0, A, 16, 0, 16) == OK
     assert cutt.cuttExpertCombineBackward(0, 2, 0, 16, 0, 0, 0, 0, 0, 0, 16, 0, 16, 0, 16, 0) == OK
     assert cutt.cuttPageStore(0, 2, 16, 2, 4, 16, 0, 0, 0, 0, (32, 16), A, 0, (512, 32, 16)) == OK
+    # no rows: gradients of rows alone are none
+    assert cutt.cuttExpertCombineBackward(*{**BACKWARD, "rows": 0, "dweights": 0}.values()) == OK
+    assert cutt.cuttExpertCombineBackward(*{**BACKWARD, "rows": 0, "dy": 0, "source": 0, "dweights": 0}.values()) == OK
     assert cutt.cuttPageStore(4, 2, 16, 2, 0, 16, 0, A, B, 0, (32, 16), 0, 0, (512, 32, 16)) == OK
 
 
@@ -145,6 +148,30 @@ def test_page_moves_refuse_rows_on_top_of_each_other(cutt):
     assert cutt.cuttPageLoad(*{**PAGES, "rows": (0, 16)}.values()) == BAD
     with pytest.raises(ValueError):
         cutt.cuttPageStore(*{**PAGES, "rows": (32,)}.values())
+
+
+SANITIZED = ["-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-g", "-O1", "-std=c++17", "-Wall", "-Wextra"]
+
+
+def test_random_arguments_under_sanitizers(tmp_path):
+    """rows_api.cpp on a stand-in for the kernels' layer that looks at what reaches it, with random and extreme arguments."""
+    exe = str(tmp_path / "rows_api_stress")
+    r = subprocess.run(["g++"] + SANITIZED + ["-I" + INCLUDE, "-I" + os.path.join(ROOT, "cutt_amd", "csrc"), os.path.join(ROOT, "tests", "rows_api_stress.cpp"),
+                        os.path.join(ROOT, "cutt_amd", "csrc", "rows_api.cpp"), "-o", exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert r.returncode == 0, r.stdout
+    r = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-3000:]
+    assert "rows api ok" in r.stdout
+
+
+def test_rows_side_by_side_do_not_overlap(cutt):
+    """Input and output as columns of one buffer: refused only where they share some (the accepted ones get as far as the launch)."""
+    def call(x, y, stride=48):
+        return cutt.cuttExpertDispatch(*{**DISPATCH, "x": x, "y": y, "xs": stride, "ys": stride}.values())
+
+    assert call(C, C + 30) == BAD and call(C, C + 66) == BAD and call(C + 64, C) != BAD and call(C, C + 32) != BAD and call(C, C + 96 * 2 + 64) != BAD
+    assert call(C + 96 + 32, C) != BAD and call(C + 96 + 30, C) == BAD and call(C + 96 - 30, C) == BAD
+    assert cutt.cuttExpertDispatch(*{**DISPATCH, "x": C, "y": C + 32, "xs": 48, "ys": 32}.values()) == BAD
 
 
 # ---- the oracle ---------------------------------------------------------------
