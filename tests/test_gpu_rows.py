@@ -299,6 +299,21 @@ def test_one_row_for_all():
     assert np.array_equal(f64(back), row_oracle.combine(np.repeat(f64(one), rows, 0), position, f64(w))[0])
 
 
+def test_rows_side_by_side():
+    """Input and output as columns of the same buffer."""
+    rng = np.random.default_rng(12)
+    position, source, rows = routing(rng, 20, 2, 4, 4, 0.2)
+    assert rows >= 20
+    p, s, w = on_gpu(position), on_gpu(source), on_gpu(rng.integers(-4, 5, (20, 2)).astype(np.float32))
+    both = on_gpu(rng.integers(-9, 10, (rows, 100)).astype(np.float32))
+    x, y = f64(both[:20, :37]), both[:, 37:74]
+    assert cutt.cuttExpertDispatch(20, 2, rows, 37, 4, st(), ptr(p), ptr(s), both.data_ptr(), 100, y.data_ptr(), 100) == 0
+    assert np.array_equal(f64(y), row_oracle.dispatch(x, position, source, np.zeros((rows, 37)))) and np.array_equal(f64(both[:20, :37]), x)
+    want = row_oracle.combine(f64(y), position, f64(w))[0]
+    assert cutt.cuttExpertCombine(20, 2, rows, 37, 0, st(), ptr(p), ptr(w), y.data_ptr(), 100, both.data_ptr(), 100) == 0
+    assert np.array_equal(f64(both[:20, :37]), want)
+
+
 def test_more_tokens_than_workgroups():
     tokens = 2 ** 21 + 77  # a launch has 2^21 workgroups for tokens at most
     g = torch.Generator(device="cuda")
