@@ -312,9 +312,11 @@ struct Choices {
 __device__ __forceinline__ uint32_t waveOfGroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // A workgroup reads a token's row once and stores it to every row that the token goes to; the last workgroups clear the empty rows.
-// Rows are bytes here: any element size, any alignment.  (Row by row of y instead, a token's row would be read once per choice.)
-// 16384 x 8 rows of 4096 bfloat16 and 8064 empty ones (1275 MB): 249 us, 216 with x left in the memory-side cache by whoever made it; rows
-// that follow each other instead of the experts' order take the same time.
+// Rows are bytes here: any element size, any alignment.  16384 x 8 rows of 4096 bfloat16 and 8064 empty ones (1275 MB): 249 us, 216 with x left in
+// the memory-side cache by whoever made it; rows that follow each other instead of the experts' order take the same time.  Row by row of y instead,
+// a token's row read once per choice: 300 us.  Rows off the 128-byte grid are slower (65536 of 2002 bytes from memory 40 us, of 2048 bytes 32): two
+// rows share a line; stores in windows on the grid, with a load of x per choice, make it 50 - 57, neighbouring tokens on one XCD 37, but
+// aligned rows 2 - 3 % slower.
 template <int N, bool NT>
 __global__ __launch_bounds__(kMaxRowThreads) void dispatchKernel(cuttHipExpertArgs a, const uint8_t* x, uint64_t xStride, uint8_t* y, uint64_t yStride,
                                                                  uint32_t tokenBlocks) {
