@@ -111,6 +111,11 @@ def test_sort_experts_of_a_range():
     check_sort(np.full((5, 2), 3), 8, 4, 8, 20)  # nobody's choice is here
 
 
+def test_sort_without_choices():
+    check_sort(np.zeros((0, 3), dtype=np.int64), 0, 5, 4, 3000)
+    check_sort(np.full((5, 1), -1), 0, 1024, 128, 20000)
+
+
 def test_sort_numbers_out_of_range():
     ids = np.array([[-1, 2 ** 62], [-2 ** 63, 1], [3, 2 ** 32], [0, 2 ** 32 + 1], [2 ** 63 - 1, -2 ** 32]])
     check_sort(ids, 0, 4, 1, 10)
@@ -409,30 +414,34 @@ def test_rows_far_apart():
         assert bool((rows[r * far:r * far + 40] == want).all())
 
 
-@pytest.mark.parametrize("tokens,choices,width", [(4200, 8, 4096), (4100, 8, 4111), (5500, 6, 4108), (8300, 4, 4096), (17000, 2, 4096)])
-def test_rows_beyond_the_memory_side_cache(tokens, choices, width):
+@pytest.mark.parametrize("tokens,choices,width,name", [(4200, 8, 4096, "bf16"), (4100, 8, 4111, "bf16"), (5500, 6, 4108, "bf16"), (8300, 4, 4096, "bf16"),
+                                                       (17000, 2, 4096, "bf16"), (33000, 1, 4096, "f16"), (4100, 8, 4098, "f16"), (6000, 7, 3300, "f16"),
+                                                       (4100, 8, 2048, "f32"), (5600, 3, 4099, "f32"), (7000, 5, 2050, "f32"), (8200, 4, 2052, "f32")])
+def test_rows_beyond_the_memory_side_cache(tokens, choices, width, name):
     """More than 256 MB of rows; whole numbers, so that every sum is exact and comparisons are bit for bit."""
+    dtype, code = TYPES[name][:2]
+    size = 4 if name == "f32" else 2
     g = torch.Generator(device="cuda")
     g.manual_seed(tokens)
     experts, align = 64, 16
     ids = torch.randint(0, experts + 2, (tokens, choices), generator=g, device="cuda", dtype=torch.int32)  # (some choices are nobody's)
     rows = cutt.cuttExpertRows(tokens, choices, experts, align)
-    assert rows * width * 2 > 256 << 20
+    assert rows * width * size > 256 << 20
     counts, offsets, position, source = run_sort(ids, 0, experts, align, rows)
     p, s = on_gpu(position.reshape(tokens, choices)), on_gpu(source)
 
     def whole(*shape):
-        return torch.randint(-8, 9, shape, generator=g, device="cuda", dtype=torch.int8).bfloat16()
+        return torch.randint(-8, 9, shape, generator=g, device="cuda", dtype=torch.int8).to(dtype)
 
     x, w = whole(tokens, width), whole(tokens, choices).float()
-    y = torch.full((rows, width), float("nan"), dtype=torch.bfloat16, device="cuda")
-    assert cutt.cuttExpertDispatch(tokens, choices, rows, width, 2, st(), ptr(p), ptr(s), ptr(x), width, ptr(y), width) == 0
+    y = torch.full((rows, width), float("nan"), dtype=dtype, device="cuda")
+    assert cutt.cuttExpertDispatch(tokens, choices, rows, width, size, st(), ptr(p), ptr(s), ptr(x), width, ptr(y), width) == 0
     token = torch.div(s, choices, rounding_mode="floor").clamp(min=0).long()
     assert torch.equal(y, x[token].masked_fill_((s < 0)[:, None], 0))
     y = torch.where((s < 0)[:, None], float("nan"), whole(rows, width))
     out, dx = torch.empty_like(x), torch.empty_like(x)
-    assert cutt.cuttExpertCombine(tokens, choices, rows, width, 2, st(), ptr(p), ptr(w), ptr(y), width, ptr(out), width) == 0
-    assert cutt.cuttExpertDispatchBackward(tokens, choices, rows, width, 2, st(), ptr(p), ptr(y), width, ptr(dx), width) == 0
+    assert cutt.cuttExpertCombine(tokens, choices, rows, width, code, st(), ptr(p), ptr(w), ptr(y), width, ptr(out), width) == 0
+    assert cutt.cuttExpertDispatchBackward(tokens, choices, rows, width, code, st(), ptr(p), ptr(y), width, ptr(dx), width) == 0
     want, plain = torch.zeros(tokens, width, device="cuda"), torch.zeros(tokens, width, device="cuda")
     dw = torch.empty_like(w)
     want_dw = torch.empty_like(w)
@@ -442,12 +451,18 @@ def test_rows_beyond_the_memory_side_cache(tokens, choices, width):
         want += torch.where(there, w[:, k:k + 1] * row, 0.0)
         plain += row
         want_dw[:, k] = (row * x.float()).sum(1)
-    assert torch.equal(out, want.bfloat16()) and torch.equal(dx, plain.bfloat16())
+    assert torch.equal(out, want.to(dtype)) and torch.equal(dx, plain.to(dtype))
     dy = torch.full_like(y, float("nan"))
-    assert cutt.cuttExpertCombineBackward(tokens, choices, rows, width, 2, st(), ptr(p), ptr(s), ptr(w), ptr(y), width, ptr(x), width, ptr(dy), width,
+    assert cutt.cuttExpertCombineBackward(tokens, choices, rows, width, code, st(), ptr(p), ptr(s), ptr(w), ptr(y), width, ptr(x), width, ptr(dy), width,
                                           ptr(dw)) == 0
     scale = torch.where(s >= 0, w.view(-1)[s.clamp(min=0).long()], 0.0)
-    assert torch.equal(dy, (x[token].float() * scale[:, None]).bfloat16()) and torch.equal(dw, want_dw)
+    want_dy = (x[token].float() * scale[:, None]).to(dtype)
+    assert torch.equal(dy, want_dy) and torch.equal(dw, want_dw)
+    dy.fill_(float("nan"))
+    dw.fill_(float("nan"))
+    assert cutt.cuttExpertCombineBackward(tokens, choices, rows, width, code, st(), ptr(p), ptr(s), ptr(w), 0, 0, ptr(x), width, ptr(dy), width, 0) == 0
+    assert cutt.cuttExpertCombineBackward(tokens, choices, rows, width, code, st(), ptr(p), 0, 0, ptr(y), width, ptr(x), width, 0, 0, ptr(dw)) == 0
+    assert torch.equal(dy, want_dy) and torch.equal(dw, want_dw)
 
 
 @pytest.mark.parametrize("layout", ["slot", "head"])
