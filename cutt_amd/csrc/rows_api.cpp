@@ -245,8 +245,9 @@ extern "C" cuttResult cuttExpertCombineBackward(int tokens, int choices, int row
   if (overlap(dyOut, dwOut)) return CUTT_INVALID_PARAMETER;
   const bool anyRows = rows != 0 && dy, anyWeights = n != 0 && dweights;
   if (!anyRows && !anyWeights) return CUTT_SUCCESS;
-  const cuttHipExpertArgs a = rowArgs(tokens, choices, rows, width, position, source, weights);
-  return launched(cuttHipCombineBackward(&a, (int)type, y, (uint64_t)yStride, dout, (uint64_t)doutStride, anyRows ? dy : nullptr, (uint64_t)dyStride,
+  // (what is not used was not checked and does not go on)
+  const cuttHipExpertArgs a = rowArgs(tokens, choices, rows, width, position, anyRows ? source : nullptr, anyRows ? weights : nullptr);
+  return launched(cuttHipCombineBackward(&a, (int)type, anyWeights ? y : nullptr, (uint64_t)yStride, dout, (uint64_t)doutStride, anyRows ? dy : nullptr, (uint64_t)dyStride,
                                          anyWeights ? dweights : nullptr, stream));
 }
 

@@ -64,6 +64,8 @@ extern "C" int cuttHipCombineBackward(const cuttHipExpertArgs* a, int type, cons
   need(dy || dw, "nothing to do reached the layer");
   need(!dy || (a->rows && a->source && (!a->tokens || a->weights)), "backward dy");
   need(!dw || a->tokens, "backward dw");
+  need(dy || (!a->weights && !a->source), "buffers that were not checked");
+  need(dw || !y, "rows that were not checked");
   const uint64_t size = type == CUTT_ROW_F32 ? 4 : 2;
   rows(dout, a->tokens, ds, a->width, size, "backward dout");
   if (dy) rows(dy, a->rows, dys, a->width, size, "backward dy");
