@@ -252,11 +252,12 @@ SortPlan planSort(uint32_t n, uint32_t align, uint32_t rows) {
 // ---------------------------------------------------------------------------
 // Rows to experts and back.  Sums of a few products per element of a row: all of it is bound by memory.  Every row is read once and written once (HBM
 // bytes by the counters equal to the algorithm's within 1 %), 16 bytes per lane at any alignment.  A workgroup takes a token and has a
-// lane for every vector of its row, up to 512: combine of 2048 x 8 rows of 4096 bfloat16 31.4 us with 512 lanes, 32.1 with 256, of 16 x 8 rows of 8192
-// 4.7 and 5.7.  Neighbouring tokens to the workgroups of one XCD: 208 -> 218 us for combine of 16384 x 8 rows, so the workgroups keep their order.
+// lane for every vector of its row, up to 1024: combine of 16 x 8 rows of 8192 bfloat16 5.7 us with 256 lanes, 4.7 with 512, 4.3 with 1024, of
+// 8192 x 8 rows 217, 212, 208; dispatch of 256 x 8 rows 11.1 us with 512, 8.6 with 1024.  The gradient of combine needs more registers and takes 512 at most (16 x
+// 8 rows 7.2 us, 7.6 with 1024), and so does dispatch past the caches (8192 x 8 rows 210 us, 215 with 1024).  Neighbouring tokens to the workgroups of one XCD: 208 -> 218 us for combine of 16384 x 8 rows, so the workgroups keep their order.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kMaxRowThreads = 512, kMaxRowWaves = kMaxRowThreads / 64;
-constexpr uint32_t kMaxBlocks = 1u << 21;  // of tokens, and of empty rows: all lanes of a launch have to be fewer than 2^32
+constexpr uint32_t kMaxRowThreads = 1024, kHalfRowThreads = 512;
+constexpr uint32_t kMaxBlocks = 1u << 20;  // of tokens, and of empty rows: all lanes of a launch have to be fewer than 2^32
 static_assert(2ull * kMaxBlocks * kMaxRowThreads <= CUTT_HIP_MAX_GRID_LANES, "a larger grid would be cut without an error");
 
 // Rows without a source, which hold zeros.  Workgroup `block` of `blocks` looks at kEmptyRows rows at a time; a wavefront clears a row.  16384 x 8 rows of 512
@@ -410,10 +411,10 @@ __device__ __forceinline__ float sumOverWave(float (&v)[B]) {
 // 8192 x 8 rows of 4096 bfloat16 (1142 MB): 219 us, 5.2 TB/s, as much read as written; a wavefront per token, without LDS: 241 us; four choices at a
 // time, for fewer registers and more wavefronts: 232.
 template <typename T, int N, int B, bool ROWS, bool WEIGHTS, bool NT>
-__global__ __launch_bounds__(kMaxRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
-                                                                     T* dy, uint64_t dyStride, float* dweights, uint32_t tokenBlocks) {
+__global__ __launch_bounds__(kHalfRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
+                                                                      T* dy, uint64_t dyStride, float* dweights, uint32_t tokenBlocks) {
   constexpr int P = B <= 1 ? 1 : B <= 2 ? 2 : B <= 4 ? 4 : 8;
-  __shared__ float part[kMaxRowWaves][P];
+  __shared__ float part[kHalfRowThreads / 64][P];
   if (ROWS && blockIdx.x >= tokenBlocks) {
     clearEmptyRows<T, N, NT>(a, dy, dyStride, blockIdx.x - tokenBlocks, gridDim.x - tokenBlocks);
     return;
@@ -511,10 +512,10 @@ extern "C" int cuttHipExpertSort(const cuttHipSortArgs* a, void* stream) {
 
 namespace {
 
-// Lanes for rows of `width` elements, N per lane: one pass over a row if kMaxRowThreads suffice.
-uint32_t rowThreads(uint32_t width, uint32_t n) {
+// Lanes for rows of `width` elements, n per lane: one pass over a row if `most` lanes suffice.
+uint32_t rowThreads(uint32_t width, uint32_t n, uint32_t most) {
   const uint64_t waves = ((uint64_t)width + 64 * n - 1) / (64 * n);
-  return waves < kMaxRowWaves ? (uint32_t)waves * 64 : kMaxRowThreads;
+  return waves < most / 64 ? (uint32_t)waves * 64 : most;
 }
 
 // Rows on the 128-byte grid.  Off it, lines that two rows share have to meet in a cache: 65536 rows of 4100 bytes 69 us through the caches, 73 past them.
@@ -532,8 +533,8 @@ extern "C" int cuttHipDispatch(const cuttHipExpertArgs* a, uint32_t elemSize, co
     b.width = (uint32_t)(bytes - at < kMaxPiece ? bytes - at : kMaxPiece);
     const bool nt = pastCaches(a->rows, bytes) && onLines(y, yStride * elemSize);
     auto kernel = b.width < 16 ? dispatchKernel<1, false> : nt ? dispatchKernel<16, true> : dispatchKernel<16, false>;
-    if (int e = launchRows(kernel, grid, rowThreads(b.width, b.width < 16 ? 1 : 16), 0, stream, b, (const uint8_t*)x + at, xStride * elemSize, (uint8_t*)y + at,
-                           yStride * elemSize, tokenBlocks))
+    const uint32_t threads = rowThreads(b.width, b.width < 16 ? 1 : 16, nt ? kHalfRowThreads : kMaxRowThreads);
+    if (int e = launchRows(kernel, grid, threads, 0, stream, b, (const uint8_t*)x + at, xStride * elemSize, (uint8_t*)y + at, yStride * elemSize, tokenBlocks))
       return e;
   }
   return 0;
@@ -543,7 +544,7 @@ namespace {
 
 template <typename T, int N>
 int combine(const cuttHipExpertArgs* a, const T* y, uint64_t yStride, T* out, uint64_t outStride, bool nt, void* stream) {
-  auto go = [&](auto kernel) { return launchRows(kernel, blocksFor(a->tokens), rowThreads(a->width, N), 0, stream, *a, y, yStride, out, outStride); };
+  auto go = [&](auto kernel) { return launchRows(kernel, blocksFor(a->tokens), rowThreads(a->width, N, kMaxRowThreads), 0, stream, *a, y, yStride, out, outStride); };
   if constexpr (N == 1) {
     return go(combineKernel<T, 1, 1, false>);
   } else {
@@ -574,8 +575,8 @@ int combineBackward(const cuttHipExpertArgs* a, const T* y, uint64_t yStride, co
                     bool nt, void* stream) {
   const uint32_t tokenBlocks = blocksFor(a->tokens);
   auto go = [&](auto kernel) {
-    return launchRows(kernel, tokenBlocks + (dy ? emptyBlocks(a->rows) : 0), rowThreads(a->width, N), 0, stream, *a, y, yStride, dout, doutStride, dy, dyStride, dweights,
-                      tokenBlocks);
+    return launchRows(kernel, tokenBlocks + (dy ? emptyBlocks(a->rows) : 0), rowThreads(a->width, N, kHalfRowThreads), 0, stream, *a, y, yStride, dout, doutStride, dy,
+                      dyStride, dweights, tokenBlocks);
   };
   if constexpr (N == 1) {
     if (!dy) return go(combineBackwardKernel<T, 1, 1, false, true, false>);

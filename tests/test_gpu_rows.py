@@ -320,7 +320,7 @@ def test_rows_side_by_side():
 
 
 def test_more_tokens_than_workgroups():
-    tokens = 2 ** 21 + 77  # a launch has 2^21 workgroups for tokens at most
+    tokens = 2 ** 21 + 77  # a launch has 2^20 workgroups for tokens at most
     g = torch.Generator(device="cuda")
     g.manual_seed(3)
     rows = tokens + 5
