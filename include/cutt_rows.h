@@ -64,7 +64,8 @@ size_t cuttExpertSortWorkspace(int tokens, int choices, int experts);
  *   ids               [tokens, choices]
  *   counts            [experts]            offsets  [experts + 1]
  *   position          [tokens, choices]    source   [rows]
- *   workspace         cuttExpertSortWorkspace bytes, aligned to 4; its contents need no preparation
+ *   workspace         cuttExpertSortWorkspace bytes, aligned to 4; its contents need no preparation and mean nothing afterwards.  Calls that
+ *                     may overlap on the GPU need one each
  * offsets[experts] > rows says that rows did not suffice.
  */
 cuttResult cuttExpertSort(int tokens, int choices, int firstExpert, int experts, int align, int rows, size_t sizeofId,
