@@ -15,26 +15,34 @@ typedef unsigned __int128 Wide;
 // Byte ranges beyond this are no device buffer's (and keep the kernels' 64-bit offsets exact).
 constexpr Wide kMaxBytes = (Wide)1 << 62;
 
-// A device buffer as a call's arguments describe it: from its first to its last byte, and of rows the bytes per row and from row to row.
+// A device buffer as a call's arguments describe it: from its first to its last byte, as rows of `row` bytes every `pitch` bytes; one piece (values, a
+// row, a row that is read again and again) has no pitch.
 struct Span {
   uintptr_t at = 0;
   Wide bytes = 0;
   Wide row = 0, pitch = 0;
 };
 
+// Whether two buffers may share a byte.  Rows lie apart if they do so modulo a number that divides both pitches (one piece takes any): they are then columns side
+// by side in the rows of a larger buffer.  Exact for equal pitches and for one piece; other pitches may be taken for overlapping where they are not.
 bool overlap(const Span& a, const Span& b) {
   if (!a.bytes || !b.bytes || a.at >= b.at + b.bytes || b.at >= a.at + a.bytes) return false;
-  // Rows side by side in the rows of one larger buffer: equal pitches, and neither row reaches the other's columns.
-  if (a.pitch == 0 || a.pitch != b.pitch) return true;
-  const Wide apart = (b.at >= a.at ? b.at - a.at : a.pitch - (a.at - b.at) % a.pitch) % a.pitch;  // from a's columns to b's
-  return !(apart >= a.row && apart + b.row <= a.pitch);
+  Wide pitch = a.pitch;
+  for (Wide r = b.pitch; r;) {  // the greatest common divisor
+    const Wide rest = pitch % r;
+    pitch = r;
+    r = rest;
+  }
+  if (!pitch) return true;
+  const Wide apart = (b.at >= a.at ? b.at - a.at : pitch - (a.at - b.at) % pitch) % pitch;  // from a's columns to b's
+  return !(apart >= a.row && apart + b.row <= pitch);
 }
 
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 // `count` contiguous values of `size` bytes.
 bool values(const void* p, unsigned long long count, size_t size, Span& s) {
-  s = {(uintptr_t)p, (Wide)count * size, 0, 0};
+  s = {(uintptr_t)p, (Wide)count * size, (Wide)count * size, 0};
   return count == 0 || (p && aligned(p, size) && s.bytes <= kMaxBytes);
 }
 
@@ -53,7 +61,7 @@ bool strided(const void* p, int n, const unsigned long long* extent, const long 
     last += (Wide)(extent[i] - 1) * (Wide)stride[i];
     if (last > kMaxBytes) return false;
   }
-  s.bytes = (last + width) * size;
+  s.bytes = s.row = (last + width) * size;
   if (n == 1 && extent[0] > 1) {
     s.row = (Wide)width * size;
     s.pitch = (Wide)stride[0] * size;

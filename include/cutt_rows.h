@@ -12,7 +12,8 @@
  *     copies nothing and does not synchronise, and can be captured into a HIP graph (make the call once before
  *     the capture, so that the library's code object is loaded).  The caller orders work of other streams;
  *   - buffers are aligned to their elements; any such address and any stride will do, multiples of 16 bytes are
- *     fastest.  What a call writes must not overlap what it reads;
+ *     fastest.  What a call writes must not overlap what it reads; columns side by side in one buffer of rows (equal strides,
+ *     or a single row on either side) do not;
  *   - no buffer's contents can make a call touch memory outside the buffers as their sizes, strides and
  *     counts describe them: positions, slots, experts and pages out of range count as absent;
  *   - the results do not depend on timing: equal inputs give equal bits.

@@ -319,6 +319,23 @@ def test_rows_side_by_side():
     assert np.array_equal(f64(both[:20, :37]), want)
 
 
+@pytest.mark.parametrize("tokens,choices,experts", [(1, 1, 1), (1, 3, 5), (4, 2, 1)])
+def test_few_rows_side_by_side(tokens, choices, experts):
+    """Columns of the same buffer where one side, or both, is a single row."""
+    rng = np.random.default_rng(choices)
+    position, source, rows = routing(rng, tokens, choices, experts, 1, 0)
+    if experts == 1:  # (the row of the last choice alone)
+        position[:], source, rows = -1, np.array([tokens * choices - 1], dtype=np.int32), 1
+        position[-1, -1] = 0
+    p, s, w = on_gpu(position), on_gpu(source), on_gpu(rng.integers(-4, 5, (tokens, choices)).astype(np.float32))
+    both = on_gpu(rng.integers(-9, 10, (max(rows, tokens), 100)).astype(np.float32))
+    x, y = f64(both[:tokens, :37]), both[:rows, 37:74]
+    assert cutt.cuttExpertDispatch(tokens, choices, rows, 37, 4, st(), ptr(p), ptr(s), both.data_ptr(), 100, y.data_ptr(), 100) == 0
+    assert np.array_equal(f64(y), row_oracle.dispatch(x, position, source, np.zeros((rows, 37)))) and np.array_equal(f64(both[:tokens, :37]), x)
+    assert cutt.cuttExpertCombine(tokens, choices, rows, 37, 0, st(), ptr(p), ptr(w), y.data_ptr(), 100, both.data_ptr(), 100) == 0
+    assert np.array_equal(f64(both[:tokens, :37]), row_oracle.combine(f64(y), position, f64(w))[0])
+
+
 def test_more_tokens_than_workgroups():
     tokens = 2 ** 21 + 77  # a launch has 2^20 workgroups for tokens at most
     g = torch.Generator(device="cuda")

@@ -1,0 +1,82 @@
+"""Which calls the row operators accept, on a stand-in for the kernels' layer: nothing is launched, so the addresses can be made up."""
+import ctypes
+import itertools
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+OK, BAD = 0, 2
+A, B, C, D, E, F, G = (0x10000000 * i for i in range(1, 8))
+
+
+@pytest.fixture(scope="module")
+def stub_lib(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("stub") / "librows.so")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-Wall", "-Wextra", "-I" + os.path.join(ROOT, "cutt_amd", "csrc"),
+                           os.path.join(ROOT, "tests", "rows_layer_stub.cpp"), os.path.join(ROOT, "cutt_amd", "csrc", "rows_api.cpp"), "-o", out])
+    return ctypes.CDLL(out)
+
+
+@pytest.fixture
+def rows(cutt, stub_lib, monkeypatch):
+    """The binding on the stand-in; `rows.launches()` counts what got through since the last look."""
+    for name in dir(cutt):
+        if name.startswith(("cuttExpert", "cuttPage")):
+            f, real = getattr(stub_lib, name), getattr(cutt.lib(), name)
+            f.argtypes, f.restype = real.argtypes, real.restype
+    monkeypatch.setattr(cutt.api, "lib", lambda: stub_lib)
+    count = ctypes.c_int.in_dll(stub_lib, "stubLaunches")
+    count.value = 0
+
+    def launches():
+        n, count.value = count.value, 0
+        return n
+
+    monkeypatch.setattr(cutt, "launches", launches, raising=False)
+    return cutt
+
+
+def bytes_of(at, rows, pitch, width):
+    return {at + r * pitch + i for r in range(rows) for i in range(width)}
+
+
+# ---- rows side by side -----------------------------------------------------------
+def test_rows_side_by_side_from_one_row_on(rows):
+    """Input and output as columns of one buffer, for every pair of row counts: refused where a byte is shared, and only there."""
+    for tokens, count in itertools.product((1, 2, 3), (1, 2, 5)):
+        for at in range(-104, 320, 6):  # 16 elements of 2 bytes, 48 from row to row
+            shared = bytes_of(D + at, tokens, 96, 32) & bytes_of(D, count, 96, 32)
+            want = BAD if shared else OK
+            assert rows.cuttExpertDispatch(tokens, 2, count, 16, 2, 0, A, B, D + at, 48, D, 48) == want, (tokens, count, at)
+            assert rows.cuttExpertCombine(count, 2, tokens, 16, 2, 0, A, B, D + at, 48, D, 48) == want, (tokens, count, at)
+            assert rows.launches() == (0 if shared else 2)
+
+
+def test_one_row_for_all_beside_the_rows(rows):
+    """A row that is read for every token (stride 0) in the columns beside the output; 16 columns of 48."""
+    for at in range(0, 192, 4):
+        shared = bytes_of(D + at, 1, 0, 32) & bytes_of(D, 8, 96, 32)
+        assert rows.cuttExpertDispatch(5, 2, 8, 16, 2, 0, A, B, D + at, 0, D, 48) == (BAD if shared else OK), at
+
+
+def test_rows_of_two_pitches(rows):
+    """What is accepted shares no byte, whatever the two pitches are; a pitch that divides the other is told apart exactly."""
+    for xs, ys in itertools.product((0, 16, 32, 48, 64, 96), repeat=2):
+        if ys < 16:
+            continue
+        for tokens, count, at in itertools.product((1, 4), (1, 3), range(-400, 400, 16)):
+            shared = bytes_of(D + at, tokens, 2 * xs, 32) & bytes_of(D, count, 2 * ys, 32)
+            code = rows.cuttExpertDispatch(tokens, 2, count, 16, 2, 0, A, B, D + at, xs, D, ys)
+            assert code == BAD or not shared, (xs, ys, tokens, count, at)
+            if tokens == 1 or count == 1 or xs == ys or xs == 0:
+                assert code == (BAD if shared else OK), (xs, ys, tokens, count, at)
+
+
+def test_values_in_the_columns_beside_the_rows(rows):
+    """Contiguous values inside a gap between rows are apart from them, values that reach the next row are not."""
+    assert rows.cuttExpertDispatch(4, 1, 8, 16, 2, 0, D + 32, B, C, 16, D, 48) == OK  # 16 bytes of positions in a gap of 64
+    assert rows.cuttExpertDispatch(4, 1, 8, 16, 2, 0, D + 80, B, C, 16, D, 48) == OK
+    assert rows.cuttExpertDispatch(4, 1, 8, 16, 2, 0, D + 84, B, C, 16, D, 48) == BAD
+    assert rows.cuttExpertDispatch(40, 1, 8, 16, 2, 0, D + 32, B, C, 16, D, 48) == BAD  # longer than the gap
