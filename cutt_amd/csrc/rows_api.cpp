@@ -239,21 +239,20 @@ extern "C" cuttResult cuttExpertCombineBackward(int tokens, int choices, int row
   const size_t size = sizeOf(type);
   if (!size || !rowSizes(tokens, choices, rows, width)) return CUTT_INVALID_PARAMETER;
   const unsigned long long n = (unsigned long long)tokens * choices;
-  // a buffer of no entries may be null without being left out
-  const bool wantRows = dy != nullptr || rows == 0, wantWeights = dweights != nullptr || n == 0;
-  if (!wantRows && !wantWeights) return CUTT_INVALID_PARAMETER;
+  // (a buffer of no entries may be null without being left out)
+  if (!dy && rows != 0 && !dweights && n != 0) return CUTT_INVALID_PARAMETER;
+  const bool anyRows = rows != 0 && dy, anyWeights = n != 0 && dweights;
+  // What only the other gradient needs is neither checked nor passed on.
   Span p, s, w, yIn, dIn, dyOut, dwOut;
   if (!values(position, n, 4, p) || !rowsRead(dout, tokens, doutStride, width, size, dIn)) return CUTT_INVALID_PARAMETER;
-  if (wantRows && (!values(source, rows, 4, s) || !values(weights, n, 4, w) || !rowsWritten(dy, rows, dyStride, width, size, dyOut)))
+  if (anyRows && (!values(source, rows, 4, s) || !values(weights, n, 4, w) || !rowsWritten(dy, rows, dyStride, width, size, dyOut)))
     return CUTT_INVALID_PARAMETER;
-  if (wantWeights && (!values(dweights, n, 4, dwOut) || (n && !rowsRead(y, rows, yStride, width, size, yIn)))) return CUTT_INVALID_PARAMETER;
+  if (anyWeights && (!values(dweights, n, 4, dwOut) || !rowsRead(y, rows, yStride, width, size, yIn))) return CUTT_INVALID_PARAMETER;
   const Span reads[] = {p, s, w, yIn, dIn};
   for (const Span& r : reads)
     if (overlap(dyOut, r) || overlap(dwOut, r)) return CUTT_INVALID_PARAMETER;
   if (overlap(dyOut, dwOut)) return CUTT_INVALID_PARAMETER;
-  const bool anyRows = rows != 0 && dy, anyWeights = n != 0 && dweights;
   if (!anyRows && !anyWeights) return CUTT_SUCCESS;
-  // (what is not used was not checked and does not go on)
   const cuttHipExpertArgs a = rowArgs(tokens, choices, rows, width, position, anyRows ? source : nullptr, anyRows ? weights : nullptr);
   return launched(cuttHipCombineBackward(&a, (int)type, anyWeights ? y : nullptr, (uint64_t)yStride, dout, (uint64_t)doutStride, anyRows ? dy : nullptr, (uint64_t)dyStride,
                                          anyWeights ? dweights : nullptr, stream));

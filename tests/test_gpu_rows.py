@@ -367,6 +367,14 @@ def test_combine_without_rows():
     assert bool((dw == 0).all())
 
 
+def test_gradient_of_weights_without_rows():
+    """No rows, and neither dy nor what only dy needs: every weight's gradient is zero."""
+    p, dout = on_gpu(np.array([[0, -1], [5, 2 ** 31 - 1], [1, 0]], dtype=np.int32)), torch.ones(3, 8, device="cuda")
+    dw = torch.full((7,), float(MARK), device="cuda")
+    assert cutt.cuttExpertCombineBackward(3, 2, 0, 8, 0, st(), ptr(p), 0, 0, 0, 8, ptr(dout), 8, 0, 8, ptr(dw)) == 0
+    assert dw.tolist() == [0.0] * 6 + [MARK]
+
+
 def test_gradients_against_differences():
     """Dispatch and combine are linear: with whole numbers, where 32 bits are exact, a difference of one step is the gradient."""
     rng = np.random.default_rng(4)

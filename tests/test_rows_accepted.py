@@ -80,3 +80,28 @@ def test_values_in_the_columns_beside_the_rows(rows):
     assert rows.cuttExpertDispatch(4, 1, 8, 16, 2, 0, D + 80, B, C, 16, D, 48) == OK
     assert rows.cuttExpertDispatch(4, 1, 8, 16, 2, 0, D + 84, B, C, 16, D, 48) == BAD
     assert rows.cuttExpertDispatch(40, 1, 8, 16, 2, 0, D + 32, B, C, 16, D, 48) == BAD  # longer than the gap
+
+
+# ---- gradients of combine, one of them left out ---------------------------------------
+BACKWARD = dict(tokens=4, choices=2, rows=8, width=16, type=2, stream=0, position=A, source=B, weights=C, y=D, ys=16, dout=E, douts=16, dy=F, dys=16,
+                dweights=G)
+
+
+def test_buffers_of_the_gradient_that_is_left_out(rows):
+    """Without dy neither source nor weights are used, without dweights y is not: null, misaligned or on top of another one, whatever the number of rows."""
+    for count in (0, 8):
+        for weights in (0, C + 1, G, F):
+            call = {**BACKWARD, "rows": count, "dy": 0, "source": weights, "weights": weights, "dys": -3}
+            assert rows.cuttExpertCombineBackward(*call.values()) == OK, (count, weights)
+            assert rows.launches() == 1
+        assert rows.cuttExpertCombineBackward(*{**BACKWARD, "rows": count, "dweights": 0, "y": F, "ys": -1}.values()) == OK
+        assert rows.launches() == (1 if count else 0)
+    for count, left in itertools.product((0, 8), ({}, {"source": 0}, {"weights": 0}, {"weights": C + 2})):
+        assert rows.cuttExpertCombineBackward(*{**BACKWARD, "rows": count, **left}.values()) == (BAD if left and count else OK)
+    assert rows.cuttExpertCombineBackward(*{**BACKWARD, "dy": 0, "dweights": 0}.values()) == BAD
+
+
+def test_gradients_of_no_tokens(rows):
+    none = {**BACKWARD, "tokens": 0, "position": 0, "weights": 0, "dout": 0}
+    assert rows.cuttExpertCombineBackward(*{**none, "dweights": 0, "y": 0}.values()) == OK and rows.launches() == 1  # empty rows to clear
+    assert rows.cuttExpertCombineBackward(*{**none, "dy": 0, "source": 0}.values()) == OK and rows.launches() == 0
