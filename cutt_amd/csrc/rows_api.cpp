@@ -121,7 +121,6 @@ cuttResult movePages(bool load, int tokens, int heads, int width, size_t sizeofT
   if (tokens < 0 || heads < 1 || width < 1 || !opaqueSize(sizeofType) || pages < 0 || pageSize < 1 || !rowStrides || !cacheStrides)
     return CUTT_INVALID_PARAMETER;
   if ((Wide)heads * (Wide)width * sizeofType > INT_MAX) return CUTT_INVALID_PARAMETER;
-  if ((v == nullptr) != (vCache == nullptr)) return CUTT_INVALID_PARAMETER;
   const long long least[2] = {load ? width : 0, load ? 0 : width};  // of the rows' strides, of the caches'
   const unsigned long long rowExtent[2] = {(unsigned long long)tokens, (unsigned long long)heads};
   const unsigned long long cacheExtent[3] = {(unsigned long long)pages, (unsigned long long)pageSize, (unsigned long long)heads};
@@ -129,7 +128,7 @@ cuttResult movePages(bool load, int tokens, int heads, int width, size_t sizeofT
   if (!values(slots, tokens, 8, s)) return CUTT_INVALID_PARAMETER;
   const void* const rowsAt[2] = {k, v};
   const void* const cacheAt[2] = {kCache, vCache};
-  const int tensors = v ? 2 : 1;
+  const int tensors = v || vCache ? 2 : 1;  // (one of the two may be null if it has no entries)
   for (int i = 0; i < tensors; i++)
     if (!strided(rowsAt[i], 2, rowExtent, rowStrides, least[0], width, sizeofType, row[i]) ||
         !strided(cacheAt[i], 3, cacheExtent, cacheStrides, least[1], width, sizeofType, cache[i]))
@@ -150,7 +149,7 @@ cuttResult movePages(bool load, int tokens, int heads, int width, size_t sizeofT
   a.slots = (const int64_t*)slots;
   for (int i = 0; i < 2; i++) {
     a.rows[i] = const_cast<void*>(rowsAt[i]);
-    a.cache[i] = const_cast<void*>(cacheAt[i]);
+    a.cache[i] = const_cast<void*>(pages ? cacheAt[i] : rowsAt[i]);  // (a cache without pages is never touched and may be null)
   }
   // (the stride of an axis with one entry is never used: it may be anything)
   a.tokenStride = tokens > 1 ? (uint64_t)rowStrides[0] : 0;

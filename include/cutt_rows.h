@@ -143,7 +143,7 @@ cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCo
  *   rowStrides[2]     elements from token to token and from head to head of k and v
  *   cacheStrides[3]   elements from page to page, slot to slot and head to head of the caches; any order of the three
  *                     ([pages, pageSize, heads, width], [pages, heads, pageSize, width], ...)
- *   v, vCache         NULL both: only k moves
+ *   v, vCache         NULL both: only k moves (a buffer of no tokens or of no pages may be NULL by itself)
  * The strides are host arrays, read during the call.
  */
 cuttResult cuttPageStore(int tokens, int heads, int width, size_t sizeofType, int pages, int pageSize, hipStream_t stream,

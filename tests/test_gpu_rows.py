@@ -640,6 +640,16 @@ def test_page_moves_shared_heads_and_misaligned_bases():
     assert int(cache[0]) == MARK and np.array_equal(cache[1:].cpu().numpy(), want.reshape(-1))
 
 
+def test_load_from_a_cache_without_pages():
+    """A cache of no pages, whose address is null: every row is zeros."""
+    slots = on_gpu(np.array([0, -1, 5], dtype=np.int64))
+    out = torch.full((2, 3 * 4 * 24 + 1), MARK, dtype=torch.int16, device="cuda")
+    assert cutt.cuttPageLoad(3, 4, 24, 2, 0, 16, st(), ptr(slots), ptr(out[0]), ptr(out[1]), (96, 24), 0, 0, (16 * 96, 96, 24)) == 0
+    assert bool((out[:, :-1] == 0).all()) and bool((out[:, -1] == MARK).all())
+    assert cutt.cuttPageStore(0, 4, 24, 2, 1, 3, st(), 0, 0, 0, (96, 24), out[0].data_ptr(), out[1].data_ptr(), (288, 96, 24)) == 0  # no tokens
+    assert bool((out[:, :-1] == 0).all()) and bool((out[:, -1] == MARK).all())
+
+
 def test_pages_far_apart():
     """A cache of more than 2^32 elements, and more than 2^31 slots."""
     far = 2 ** 32 + 48

@@ -105,3 +105,32 @@ def test_gradients_of_no_tokens(rows):
     none = {**BACKWARD, "tokens": 0, "position": 0, "weights": 0, "dout": 0}
     assert rows.cuttExpertCombineBackward(*{**none, "dweights": 0, "y": 0}.values()) == OK and rows.launches() == 1  # empty rows to clear
     assert rows.cuttExpertCombineBackward(*{**none, "dy": 0, "source": 0}.values()) == OK and rows.launches() == 0
+
+
+# ---- rows in pages -----------------------------------------------------------------
+PAGES = dict(tokens=4, heads=2, width=16, size=2, pages=4, page=16, stream=0, slots=A, k=B, v=C, rows=(32, 16), kc=D, vc=E, cache=(512, 32, 16))
+
+
+def pages_field(stub_lib, name):
+    """A field of what the layer was last asked to move."""
+    class Args(ctypes.Structure):
+        _fields_ = ([(n, ctypes.c_uint32) for n in ("tokens", "heads", "width", "elemSize", "pages", "pageSize")] + [("slots", ctypes.c_void_p)] +
+                    [(n, ctypes.c_void_p * 2) for n in ("rows", "cache")] +
+                    [(n, ctypes.c_uint64) for n in ("tokenStride", "headStride", "pageStride", "slotStride", "cacheHeadStride")] + [("load", ctypes.c_int)])
+    return getattr(Args.in_dll(stub_lib, "stubPages"), name)
+
+
+def test_empty_buffers_may_be_null(rows, stub_lib):
+    """Keys and values of no tokens, or a cache of no pages: null without a say in whether values move too."""
+    for call in (rows.cuttPageStore, rows.cuttPageLoad):
+        for null in ({"k": 0, "v": 0}, {"v": 0}, {"k": 0, "v": 0, "slots": 0}, {"k": 0, "v": 0, "vc": 0}):
+            assert call(*{**PAGES, "tokens": 0, **null}.values()) == OK, null
+        assert call(*{**PAGES, "tokens": 0, "k": 0, "v": 0, "vc": E + 1}.values()) == BAD  # (what has entries is checked)
+        assert rows.launches() == 0
+        for null in ({"kc": 0, "vc": 0}, {"kc": 0}, {"vc": 0}):
+            assert call(*{**PAGES, "pages": 0, **null}.values()) == OK, null
+            assert rows.launches() == (1 if call is rows.cuttPageLoad else 0)
+            if call is rows.cuttPageLoad:  # zeros for keys and values
+                assert list(pages_field(stub_lib, "rows")) == [B, C] and pages_field(stub_lib, "pages") == 0
+        for null in ({"k": 0}, {"v": 0}, {"vc": 0}, {"kc": 0}):
+            assert call(*{**PAGES, **null}.values()) == BAD, null
