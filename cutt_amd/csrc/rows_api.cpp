@@ -46,10 +46,19 @@ bool values(const void* p, unsigned long long count, size_t size, Span& s) {
   return count == 0 || (p && aligned(p, size) && s.bytes <= kMaxBytes);
 }
 
-// Extents in elements along each of n strided axes over `width` contiguous elements.
-bool strided(const void* p, int n, const unsigned long long* extent, const long long* stride, long long least, unsigned long long width,
-             size_t size, Span& s) {
+// The axes of a strided buffer that have more than one entry, the smallest stride first; in elements.
+struct Axes {
+  int n = 0;
+  unsigned long long extent[3];
+  Wide stride[3];
+};
+
+// Extents and strides in elements along each of n axes over `width` contiguous elements.  Strides are 0 and more; of what is written each has to lead past
+// everything that the smaller ones reach, so that no two entries share an element.
+bool strided(const void* p, int n, const unsigned long long* extent, const long long* stride, bool written, unsigned long long width, size_t size, Span& s,
+             Axes& axes) {
   s = {(uintptr_t)p, 0, 0, 0};
+  axes.n = 0;
   Wide last = 0;
   for (int i = 0; i < n; i++)
     if (extent[i] == 0) return true;
@@ -57,9 +66,21 @@ bool strided(const void* p, int n, const unsigned long long* extent, const long 
   if (!p || !aligned(p, size)) return false;
   for (int i = 0; i < n; i++) {
     if (extent[i] == 1) continue;
-    if (stride[i] < least) return false;
+    if (stride[i] < 0) return false;
     last += (Wide)(extent[i] - 1) * (Wide)stride[i];
     if (last > kMaxBytes) return false;
+    int at = axes.n++;
+    for (; at > 0 && axes.stride[at - 1] > (Wide)stride[i]; at--) {
+      axes.extent[at] = axes.extent[at - 1];
+      axes.stride[at] = axes.stride[at - 1];
+    }
+    axes.extent[at] = extent[i];
+    axes.stride[at] = (Wide)stride[i];
+  }
+  Wide reach = width;
+  for (int i = 0; written && i < axes.n; i++) {
+    if (axes.stride[i] < reach) return false;
+    reach += (axes.extent[i] - 1) * axes.stride[i];
   }
   s.bytes = s.row = (last + width) * size;
   if (n == 1 && extent[0] > 1) {
@@ -70,10 +91,25 @@ bool strided(const void* p, int n, const unsigned long long* extent, const long 
 }
 
 bool rowsRead(const void* p, unsigned long long count, long long stride, unsigned long long width, size_t size, Span& s) {
-  return strided(p, 1, &count, &stride, 0, width, size, s);
+  Axes axes;
+  return strided(p, 1, &count, &stride, false, width, size, s, axes);
 }
 bool rowsWritten(const void* p, unsigned long long count, long long stride, unsigned long long width, size_t size, Span& s) {
-  return strided(p, 1, &count, &stride, (long long)width, width, size, s);
+  Axes axes;
+  return strided(p, 1, &count, &stride, true, width, size, s, axes);
+}
+
+// Whether two buffers of the same written axes, the second one `apart` bytes behind the first, share a byte: whether `apart` is less than a row off a sum of
+// steps along the axes.  What the smaller strides reach either way, with a row, stays within one step of an axis, so that only the two multiples of its stride
+// around what is left to go can lead there.
+bool meet(__int128 apart, const Axes& axes, int n, unsigned long long width, size_t size) {
+  if (n == 0) return (apart < 0 ? -apart : apart) < (__int128)width * (__int128)size;
+  const __int128 stride = (__int128)(axes.stride[n - 1] * size), most = axes.extent[n - 1] - 1;
+  __int128 steps = apart / stride;
+  if (steps * stride > apart) steps--;  // (rounded down)
+  for (int i = 0; i < 2; i++, steps++)
+    if (steps <= most && -steps <= most && meet(apart - steps * stride, axes, n - 1, width, size)) return true;
+  return false;
 }
 
 size_t sizeOf(cuttRowType type) { return type == CUTT_F32 ? 4 : type == CUTT_F16 || type == CUTT_BF16 ? 2 : 0; }
@@ -121,23 +157,26 @@ cuttResult movePages(bool load, int tokens, int heads, int width, size_t sizeofT
   if (tokens < 0 || heads < 1 || width < 1 || !opaqueSize(sizeofType) || pages < 0 || pageSize < 1 || !rowStrides || !cacheStrides)
     return CUTT_INVALID_PARAMETER;
   if ((Wide)heads * (Wide)width * sizeofType > INT_MAX) return CUTT_INVALID_PARAMETER;
-  const long long least[2] = {load ? width : 0, load ? 0 : width};  // of the rows' strides, of the caches'
   const unsigned long long rowExtent[2] = {(unsigned long long)tokens, (unsigned long long)heads};
   const unsigned long long cacheExtent[3] = {(unsigned long long)pages, (unsigned long long)pageSize, (unsigned long long)heads};
   Span s, row[2], cache[2];
+  Axes rowAxes, cacheAxes;  // (the same for both tensors)
   if (!values(slots, tokens, 8, s)) return CUTT_INVALID_PARAMETER;
   const void* const rowsAt[2] = {k, v};
   const void* const cacheAt[2] = {kCache, vCache};
   const int tensors = v || vCache ? 2 : 1;  // (one of the two may be null if it has no entries)
   for (int i = 0; i < tensors; i++)
-    if (!strided(rowsAt[i], 2, rowExtent, rowStrides, least[0], width, sizeofType, row[i]) ||
-        !strided(cacheAt[i], 3, cacheExtent, cacheStrides, least[1], width, sizeofType, cache[i]))
+    if (!strided(rowsAt[i], 2, rowExtent, rowStrides, load, width, sizeofType, row[i], rowAxes) ||
+        !strided(cacheAt[i], 3, cacheExtent, cacheStrides, !load, width, sizeofType, cache[i], cacheAxes))
       return CUTT_INVALID_PARAMETER;
   for (int i = 0; i < tensors; i++) {
     for (int j = 0; j < tensors; j++)
       if (overlap(row[i], cache[j])) return CUTT_INVALID_PARAMETER;
     if (overlap(load ? row[i] : cache[i], s)) return CUTT_INVALID_PARAMETER;
   }
+  const Span* const out = load ? row : cache;
+  const Axes& outAxes = load ? rowAxes : cacheAxes;
+  if (out[0].bytes && out[1].bytes && meet((__int128)out[1].at - (__int128)out[0].at, outAxes, outAxes.n, width, sizeofType)) return CUTT_INVALID_PARAMETER;
   if (tokens == 0 || (!load && pages == 0)) return CUTT_SUCCESS;
   cuttHipPageArgs a;
   a.tokens = (uint32_t)tokens;

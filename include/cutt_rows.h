@@ -143,6 +143,8 @@ cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCo
  *   rowStrides[2]     elements from token to token and from head to head of k and v
  *   cacheStrides[3]   elements from page to page, slot to slot and head to head of the caches; any order of the three
  *                     ([pages, pageSize, heads, width], [pages, heads, pageSize, width], ...)
+ *                     What is written must not lie on top of itself: each stride of its axes of more than one entry leads past all that the
+ *                     smaller ones reach, and the two written tensors share no element (they may interleave)
  *   v, vCache         NULL both: only k moves (a buffer of no tokens or of no pages may be NULL by itself)
  * The strides are host arrays, read during the call.
  */

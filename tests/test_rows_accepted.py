@@ -134,3 +134,55 @@ def test_empty_buffers_may_be_null(rows, stub_lib):
                 assert list(pages_field(stub_lib, "rows")) == [B, C] and pages_field(stub_lib, "pages") == 0
         for null in ({"k": 0}, {"v": 0}, {"vc": 0}, {"kc": 0}):
             assert call(*{**PAGES, **null}.values()) == BAD, null
+
+
+def cells(at, extents, strides, width, size):
+    """Every byte of every row, as often as it is named."""
+    return [at + (sum(i * s for i, s in zip(index, strides)) + w) * size + b for index in itertools.product(*map(range, extents)) for w in range(width)
+            for b in range(size)]
+
+
+def test_page_moves_write_every_element_once(rows):
+    """Strides of the written side: what is accepted names no byte twice, and strides in any order that nest are accepted."""
+    nested = 0
+    for heads, tokens, pages, page in ((2, 4, 2, 3), (3, 2, 3, 1), (1, 3, 2, 2), (2, 1, 1, 4)):
+        for strides in itertools.product((0, 2, 3, 4, 6, 8, 12), repeat=3):
+            args = (heads, 3, 2, pages, page, 0, A)
+            twice = len(cells(0, (pages, page, heads), strides, 3, 2)) != len(set(cells(0, (pages, page, heads), strides, 3, 2)))
+            code = rows.cuttPageStore(tokens, *args, B, 0, (24, 3), D, 0, strides)
+            assert code == BAD if twice else True, (heads, pages, page, strides)
+            reach, fits = 3, True
+            for stride, extent in sorted((s, e) for s, e in zip(strides, (pages, page, heads)) if e > 1):
+                fits, reach = fits and stride >= reach, reach + (extent - 1) * stride
+            assert code == (OK if fits else BAD), (heads, pages, page, strides)
+            nested += fits
+            two = strides[:2]
+            code = rows.cuttPageLoad(tokens, *args, B, 0, two, D, 0, (0, 0, 0))
+            named = cells(0, (tokens, heads), two, 3, 2)
+            assert code == BAD if len(named) != len(set(named)) else True, (tokens, heads, two)
+    assert nested > 50
+
+
+def test_page_moves_write_two_tensors(rows):
+    """Keys and values that are written: refused exactly where they share a byte, interleaved ones included."""
+    layouts = [((2, 3, 2), (48, 16, 8)), ((2, 3, 2), (48, 8, 24)), ((3, 2, 2), (8, 24, 48)), ((2, 1, 3), (40, 0, 10)), ((1, 1, 1), (0, 0, 0)), ((2, 2, 2), (100, 37, 9))]
+    for (pages, page, heads), strides in layouts:
+        first = set(cells(0, (pages, page, heads), strides, 4, 2))
+        for apart in range(-340, 340, 2):
+            shared = any(b + apart in first for b in first)
+            code = rows.cuttPageStore(5, heads, 4, 2, pages, page, 0, A, B, C, (32, 4), D, D + apart, strides)
+            assert code == (BAD if shared else OK), (strides, apart)
+            two = (strides[0], strides[2])
+            rows_named = set(cells(0, (pages, heads), two, 4, 2))
+            shared = any(b + apart in rows_named for b in rows_named)
+            code = rows.cuttPageLoad(pages, heads, 4, 2, 7, 3, 0, A, D, D + apart, two, B, C, (64, 16, 8))
+            assert code == (BAD if shared else OK), (two, apart)
+    assert rows.cuttPageLoad(*{**PAGES, "v": B}.values()) == BAD and rows.cuttPageStore(*{**PAGES, "vc": D}.values()) == BAD
+    # what is only read may be the same for both
+    assert rows.cuttPageStore(*{**PAGES, "v": B}.values()) == OK and rows.cuttPageLoad(*{**PAGES, "vc": D}.values()) == OK
+    # keys and values beside each other in every slot, far apart and beyond 32 bits
+    for far in (1 << 20, 1 << 33, 1 << 50):
+        wide = {**PAGES, "cache": (far * 64, far, 32)}
+        assert rows.cuttPageStore(*{**wide, "kc": D, "vc": D + 32}.values()) == OK
+        assert rows.cuttPageStore(*{**wide, "kc": D, "vc": D + 2 * far}.values()) == BAD
+        assert rows.cuttPageStore(*{**wide, "kc": D, "vc": D + 2 * far * 16}.values()) == OK  # behind the last slot of a page
