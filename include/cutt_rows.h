@@ -16,7 +16,9 @@
  *     or a single row on either side) do not;
  *   - no buffer's contents can make a call touch memory outside the buffers as their sizes, strides and
  *     counts describe them: positions, slots, experts and pages out of range count as absent;
- *   - the results do not depend on timing: equal inputs give equal bits.
+ *   - the results do not depend on timing: equal inputs give equal bits.  The one exception is a place that the caller's numbers
+ *     name twice for writing (a row in two positions, a slot of two tokens): each of its elements is then one of those
+ *     that were to go there, not said which, nor that its neighbours have the same origin.
  *
  * All functions return CUTT_SUCCESS, CUTT_INVALID_PARAMETER (null, misaligned or overlapping buffers, sizes out of range;
  * nothing was launched) or CUTT_INTERNAL_ERROR (the HIP runtime refused a launch).
@@ -76,7 +78,7 @@ cuttResult cuttExpertSort(int tokens, int choices, int firstExpert, int experts,
 /*
  * y[position[t, k], :] = x[t, :], and zeros in every row with source < 0.
  *   x [tokens, width] with row stride xStride, y [rows, width] with row stride yStride
- * position and source are those of one cuttExpertSort; rows whose source is >= 0 but that no position names are not written.
+ * position and source are those of one cuttExpertSort, here and below; rows whose source is >= 0 but that no position names are not written.
  */
 cuttResult cuttExpertDispatch(int tokens, int choices, int rows, int width, size_t sizeofType, hipStream_t stream,
                               const int* position, const int* source, const void* x, long long xStride, void* y,
@@ -136,7 +138,8 @@ cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCo
 /*
  * Rows into pages: for every token t and head h, with s = slots[t],
  *   kCache[s / pageSize, s % pageSize, h, :] = k[t, h, :], the same for v.  Tokens whose slot is not in
- * 0 .. pages * pageSize - 1 are left out.  Slots that are named twice get one of the rows, not said which.
+ * 0 .. pages * pageSize - 1 are left out.  The others' slots should differ, as cuttPageTables makes them from pages that differ: a slot that two
+ * tokens name may end up with elements of either, in k and in v (see above).
  * A token's heads * width * sizeofType bytes are fewer than 2^31.
  *
  *   slots             [tokens], 64-bit

@@ -640,6 +640,25 @@ def test_page_moves_shared_heads_and_misaligned_bases():
     assert int(cache[0]) == MARK and np.array_equal(cache[1:].cpu().numpy(), want.reshape(-1))
 
 
+@pytest.mark.parametrize("layout", ["slot", "head"])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.int64])
+def test_slots_of_two_tokens(dtype, layout):
+    """Every element of a slot that several tokens name is one of theirs at that place; all other slots are what they are without that."""
+    tokens, heads, width, page, pages = 900, 3, 700, 8, 100
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    slots = torch.randperm(pages * page, generator=g, device="cuda").repeat(2)[:tokens]  # the first 100 twice
+    rows = torch.randint(0, 100, (2, tokens, heads, width), generator=g, device="cuda").to(dtype)
+    caches = torch.full((2, pages, page, heads, width) if layout == "slot" else (2, pages, heads, page, width), MARK, dtype=dtype, device="cuda")
+    at = caches if layout == "slot" else caches.transpose(2, 3)
+    assert cutt.cuttPageStore(tokens, heads, width, rows.element_size(), pages, page, st(), ptr(slots), ptr(rows[0]), ptr(rows[1]), rows.stride()[1:3],
+                              ptr(caches[0]), ptr(caches[1]), at.stride()[1:4]) == 0
+    got = at.reshape(2, pages * page, heads, width)[:, slots[:800]]
+    twice, once = got[:, :100], got[:, 100:]
+    assert torch.equal(once, rows[:, 100:800])
+    assert bool(((twice == rows[:, :100]) | (twice == rows[:, 800:])).all())
+
+
 def test_load_from_a_cache_without_pages():
     """A cache of no pages, whose address is null: every row is zeros."""
     slots = on_gpu(np.array([0, -1, 5], dtype=np.int64))
