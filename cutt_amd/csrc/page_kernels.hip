@@ -200,8 +200,9 @@ struct PageMove {
 };
 
 // A workgroup takes a few tokens' rows of all heads at a time, N bytes per lane.  TOKENS_INNER: neighbouring lanes go from a row to the next
-// token's of the same head, else to the next head's: as the cache has its slots and heads.  20000 tokens, 4 heads of 80, slots of a head together:
-// 12.6 us so, 13.7 the other way; the load above 175 and 178.
+// token's of the same head, else to the next head's: as the written side has them.  131072 tokens, 8 heads of 80 bfloat16, whose rows share lines, pages
+// [page, slot, head]: into pages of one slot 130 us so and 151 the other way, out of them into [head, token] 128 and 155, out of pages of 16 slots 125 and
+// 151; [page, head, slot] into [token, head] 125 and 134.  Rows on the grid hardly care: that last one of 128 elements 169 us so, 167 the other way.
 template <int N, bool LOAD, bool TOKENS_INNER, bool NT>
 __global__ __launch_bounds__(kThreads) void pageMoveKernel(PageMove a) {
   uint8_t* const rows = a.rows[blockIdx.y];
@@ -282,7 +283,7 @@ extern "C" int cuttHipPageMove(const cuttHipPageArgs* a, void* stream) {
   if (m.groupTokens < 1) m.groupTokens = 1;
   if (m.groupTokens > m.tokens) m.groupTokens = m.tokens;
   m.groupItems = m.groupTokens * perToken;
-  const bool tokensInner = a->slotStride < a->cacheHeadStride;
+  const bool tokensInner = cuttHipTokensInner(a);
   m.byVecs = cuttHipMakeDivisor(m.vecs);
   m.byInner = cuttHipMakeDivisor(tokensInner ? m.groupTokens : m.heads);
   m.pages = a->pages;

@@ -69,6 +69,14 @@ typedef struct cuttHipPageArgs {
   int load;               /* 0: rows to the cache, 1: back */
 } cuttHipPageArgs;
 
+/* Whether neighbouring lanes go from a row to the next token's of the same head rather than to the next head's: as those come closer on the side that is
+ * written, where lines that two rows share have to be put together (pageMoveKernel).  The next token's slot is the next one of its
+ * page, or the next page where a page has one slot.  The stride of an axis with one entry is 0, and either order is then the same. */
+static inline int cuttHipTokensInner(const cuttHipPageArgs* a) {
+  if (a->load) return a->tokenStride < a->headStride;
+  return (a->pageSize > 1 ? a->slotStride : a->pageStride) < a->cacheHeadStride;
+}
+
 int cuttHipPageMove(const cuttHipPageArgs* a, void* stream);
 
 #ifdef __cplusplus

@@ -16,4 +16,5 @@ int cuttHipCombineBackward(const cuttHipExpertArgs* a, int, const void*, uint64_
 }
 int cuttHipPageTables(const cuttHipTablesArgs*, void*) { return stubLaunches++, 0; }
 int cuttHipPageMove(const cuttHipPageArgs* a, void*) { return stubPages = *a, stubLaunches++, 0; }
+int stubTokensInner() { return cuttHipTokensInner(&stubPages); }
 }

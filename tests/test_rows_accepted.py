@@ -186,3 +186,17 @@ def test_page_moves_write_two_tensors(rows):
         assert rows.cuttPageStore(*{**wide, "kc": D, "vc": D + 32}.values()) == OK
         assert rows.cuttPageStore(*{**wide, "kc": D, "vc": D + 2 * far}.values()) == BAD
         assert rows.cuttPageStore(*{**wide, "kc": D, "vc": D + 2 * far * 16}.values()) == OK  # behind the last slot of a page
+
+
+def test_order_of_the_lanes(rows, stub_lib):
+    """Lanes go to the next token or to the next head, whichever comes closer on the written side; behind a page's only slot that is the next page."""
+    def inner(call, **change):
+        assert call(*{**PAGES, **change}.values()) == OK, change
+        return stub_lib.stubTokensInner()
+
+    by_slot, by_head, pages_by_slot, pages_by_head = (32, 16), (16, 64), (512, 32, 16), (512, 16, 256)
+    for other in (by_slot, by_head):
+        assert inner(rows.cuttPageStore, rows=other, cache=pages_by_slot) == 0 and inner(rows.cuttPageStore, rows=other, cache=pages_by_head) == 1
+        assert inner(rows.cuttPageStore, rows=other, page=1, cache=(32, -5, 16)) == 0 and inner(rows.cuttPageStore, rows=other, page=1, cache=(16, 99, 64)) == 1
+    for other, page in ((pages_by_slot, 16), (pages_by_head, 16), ((32, 32, 16), 1)):
+        assert inner(rows.cuttPageLoad, rows=by_slot, cache=other, page=page) == 0 and inner(rows.cuttPageLoad, rows=by_head, cache=other, page=page) == 1
