@@ -89,6 +89,14 @@ __device__ __forceinline__ uint64_t sameKey(uint32_t key) {
   return (uint64_t)high << 32 | low;
 }
 
+// What the wavefront's lanes have written to LDS before is seen by its other lanes after.  LDS serves a wavefront's accesses in their order: this only
+// keeps the compiler from changing it.
+__device__ __forceinline__ void waveFence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <typename Id, bool COUNTED, int ITEMS, int BITS>
 __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs a, SortPlan p) {
   constexpr uint32_t kSortItems = ITEMS, kSortPart = kSortThreads * ITEMS;
@@ -197,7 +205,7 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
   uint32_t* const mine = seen + wave * (E + 1);
   for (uint64_t part = from; part < to; part += kSortPart) {
     for (uint32_t e = lane; e <= E; e += 64) mine[e] = 0;
-    __builtin_amdgcn_wave_barrier();
+    waveFence();
     uint32_t rank[kSortItems];
     if (part != from) take(part);
 #pragma unroll
@@ -205,10 +213,10 @@ __global__ __launch_bounds__(kSortThreads) void expertSortKernel(cuttHipSortArgs
       const uint64_t same = sameKey<BITS>(expert[j]);
       const uint32_t below = __popcll(same & ((1ull << lane) - 1));
       const uint32_t before = mine[expert[j]];  // (the wavefront's lanes all read, then one lane per expert writes)
-      __builtin_amdgcn_wave_barrier();
+      waveFence();
       rank[j] = before + below;
       if (below == 0) mine[expert[j]] = before + __popcll(same);
-      __builtin_amdgcn_wave_barrier();
+      waveFence();
     }
     __syncthreads();
     for (uint32_t e = tid; e < E; e += kSortThreads) {
