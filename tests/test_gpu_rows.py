@@ -100,6 +100,29 @@ def test_sort_large(tokens, choices, experts):
         assert np.array_equal(g, w)
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("experts", [60, 64, 200, 255, 256, 1000, 1024])
+@pytest.mark.parametrize("tokens,choices", [(65536, 1), (65537, 1), (20000, 5), (16384, 8), (43691, 3), (131073, 1)])
+def test_sort_choices_per_lane(tokens, choices, experts, dtype):
+    """Around the numbers of choices at which a lane takes more of them, for every width of an expert's number; a range of experts out of more."""
+    rng = np.random.default_rng(tokens + experts)
+    first, rows = 7, cutt.cuttExpertRows(tokens, choices, experts, 16)
+    ids = rng.integers(0, experts + 20, (tokens, choices))
+    ids[rng.random((tokens, choices)) < 0.3] = first + experts // 2  # (an expert in demand)
+    got = run_sort(torch.as_tensor(ids, dtype=dtype, device="cuda"), first, experts, 16, rows)
+    key = ids.reshape(-1) - first
+    key = np.where((key >= 0) & (key < experts), key, experts)
+    counts = np.bincount(key, minlength=experts + 1)[:experts]
+    offsets = np.concatenate([[0], np.cumsum((counts + 15) // 16 * 16)])
+    order = np.argsort(key, kind="stable")[:counts.sum()]
+    rank = np.arange(order.size) - (np.cumsum(counts) - counts)[key[order]]
+    position, source = np.full(key.size, -1), np.full(rows, -1)
+    position[order] = offsets[key[order]] + rank
+    source[position[order]] = order
+    for name, g, w in zip(("counts", "offsets", "position", "source"), got, (counts, offsets, position, source)):
+        assert np.array_equal(g, w), name
+
+
 def test_sort_one_expert_takes_all():
     check_sort(np.full((700, 3), 4), 0, 9, 32, 2200)
 
