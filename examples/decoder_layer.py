@@ -51,6 +51,7 @@ class Routing:
                                   workspace.data_ptr(), space), "cuttExpertSort")
 
 
+# Rows move and add up linearly, so the gradients' own gradients are the same operators again.
 class Dispatch(torch.autograd.Function):
     """x [tokens, width] -> rows [routing.rows, width]"""
 
@@ -65,11 +66,24 @@ class Dispatch(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, drows):
-        r, drows = ctx.routing, drows.contiguous()
-        dx = torch.empty(r.tokens, drows.shape[1], dtype=drows.dtype, device=drows.device)
-        check(cutt.cuttExpertDispatchBackward(r.tokens, r.choices, r.rows, drows.shape[1], row_type(drows), stream(), r.position.data_ptr(),
-                                              drows.data_ptr(), drows.stride(0), dx.data_ptr(), dx.stride(0)), "cuttExpertDispatchBackward")
-        return dx, None
+        return Gather.apply(drows, ctx.routing), None
+
+
+class Gather(torch.autograd.Function):
+    """rows [routing.rows, width] -> [tokens, width], the sums of the tokens' rows: the gradient of Dispatch, and Dispatch is its own."""
+
+    @staticmethod
+    def forward(ctx, rows, routing):
+        r, rows = routing, rows.contiguous()
+        ctx.routing = r
+        out = torch.empty(r.tokens, rows.shape[1], dtype=rows.dtype, device=rows.device)
+        check(cutt.cuttExpertDispatchBackward(r.tokens, r.choices, r.rows, rows.shape[1], row_type(rows), stream(), r.position.data_ptr(),
+                                              rows.data_ptr(), rows.stride(0), out.data_ptr(), out.stride(0)), "cuttExpertDispatchBackward")
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        return Dispatch.apply(dout, ctx.routing), None
 
 
 class Combine(torch.autograd.Function):
@@ -77,9 +91,9 @@ class Combine(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, rows, weights, routing):
-        r, rows, weights = routing, rows.contiguous(), weights.contiguous()
-        ctx.routing = r
+        ctx.routing = r = routing
         ctx.save_for_backward(rows, weights)
+        rows, weights = rows.contiguous(), weights.contiguous()
         out = torch.empty(r.tokens, rows.shape[1], dtype=rows.dtype, device=rows.device)
         check(cutt.cuttExpertCombine(r.tokens, r.choices, r.rows, rows.shape[1], row_type(rows), stream(), r.position.data_ptr(),
                                      weights.data_ptr(), rows.data_ptr(), rows.stride(0), out.data_ptr(), out.stride(0)), "cuttExpertCombine")
@@ -87,13 +101,37 @@ class Combine(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        r, dout = ctx.routing, dout.contiguous()
         rows, weights = ctx.saved_tensors
-        drows, dweights = torch.empty_like(rows), torch.empty_like(weights)
+        return (*CombineGradients.apply(rows, weights, dout, ctx.routing, *ctx.needs_input_grad[:2]), None)
+
+
+class CombineGradients(torch.autograd.Function):
+    """The gradients of Combine for its rows and its weights, either of them None if it is not wanted."""
+
+    @staticmethod
+    def forward(ctx, rows, weights, dout, routing, of_rows, of_weights):
+        ctx.routing = r = routing
+        ctx.save_for_backward(rows, weights, dout)
+        rows, weights, dout = rows.contiguous(), weights.contiguous(), dout.contiguous()
+        drows = torch.empty_like(rows) if of_rows else None
+        dweights = torch.empty_like(weights) if of_weights else None
         check(cutt.cuttExpertCombineBackward(r.tokens, r.choices, r.rows, rows.shape[1], row_type(rows), stream(), r.position.data_ptr(),
                                              r.source.data_ptr(), weights.data_ptr(), rows.data_ptr(), rows.stride(0), dout.data_ptr(), dout.stride(0),
-                                             drows.data_ptr(), drows.stride(0), dweights.data_ptr()), "cuttExpertCombineBackward")
-        return drows, dweights, None
+                                             drows.data_ptr() if of_rows else 0, rows.stride(0), dweights.data_ptr() if of_weights else 0),
+              "cuttExpertCombineBackward")
+        return drows, dweights
+
+    @staticmethod
+    def backward(ctx, a, b):
+        rows, weights, dout = ctx.saved_tensors
+        r, drows, dweights, ddout = ctx.routing, None, None, []
+        if a is not None:
+            dweights = CombineGradients.apply(a, weights, dout, r, False, True)[1]
+            ddout.append(Combine.apply(a, weights, r))
+        if b is not None:
+            drows = CombineGradients.apply(rows, b, dout, r, True, False)[0]
+            ddout.append(Combine.apply(rows, b, r))
+        return drows, dweights, sum(ddout[1:], ddout[0]), None, None, None
 
 
 class Experts:
@@ -255,16 +293,22 @@ def serve(width=256, heads=4, experts=8, choices=2, prompts=(37, 1, 64, 0, 5), s
     return worst, biggest
 
 
-def train(width=128, hidden=256, experts=8, choices=3, tokens=100, dtype=torch.float32, seed=0):
-    """The largest relative difference (norms) between the gradients through the operators and through plain torch operations."""
+def train(width=128, hidden=256, experts=8, choices=3, tokens=100, dtype=torch.float32, seed=0, second=False):
+    """The largest relative difference (norms) between the gradients through the operators and through plain torch operations.  second: between the
+    gradients of the gradients' products with a fixed direction."""
     torch.manual_seed(seed)
     layer = Experts(width, hidden, experts, choices, dtype=dtype)
     x = torch.randn(tokens, width, device="cuda").to(dtype).requires_grad_()
     goal = torch.randn(tokens, width, device="cuda")
+    leaves = [x] + layer.parameters()
+    along = [torch.randn_like(t) for t in leaves]
     grads = []
     for way in (layer, layer.plain):
         loss = ((way(x).float() - goal) ** 2).mean()
-        grads.append(torch.autograd.grad(loss, [x] + layer.parameters()))
+        grad = torch.autograd.grad(loss, leaves, create_graph=second)
+        if second:
+            grad = torch.autograd.grad(sum((g * d).sum() for g, d in zip(grad, along)), leaves)
+        grads.append(grad)
     return max(float((a.double() - b.double()).norm() / b.double().norm()) for a, b in zip(*grads))
 
 

@@ -28,3 +28,29 @@ def test_gradients(experts, choices, tokens):
 
 def test_gradients_in_bfloat16():
     assert decoder_layer.train(dtype=torch.bfloat16) <= 2.0 ** -5
+
+
+@pytest.mark.parametrize("experts,choices,tokens", [(8, 3, 100), (1, 1, 5), (16, 16, 33), (4, 2, 1)])
+def test_second_derivatives(experts, choices, tokens):
+    """Through the gradients once more: twice the chain."""
+    assert decoder_layer.train(experts=experts, choices=choices, tokens=tokens, second=True) <= 6e-4
+
+
+@pytest.mark.parametrize("of_rows,of_weights", [(True, False), (False, True), (True, True)])
+def test_one_gradient_of_combine(of_rows, of_weights):
+    """Rows and weights that are not contiguous, one of them or both with a gradient; small whole numbers, so that every sum is exact."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+
+    def whole(*shape):
+        return torch.randint(-4, 5, shape, generator=g, device="cuda").float()
+
+    routing = decoder_layer.Routing(torch.randint(0, 4, (9, 2), generator=g, device="cuda"), 4, 4)
+    rows, weights, dout = whole(16, routing.rows).requires_grad_(of_rows), whole(2, 9).requires_grad_(of_weights), whole(9, 16)
+    leaves = [t for t in (rows, weights) if t.requires_grad]
+    at = routing.position.long()
+    assert int(at.min()) >= 0
+    got = torch.autograd.grad((decoder_layer.Combine.apply(rows.t(), weights.t(), routing) * dout).sum(), leaves)
+    want = torch.autograd.grad(((rows.t()[at] * weights.t()[:, :, None]).sum(1) * dout).sum(), leaves)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
