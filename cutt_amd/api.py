@@ -230,45 +230,61 @@ def cuttDestroy(handle):
 
 
 # The row operators (include/cutt_rows.h): device buffers are integer addresses (0 or None: NULL), the functions return the
-# result code.
+# result code.  Negative sizes and sizes of 2^31 and more are refused here: ctypes would drop their upper bits without a word.
 def cuttExpertRows(tokens, choices, experts, align):
     """Rows that suffice for any choice of experts; -1 for arguments out of range."""
-    return lib().cuttExpertRows(tokens, choices, experts, align)
+    if (tokens | choices | experts | align) >> 31:
+        return -1
+    return (_lib or lib()).cuttExpertRows(tokens, choices, experts, align)
 
 
 def cuttExpertSortWorkspace(tokens, choices, experts):
     """Bytes of workspace that cuttExpertSort needs."""
-    return lib().cuttExpertSortWorkspace(tokens, choices, experts)
+    if (tokens | choices | experts) >> 31:
+        return 0
+    return (_lib or lib()).cuttExpertSortWorkspace(tokens, choices, experts)
 
 
 def cuttExpertSort(tokens, choices, firstExpert, experts, align, rows, sizeofId, stream, ids, counts, offsets, position, source,
                    workspace=0, workspaceBytes=0):
-    return lib().cuttExpertSort(tokens, choices, firstExpert, experts, align, rows, sizeofId, stream, ids, counts, offsets, position,
-                                source, workspace, workspaceBytes)
+    if (tokens | choices | experts | align | rows | sizeofId) >> 31 or not -2 ** 31 <= firstExpert < 2 ** 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttExpertSort(tokens, choices, firstExpert, experts, align, rows, sizeofId, stream, ids, counts, offsets, position,
+                                          source, workspace, workspaceBytes)
 
 
 def cuttExpertDispatch(tokens, choices, rows, width, sizeofType, stream, position, source, x, xStride, y, yStride):
-    return lib().cuttExpertDispatch(tokens, choices, rows, width, sizeofType, stream, position, source, x, xStride, y, yStride)
+    if (tokens | choices | rows | width | sizeofType) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttExpertDispatch(tokens, choices, rows, width, sizeofType, stream, position, source, x, xStride, y, yStride)
 
 
 def cuttExpertDispatchBackward(tokens, choices, rows, width, type, stream, position, dy, dyStride, dx, dxStride):
-    return lib().cuttExpertDispatchBackward(tokens, choices, rows, width, type, stream, position, dy, dyStride, dx, dxStride)
+    if (tokens | choices | rows | width | type) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttExpertDispatchBackward(tokens, choices, rows, width, type, stream, position, dy, dyStride, dx, dxStride)
 
 
 def cuttExpertCombine(tokens, choices, rows, width, type, stream, position, weights, y, yStride, out, outStride):
-    return lib().cuttExpertCombine(tokens, choices, rows, width, type, stream, position, weights, y, yStride, out, outStride)
+    if (tokens | choices | rows | width | type) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttExpertCombine(tokens, choices, rows, width, type, stream, position, weights, y, yStride, out, outStride)
 
 
 def cuttExpertCombineBackward(tokens, choices, rows, width, type, stream, position, source, weights, y, yStride, dout, doutStride, dy,
                               dyStride, dweights):
-    return lib().cuttExpertCombineBackward(tokens, choices, rows, width, type, stream, position, source, weights, y, yStride, dout,
-                                           doutStride, dy, dyStride, dweights)
+    if (tokens | choices | rows | width | type) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttExpertCombineBackward(tokens, choices, rows, width, type, stream, position, source, weights, y, yStride, dout,
+                                                     doutStride, dy, dyStride, dweights)
 
 
 def cuttPageTables(requests, pageSize, tableWidth, freeCount, tokens, stream, cached, added, freePages, tables, starts, used, slots,
                    positions):
-    return lib().cuttPageTables(requests, pageSize, tableWidth, freeCount, tokens, stream, cached, added, freePages, tables, starts, used,
-                                slots, positions)
+    if (requests | pageSize | tableWidth | freeCount | tokens) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttPageTables(requests, pageSize, tableWidth, freeCount, tokens, stream, cached, added, freePages, tables, starts, used,
+                                          slots, positions)
 
 
 _PACK = {n: struct.Struct("%dq" % n).pack for n in (2, 3)}
@@ -284,13 +300,17 @@ def _strides(v, n):
 
 
 def cuttPageStore(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides):
-    return lib().cuttPageStore(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, _strides(rowStrides, 2), kCache,
-                               vCache, _strides(cacheStrides, 3))
+    if (tokens | heads | width | sizeofType | pages | pageSize) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttPageStore(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, _strides(rowStrides, 2), kCache,
+                                         vCache, _strides(cacheStrides, 3))
 
 
 def cuttPageLoad(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, rowStrides, kCache, vCache, cacheStrides):
-    return lib().cuttPageLoad(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, _strides(rowStrides, 2), kCache,
-                              vCache, _strides(cacheStrides, 3))
+    if (tokens | heads | width | sizeofType | pages | pageSize) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttPageLoad(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, _strides(rowStrides, 2), kCache,
+                                        vCache, _strides(cacheStrides, 3))
 
 
 def get_plan_info(handle):

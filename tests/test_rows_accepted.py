@@ -26,7 +26,7 @@ def rows(cutt, stub_lib, monkeypatch):
         if name.startswith(("cuttExpert", "cuttPage")):
             f, real = getattr(stub_lib, name), getattr(cutt.lib(), name)
             f.argtypes, f.restype = real.argtypes, real.restype
-    monkeypatch.setattr(cutt.api, "lib", lambda: stub_lib)
+    monkeypatch.setattr(cutt.api, "_lib", stub_lib)
     count = ctypes.c_int.in_dll(stub_lib, "stubLaunches")
     count.value = 0
 
@@ -200,3 +200,26 @@ def test_order_of_the_lanes(rows, stub_lib):
         assert inner(rows.cuttPageStore, rows=other, page=1, cache=(32, -5, 16)) == 0 and inner(rows.cuttPageStore, rows=other, page=1, cache=(16, 99, 64)) == 1
     for other, page in ((pages_by_slot, 16), (pages_by_head, 16), ((32, 32, 16), 1)):
         assert inner(rows.cuttPageLoad, rows=by_slot, cache=other, page=page) == 0 and inner(rows.cuttPageLoad, rows=by_head, cache=other, page=page) == 1
+
+
+# ---- the binding ---------------------------------------------------------------------
+def test_sizes_beyond_32_bits_are_refused(rows):
+    """A size is refused whatever its lower 32 bits say."""
+    calls = [(rows.cuttExpertSort, (4, 2, 0, 8, 1, 8, 4, 0, A, B, C, D, E), (0, 1, 2, 3, 4, 5, 6)), (rows.cuttExpertDispatch, (4, 2, 8, 16, 2, 0, A, B, C, 16, D, 16), range(5)),
+             (rows.cuttExpertDispatchBackward, (4, 2, 8, 16, 2, 0, A, C, 16, D, 16), range(5)),
+             (rows.cuttExpertCombine, (4, 2, 8, 16, 2, 0, A, B, C, 16, D, 16), range(5)), (rows.cuttExpertCombineBackward, tuple(BACKWARD.values()), range(5)),
+             (rows.cuttPageTables, (4, 16, 8, 8, 32, 0, A, B, C, D, E, F, G, 0), range(5)), (rows.cuttPageStore, tuple(PAGES.values()), range(6)),
+             (rows.cuttPageLoad, tuple(PAGES.values()), range(6))]
+    for call, args, sizes in calls:
+        assert call(*args) == OK and rows.launches() == 1, call
+        for i in sizes:
+            for more in (2 ** 32, -2 ** 32, 2 ** 63, 2 ** 64, 3 * 2 ** 64):
+                assert call(*args[:i], args[i] + more, *args[i + 1:]) == BAD, (call, i, more)
+    assert rows.launches() == 0
+    assert rows.cuttExpertSort(4, 2, -2 ** 31, 8, 1, 8, 4, 0, A, B, C, D, E) == OK and rows.cuttExpertSort(4, 2, 2 ** 31 - 1, 8, 1, 8, 4, 0, A, B, C, D, E) == OK
+    for i in range(4):
+        sizes = [3, 2, 8, 16]
+        assert rows.cuttExpertRows(*sizes) == 6 + 6 * 15
+        sizes[i] += 2 ** 32
+        assert rows.cuttExpertRows(*sizes) == -1
+    assert rows.cuttExpertSortWorkspace(2 ** 13 + 2 ** 32, 1, 8) == 0 and rows.cuttExpertSortWorkspace(2 ** 13, 1, 8) > 0
