@@ -3,7 +3,7 @@
  * choices, the move of the tokens' rows to their experts, the weighted sum back, and the gradients of both.
  *
  * Times in the comments: MI355X, back to back in a graph, the buffers of several calls in rotation unless they say "the same buffers"; a launch
- * of an empty kernel takes about 2.2 us there, a copy of 512 MB runs at 5.3 - 5.6 TB/s.
+ * of an empty kernel takes about 2.2 us there, this library's copy of 512 MiB runs at 6.4 TB/s, torch's at 5.3.
  */
 #include <algorithm>
 
@@ -27,20 +27,22 @@ using Number = std::integral_constant<int, X>;
 // workgroup adds the columns up.  Whole numbers only: the order of the LDS atomics does not show.
 //
 // Bound by launches and latencies, not by its bytes (262144 choices are 4 MB, under 1 us): the choices, the table, the scan over the
-// experts and the scattered 4-byte stores of `source` wait for each other.  512 choices 3.8 us, 4096 5.4, 65536 8.1, 262144 10.9, 1048576
-// 19 (128 or 256 experts, two launches from the third on).
+// experts and the scattered 4-byte stores of `source` wait for each other.  512 choices 3.9 us (segments of 64
+// rows; of single rows, in one workgroup, 4.6), 4096 5.4 (128 experts), 65536 8.3, 262144 11.7, 1048576
+// 23.0 (256 experts, two launches); 262144 choices of 512 experts 13.6, of 1024 17.3.  Of the 11.7 (17.3) the sums over the table take 2.0 (6.7), matching
+// 1.0 (1.2), the stores of `source` 1.2 (1.5).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
-constexpr uint32_t kCountLoads = 16;   // a workgroup's loads of the table go out at once: 262144 choices 25.9 -> 11.3 us against 8 loads of 4 bytes
+constexpr uint32_t kCountLoads = 16;   // a workgroup's loads of the table go out at once: 262144 choices 11.7 us, of 1024 experts 17.3; 12.1 and 18.7 with 4
 constexpr uint32_t kSortGroups = 256;  // at most: beyond, stretches get longer and the table does not grow
-// Choices that every workgroup counts for itself.  8192 choices, 256 experts: 7.1 us so, 7.9 with the table, but 17.0 and 7.7 where all are one expert's
+// Choices that every workgroup counts for itself.  8192 choices, 256 experts: 7.2 us so, 7.9 with the table, but 16.8 and 7.7 where all are one expert's
 // and their LDS atomics follow each other.
 constexpr uint32_t kCountAll = 4096;
-// More workgroups for the rows that stay empty: 512 choices, 128 experts' segments in multiples of 64 rows, 5.2 us with one workgroup, 3.8 with 8.
+// More workgroups for the rows that stay empty: 512 choices, 128 experts' segments in multiples of 64 rows, 5.1 us with one workgroup, 3.9 with 8.
 constexpr uint32_t kRowsPerGroup = 1024, kRowGroups = 16;
-// Choices that a lane places at a time: one up to the first number, two up to the second, four beyond.  More per lane are more steps in turn (512
-// choices: 5.2 us with one, 6.5 with two, 8.3 with four), fewer a longer table (262144 choices: 11.5 us with two, 10.9 with four; 65536: 8.4 with
-// one, 8.7 with two).
+// Choices that a lane places at a time: one up to the first number, two up to the second, four beyond.  More per lane are more steps in turn, fewer a
+// longer table.  256 experts, us with one, two and four: 65536 choices 8.3, 8.8, 10.1; 98304 10.0, 9.4, 11.0; 262144 12.0, 11.8, 11.7 (of 1024 experts 21.9,
+// 21.1, 17.3).
 constexpr uint32_t kOneItem = 65536, kTwoItems = 131072;
 
 struct SortPlan {
@@ -258,8 +260,9 @@ SortPlan planSort(uint32_t n, uint32_t align, uint32_t rows) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows to experts and back.  Sums of a few products per element of a row: all of it is bound by memory.  Every row is read once and written once (HBM
-// bytes by the counters equal to the algorithm's within 1 %), 16 bytes per lane at any alignment.  A workgroup takes a token and has a
+// Rows to experts and back.  Sums of a few products per element of a row: all of it is bound by memory.  Every row is read once and written once (by the
+// counters at most 2 % more HBM bytes than the algorithm's for rows on the 128-byte grid; 4 % more read off it, where two rows share a line), 16 bytes per
+// lane at any alignment.  A workgroup takes a token and has a
 // lane for every vector of its row, up to 1024: combine of 16 x 8 rows of 8192 bfloat16 5.7 us with 256 lanes, 4.7 with 512, 4.3 with 1024, of
 // 8192 x 8 rows 217, 212, 208; dispatch of 256 x 8 rows 11.1 us with 512, 8.6 with 1024.  The gradient of combine needs more registers and takes 512 at most (16 x
 // 8 rows 7.2 us, 7.6 with 1024), and so does dispatch past the caches (8192 x 8 rows 210 us, 215 with 1024).  Neighbouring tokens to the workgroups of one XCD: 208 -> 218 us for combine of 16384 x 8 rows, so the workgroups keep their order.
@@ -362,7 +365,7 @@ __global__ __launch_bounds__(kMaxRowThreads) void dispatchKernel(cuttHipExpertAr
 
 // A workgroup sums a token's rows, 16 bytes of each per lane, in 32 bits and in the order of the choices, with one rounding at the end.
 // The loads of all choices are in flight together.  16384 x 8 rows of 4096 bfloat16 (1209 MB): 208 us, 5.8 TB/s; the gradient of dispatch
-// of 8191 x 4 rows of 2050 floats (336 MB) 55 us.
+// of 8191 x 4 rows of 2050 floats (336 MB) 59 us.
 template <typename T, int N, int B, bool NT>
 __global__ __launch_bounds__(kMaxRowThreads) void combineKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, T* out, uint64_t outStride) {
   const uint32_t lane = threadIdx.x & 63;
@@ -417,7 +420,9 @@ __device__ __forceinline__ float sumOverWave(float (&v)[B]) {
 // A workgroup takes a token: its gradient row is multiplied into the rows it came from, and with them.  The last workgroups clear the empty rows.
 // The dot products are summed in 32 bits: a lane's columns, the lanes of a wavefront pairwise, the wavefronts in turn, always in the same order.
 // 8192 x 8 rows of 4096 bfloat16 (1142 MB): 219 us, 5.2 TB/s, as much read as written; a wavefront per token, without LDS: 241 us; four choices at a
-// time, for fewer registers and more wavefronts: 232.
+// time, for fewer registers and more wavefronts: 232.  With a tenth of the choices absent 219, the rows alone 141, the weights alone 99.  Few tokens are a chain of
+// latencies (choices, rows, the sums over a wavefront and over the wavefronts): one token with 6 rows of 5120 halves 4.8 us, the rows alone 3.0, the weights alone
+// 4.0; 256 such tokens 12.2, 7.2, 7.9.  Off the 128-byte grid 16384 x 8 rows of 2111 bfloat16 287 us, 4.1 TB/s.
 template <typename T, int N, int B, bool ROWS, bool WEIGHTS, bool NT>
 __global__ __launch_bounds__(kHalfRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
                                                                       T* dy, uint64_t dyStride, float* dweights, uint32_t tokenBlocks) {

@@ -32,7 +32,8 @@ struct Request {
 // Tokens and pages then find their request by a search in LDS.
 //
 // Bound by the launch and a chain of latencies (lengths, scan, search, table, store): 256 requests of one token 4.4 us, 96 requests with 98352 tokens (1.2
-// MB) 4.5, 2048 requests 6.8.  More requests than one scan takes (kScan, 25 KB of LDS): two launches, 11 us for 2049, 15 for 4096, 50 for 20000.
+// MB) 4.5, 2048 requests 6.8.  More requests than one scan takes (kScan, 25 KB of LDS): two launches, the first with one workgroup that scans part after part and writes all
+// tables: 11 us for 2049, 15 for 4096, 50 for 20000.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kPerThread = 8, kScan = kThreads * kPerThread;
 
@@ -180,7 +181,8 @@ __global__ __launch_bounds__(kThreads) void pageSlotsKernel(cuttHipTablesArgs a)
 
 // ---------------------------------------------------------------------------
 // Rows to their slots and back.  Bound by memory: every row is read once and written once.  131072 tokens, 8 heads of 128 bfloat16, keys and values
-// (1075 MB), out of pages [page, head, slot] to [head, token] 175 us (6.1 TB/s), into them from a projection's output 199 us; 256 tokens 2.6 us.
+// (1075 MB), out of pages [page, head, slot] to [head, token] 176 us (6.1 TB/s), into them from a projection's output 199 us, into pages
+// [page, slot, head] 214; 256 tokens 2.6 us.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMaxBlocks = 1u << 20;
 constexpr int kPerLane = 2;  // vectors a lane keeps in flight; that load: 180 us with one, 175 with two, 190 with four, 197 with eight

@@ -28,8 +28,8 @@ int launchRows(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t lds, void
 
 // Whether rows are more than the memory-side cache (256 MB) holds.  Then what is read cannot have been left there by whoever wrote it, nor what is
 // written be found there, and accesses past the caches are faster; below it they cost the next kernel more than they give.  MI355X, 8 choices, 4096
-// bfloat16: dispatch of 8192 tokens (537 MB of rows) 104 us past the caches, 115 through them, combine 96 and 109; dispatch and a combine that reads its
-// rows right after it, 134 MB: 60 us past, 52 through, 537 MB: 202 and 205.
+// bfloat16: dispatch of 8192 tokens (537 MB of rows) 105 us past the caches, 118 through them, combine 104 and 119; dispatch and a combine that reads its
+// rows right after it, 134 MB: 58 us past, 52 through, 537 MB: 211 and 253.
 inline bool pastCaches(uint64_t rows, uint64_t rowBytes) { return rows * rowBytes > ((uint64_t)256 << 20); }
 
 // n / d for a divisor made by cuttHipMakeDivisor(d), n below 2^31.

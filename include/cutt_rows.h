@@ -127,6 +127,9 @@ cuttResult cuttExpertCombineBackward(int tokens, int choices, int rows, int widt
  *                     absent (a table entry below 0, or beyond the table's width) and for starts[requests] <= i < tokens
  *   positions[i]      its position in its request, -1 for i >= starts[requests].  NULL: not wanted
  *
+ * The list itself stays: the caller takes used[0] entries off its front before the next call.  A captured call reads the same
+ * buffers at every replay; its caller moves the list up between replays (entries below 0 are no pages and may fill its end).
+ *
  *   requests, freeCount, tokens >= 0, pageSize >= 1, tableWidth >= 1
  *   cached, added     [requests]; values below 0 count as 0; sums and positions are 2^31 - 1 at most
  *   tables            [requests, tableWidth], read and written
@@ -148,6 +151,7 @@ cuttResult cuttPageTables(int requests, int pageSize, int tableWidth, int freeCo
  *                     ([pages, pageSize, heads, width], [pages, heads, pageSize, width], ...)
  *                     What is written must not lie on top of itself: each stride of its axes of more than one entry leads past all that the
  *                     smaller ones reach, and the two written tensors share no element (they may interleave)
+ *                     k and v share width and strides, and so do their caches; where they do not, each moves in a call of its own
  *   v, vCache         NULL both: only k moves (a buffer of no tokens or of no pages may be NULL by itself)
  * The strides are host arrays, read during the call.
  */
