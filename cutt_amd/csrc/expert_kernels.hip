@@ -422,7 +422,7 @@ __device__ __forceinline__ float sumOverWave(float (&v)[B]) {
 // 8192 x 8 rows of 4096 bfloat16 (1142 MB): 219 us, 5.2 TB/s, as much read as written; a wavefront per token, without LDS: 241 us; four choices at a
 // time, for fewer registers and more wavefronts: 232.  With a tenth of the choices absent 219, the rows alone 141, the weights alone 99.  Few tokens are a chain of
 // latencies (choices, rows, the sums over a wavefront and over the wavefronts): one token with 6 rows of 5120 halves 4.8 us, the rows alone 3.0, the weights alone
-// 4.0; 256 such tokens 12.2, 7.2, 7.9.  Off the 128-byte grid 16384 x 8 rows of 2111 bfloat16 287 us, 4.1 TB/s.
+// 4.0; 256 such tokens 12.2, 7.2, 7.9.  Off the 128-byte grid 16384 x 8 rows of 2111 bfloat16 290 us, 4.1 TB/s.
 template <typename T, int N, int B, bool ROWS, bool WEIGHTS, bool NT>
 __global__ __launch_bounds__(kHalfRowThreads) void combineBackwardKernel(cuttHipExpertArgs a, const T* y, uint64_t yStride, const T* dout, uint64_t doutStride,
                                                                       T* dy, uint64_t dyStride, float* dweights, uint32_t tokenBlocks) {
@@ -532,6 +532,9 @@ uint32_t rowThreads(uint32_t width, uint32_t n, uint32_t most) {
 }
 
 // Rows on the 128-byte grid.  Off it, lines that two rows share have to meet in a cache: 65536 rows of 4100 bytes 69 us through the caches, 73 past them.
+// So for dispatch, which only stores them; the gradient of combine, which reads as many, stores past the caches on the grid and off it: 65536 rows of 4100 bytes
+// 133 us so, 144 with stores through the caches, 138 with all of it through them; 131072 of 4222 bytes 290, 298, 299.  Combine's reads of the same rows: 57 us
+// past and 60 through, 129 and 123.
 bool onLines(const void* p, uint64_t strideBytes) { return ((uintptr_t)p | strideBytes) % 128 == 0; }
 
 }  // namespace
