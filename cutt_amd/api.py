@@ -1,6 +1,6 @@
 """ctypes binding of libcutt.so: the four plan functions of include/cutt.h, the row
-operators of include/cutt_rows.h and the hooks of include/cutt_ext.h, with the same names
-and argument order.
+operators of include/cutt_rows.h, the products of include/cutt_products.h and the hooks of
+include/cutt_ext.h, with the same names and argument order.
 
 Device buffers are passed as integer addresses (e.g. ``tensor.data_ptr()``),
 streams as integer ``hipStream_t`` values (e.g.
@@ -29,6 +29,7 @@ METHOD_NAMES = {0: "Unknown", 1: "Trivial", 2: "Packed", 3: "PackedSplit", 4: "T
 # element types of rows that are summed (cuttRowType)
 CUTT_F32, CUTT_F16, CUTT_BF16 = 0, 1, 2
 CUTT_MAX_EXPERTS = 1024
+CUTT_MAX_HEAD_WIDTH = 256
 
 
 class CuttError(RuntimeError):
@@ -177,7 +178,11 @@ def lib():
             ("cuttExpertCombineBackward", [i] * 5 + [vp] * 4 + [vp, ll] * 3 + [vp], i),
             ("cuttPageTables", [i] * 5 + [vp] * 9, i),
             ("cuttPageStore", [i] * 3 + [z, i, i] + [vp] * 8, i),
-            ("cuttPageLoad", [i] * 3 + [z, i, i] + [vp] * 8, i)):
+            ("cuttPageLoad", [i] * 3 + [z, i, i] + [vp] * 8, i),
+            ("cuttGroupedProduct", [i] * 6 + [vp, vp, vp, ll, vp, vp, vp, ll], i),
+            ("cuttGroupedProductWeights", [i] * 5 + [vp, vp, vp, ll, vp, ll, vp, vp], i),
+            ("cuttAttendPagesWorkspace", [i] * 7, z),
+            ("cuttAttendPages", [i] * 10 + [ctypes.c_float] + [vp] * 13 + [z], i)):
         f = getattr(l, name)
         f.argtypes, f.restype = args, result
     _lib = l
@@ -311,6 +316,37 @@ def cuttPageLoad(tokens, heads, width, sizeofType, pages, pageSize, stream, slot
         return CUTT_INVALID_PARAMETER
     return (_lib or lib()).cuttPageLoad(tokens, heads, width, sizeofType, pages, pageSize, stream, slots, k, v, _strides(rowStrides, 2), kCache,
                                         vCache, _strides(cacheStrides, 3))
+
+
+# The products (include/cutt_products.h), in the same manner.
+def cuttGroupedProduct(rows, groups, inner, outer, type, transposed, stream, offsets, x, xStride, w, wStrides, y, yStride):
+    if (rows | groups | inner | outer | type) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttGroupedProduct(rows, groups, inner, outer, type, bool(transposed), stream, offsets, x, xStride, w, _strides(wStrides, 2),
+                                              y, yStride)
+
+
+def cuttGroupedProductWeights(rows, groups, inner, outer, type, stream, offsets, x, xStride, dy, dyStride, dw, dwStrides):
+    if (rows | groups | inner | outer | type) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttGroupedProductWeights(rows, groups, inner, outer, type, stream, offsets, x, xStride, dy, dyStride, dw,
+                                                     _strides(dwStrides, 2))
+
+
+def cuttAttendPagesWorkspace(queries, heads, keyHeads, width, pageSize, tableWidth, window):
+    """Bytes of workspace that cuttAttendPages needs."""
+    if (queries | heads | keyHeads | width | pageSize | tableWidth | window) >> 31:
+        return 0
+    return (_lib or lib()).cuttAttendPagesWorkspace(queries, heads, keyHeads, width, pageSize, tableWidth, window)
+
+
+def cuttAttendPages(queries, requests, heads, keyHeads, width, type, pages, pageSize, tableWidth, window, scale, stream, tables, owners, positions, q,
+                    qStrides, kCache, vCache, cacheStrides, out, outStrides, logSums=0, workspace=0, workspaceBytes=0):
+    if (queries | requests | heads | keyHeads | width | type | pages | pageSize | tableWidth | window) >> 31:
+        return CUTT_INVALID_PARAMETER
+    return (_lib or lib()).cuttAttendPages(queries, requests, heads, keyHeads, width, type, pages, pageSize, tableWidth, window, scale, stream, tables,
+                                           owners, positions, q, _strides(qStrides, 2), kCache, vCache, _strides(cacheStrides, 3), out,
+                                           _strides(outStrides, 2), logSums, workspace, workspaceBytes)
 
 
 def get_plan_info(handle):
