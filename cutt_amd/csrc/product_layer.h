@@ -6,6 +6,7 @@
 #ifndef CUTT_PRODUCT_LAYER_H
 #define CUTT_PRODUCT_LAYER_H
 
+#include "../../include/cutt_products.h"
 #include "row_layer.h"
 
 #ifdef __cplusplus
