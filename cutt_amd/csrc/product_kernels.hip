@@ -10,9 +10,10 @@ using namespace cutt;
 
 namespace {
 
-// A group's rows, and the first of the tile that a workgroup has to do.
+// A group, the end of its rows, and the first row of one of its tiles.
 struct Segment {
   uint32_t group, first, end;
+  uint32_t before, tiles;  // tiles of the groups before it, and of its own
 };
 
 __device__ __forceinline__ uint32_t boundOf(const cuttHipProductArgs& a, uint32_t e) { return min((uint32_t)max(a.offsets[e], 0), a.rows); }
@@ -35,10 +36,12 @@ __device__ __forceinline__ bool findTile(const cuttHipProductArgs& a, uint32_t t
     const uint64_t found = __ballot(tile < upTo);
     if (found) {
       const uint32_t at = __builtin_ctzll(found);
-      s.group = base + at;
+      s.group = __builtin_amdgcn_readfirstlane(base + at);
       s.end = __builtin_amdgcn_readlane(hi, at);
       const uint64_t first = (uint64_t)__builtin_amdgcn_readlane(lo, at) + (uint64_t)(tile - __builtin_amdgcn_readlane(upTo - n, at)) * BM;
-      s.first = (uint32_t)first;
+      s.first = __builtin_amdgcn_readfirstlane((uint32_t)first);
+      s.before = __builtin_amdgcn_readlane(upTo - n, at);
+      s.tiles = __builtin_amdgcn_readlane(n, at);
       return first < s.end;
     }
     before = __builtin_amdgcn_readlane(upTo, 63);
@@ -57,9 +60,8 @@ struct Tile {
   static constexpr int PER = ACROSS ? B / E : 8;  // pieces per row of the tile
   static constexpr int PIECES = 8 * B;
   static __device__ __forceinline__ uint32_t skew(uint32_t row) {
-    if (!ACROSS) return row & 7;
-    if (sizeof(T) == 4) return 0;
-    return (((row & 3) | (row >> 3 & 1) << 2) * 2) & (PER - 1);
+    if (!ACROSS) return (row ^ row >> 3) & 7;
+    return 0;
   }
   static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) { return row * PER + (piece ^ skew(row)); }
 };
@@ -89,69 +91,99 @@ struct Loader {
   }
 };
 
-// Fragments of F times 16 rows (from row `first` on) for step s of the tile's two.  at(t, j): the j-th instruction's operand for rows t.
-// Which row of the tile a lane's row l of fragment t is: rowOf(t, l).
+// Fragments of F times 16 rows (from row `first` on) for step s of the tile's two.  at(t): the instruction's operand for rows t.
+// Which row of the tile a lane's row l of fragment t is: rowOf(t, l).  Across k a lane loads neighbouring rows' elements together, k by k, and turns them in its registers:
+// two k's to a word, with one instruction for each.  (LDS can turn them while it reads; but the compiler, which does not know what those reads touch, then waits for all that
+// is on its way to LDS.)
 template <typename T, bool ACROSS, int B, int F>
 struct Fragments {
   using L = Tile<T, ACROSS, B>;
-  Chunk<T> v[F];
-  __device__ __forceinline__ void load(const Chunk<T>* lds, uint32_t first, int s) {
+  static constexpr int E = kPer16<T>, C = ACROSS ? (F < E ? F : E) : 1;  // rows that a lane has side by side
+  AlignedVec<T, ACROSS ? C : E> v[ACROSS ? F / C * E : F];
+  static constexpr int LOADS = ACROSS ? F / C * E : F;
+  __device__ __forceinline__ void loadOne(const Chunk<T>* lds, uint32_t first, int s, int i) {
     const uint32_t l = threadIdx.x & 15, quarter = (threadIdx.x & 63) >> 4;
     if constexpr (!ACROSS) {
-#pragma unroll
-      for (int t = 0; t < F; t++) v[t] = lds[L::place(first + t * 16 + l, s * 4 + quarter)];
-    } else if constexpr (sizeof(T) == 2) {
-      // Sixteen lanes load 4 k's of 16 columns, 8 bytes each, and get 4 k's of one column each.
-      typedef short Four __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) Four* Lds;
-#pragma unroll
-      for (int t = 0; t < F; t++) {
-        union {
-          Four four[2];
-          Chunk<T> whole;
-        } u;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t k = s * 32 + quarter * 8 + h * 4 + (l >> 2), col = first + t * 16 + (l & 3) * 4;
-          const char* const at = reinterpret_cast<const char*>(lds + L::place(k, col / 8)) + (col & 7) * 2;
-          u.four[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at);
-        }
-        v[t] = u.whole;
-      }
+      v[i] = lds[L::place(first + i * 16 + l, s * 4 + quarter)];
     } else {
-      static_assert(F % 4 == 0, "a lane takes four neighbouring columns");
-#pragma unroll
-      for (int t = 0; t < F; t += 4)
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[t + j] = lds[L::place(s * 16 + quarter * 4 + j, (first + t * 16) / 4 + l)];
+      const T* const line = reinterpret_cast<const T*>(lds + L::place((s * 4 + quarter) * E + i % E, 0));
+      v[i] = *reinterpret_cast<const AlignedVec<T, C>*>(line + first + i / E * 16 * C + l * C);
     }
+  }
+  // Part i of n of the loads.
+  __device__ __forceinline__ void load(const Chunk<T>* lds, uint32_t first, int s, int i = 0, int n = 1) {
+#pragma unroll
+    for (int j = 0; j < LOADS; j++)
+      if (j * n / LOADS == i) loadOne(lds, first, s, j);
   }
   __device__ __forceinline__ Chunk<T> at(int t) const {
-    if constexpr (ACROSS && sizeof(T) == 4) {
+    if constexpr (!ACROSS) {
+      return v[t];
+    } else if constexpr (sizeof(T) == 4) {
       Chunk<T> c;
 #pragma unroll
-      for (int j = 0; j < 4; j++) c[j] = v[t / 4 * 4 + j][t % 4];
+      for (int j = 0; j < E; j++) c[j] = v[t / C * E + j][t % C];
       return c;
+    } else {
+      static_assert(C >= 2, "whole words");
+      typedef uint32_t Words __attribute__((ext_vector_type(4)));
+      typedef uint32_t Piece __attribute__((ext_vector_type(C / 2)));
+      Words c;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t even = __builtin_bit_cast(Piece, v[t / C * E + 2 * i])[t % C / 2], odd = __builtin_bit_cast(Piece, v[t / C * E + 2 * i + 1])[t % C / 2];
+        c[i] = __builtin_amdgcn_perm(odd, even, t % 2 ? 0x07060302 : 0x05040100);
+      }
+      return __builtin_bit_cast(Chunk<T>, c);
     }
-    return v[t];
   }
-  static __device__ __forceinline__ uint32_t rowOf(int t, uint32_t l) {
-    return ACROSS && sizeof(T) == 4 ? t / 4 * 64 + l * 4 + t % 4 : t * 16 + l;
-  }
+  static __device__ __forceinline__ uint32_t rowOf(int t, uint32_t l) { return ACROSS ? t / C * 16 * C + l * C + t % C : t * 16 + l; }
 };
 
-// n results of a row, side by side.
-template <typename T>
-__device__ __forceinline__ void storeFour(T* p, Acc v, uint32_t n) {
-  Pack<T, 4> o;
+// The first n of N results of a row, side by side.
+template <typename T, int N>
+__device__ __forceinline__ void storeSome(T* p, const float (&v)[N], uint32_t n) {
+  Pack<T, N> o;
 #pragma unroll
-  for (int i = 0; i < 4; i++) o.set(i, (T)v[i]);
-  if (n >= 4) {
+  for (int i = 0; i < N; i++) o.set(i, (T)v[i]);
+  if (n >= N) {
     o.store(p);
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++)
+    for (uint32_t i = 0; i < N; i++)
       if (i < n) p[i] = o.get(i);
+  }
+}
+
+// A wavefront's results, rows m0 and columns n0 on of m and n, to `to`.
+template <typename T, bool MACROSS, bool NACROSS, int BM, int BN, int FM, int FN>
+__device__ __forceinline__ void storeResults(const Acc (&acc)[FM][FN], T* to, uint64_t stride, uint32_t m0, uint32_t m, uint32_t n0, uint32_t n) {
+  using N = Fragments<T, NACROSS, BN, FN>;
+  const uint32_t l = threadIdx.x & 15, quarter = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int i = 0; i < FM; i++) {
+    const uint32_t row = m0 + Fragments<T, MACROSS, BM, FM>::rowOf(i, l);
+    if (row >= m) continue;
+    T* const line = to + row * stride;
+    if constexpr (NACROSS) {
+#pragma unroll
+      for (int j = 0; j < FN; j += N::C)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const uint32_t col = n0 + N::rowOf(j, quarter * 4 + r);
+          float v[N::C];
+#pragma unroll
+          for (int x = 0; x < N::C; x++) v[x] = acc[i][j + x][r];
+          if (col < n) storeSome(line + col, v, n - col);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < FN; j++) {
+        const uint32_t col = n0 + j * 16 + quarter * 4;
+        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (col < n) storeSome(line + col, v, n - col);
+      }
+    }
   }
 }
 
@@ -160,7 +192,7 @@ template <typename T, bool MACROSS, bool NACROSS, int BM, int BN, int WM, int WN
 __device__ __forceinline__ void productTile(const T* from, uint64_t mStride, uint32_t m, const T* with, uint64_t nStride, uint32_t n, uint32_t along, T* to,
                                             uint64_t toStride, Chunk<T>* lds) {
   constexpr int THREADS = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16;
-  const uint32_t wave = threadIdx.x >> 6, l = threadIdx.x & 15, quarter = (threadIdx.x & 63) >> 4;
+  const uint32_t wave = threadIdx.x >> 6;
   const uint32_t m0 = wave / WN * (BM / WM), n0 = wave % WN * (BN / WN);
   Chunk<T>* const ldsN = lds + 8 * BM;
   Loader<T, MACROSS, BM, THREADS> loadM;
@@ -192,29 +224,176 @@ __device__ __forceinline__ void productTile(const T* from, uint64_t mStride, uin
         for (int j = 0; j < FN; j++) acc[i][j] = multiply(fn.at(j), fm.at(i), acc[i][j]);
     }
   }
+  storeResults<T, MACROSS, NACROSS, BM, BN>(acc, to, toStride, m0, m, n0, n);
+}
+
+// ---------------------------------------------------------------------------
+// Rings of tiles.  As above, but the operands go from memory straight to LDS, to one of R places in turn, and the fragments of a half tile are read while the other half's are
+// multiplied.  For operands on the 16-byte grid.  What is outside (rows behind a group's end, k's behind the last) is beyond the end that the loads' descriptor
+// states, and comes as zeros without being read.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kOutside = 0x80000000u;  // an offset beyond every descriptor's end
+
+template <int N>
+__device__ __forceinline__ void waitForLoads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);  // vmcnt alone
+  asm volatile("" ::: "memory");
+}
+// What this wavefront reads from LDS has arrived.
+__device__ __forceinline__ void waitForLds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt alone
+  asm volatile("" ::: "memory");
+}
+// It has, and all wavefronts are here.
+__device__ __forceinline__ void meet() {
+  waitForLds();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// All wavefronts of the workgroup.  The operands' parts are below 2^30 bytes each, from the first to the last element.
+template <typename T, bool MACROSS, bool NACROSS, int BM, int BN, int WM, int WN, int R>
+__device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uint32_t m, const T* with, uint32_t nStride, uint32_t n, uint32_t along, T* to,
+                                            uint64_t toStride, Chunk<T>* lds) {
+  using LM = Tile<T, MACROSS, BM>;
+  using LN = Tile<T, NACROSS, BN>;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  constexpr uint32_t WAVES = WM * WN, K = LM::K, PIECES = 8 * (BM + BN);
+  constexpr uint32_t ALLM = BM / 8, ALL = (BM + BN) / 8, LOADS = (ALL + WAVES - 1) / WAVES;  // a wavefront's load: 64 pieces
+  constexpr bool EVEN = ALLM % WAVES == 0 && ALL % WAVES == 0;  // (then it is known which load is of which operand)
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t m0 = wave / WN * (BM / WM), n0 = wave % WN * (BN / WN);
+
+  // This wavefront's loads of a tile.
+  __amdgpu_buffer_rsrc_t source[LOADS];
+  uint32_t offset[LOADS], kOf[LOADS], step[LOADS], place[LOADS];
 #pragma unroll
-  for (int i = 0; i < FM; i++) {
-    const uint32_t row = m0 + Fragments<T, MACROSS, BM, FM>::rowOf(i, l);
-    if (row >= m) continue;
-    T* const line = to + row * toStride;
-    if constexpr (NACROSS && sizeof(T) == 4) {
+  for (uint32_t u = 0; u < LOADS; u++) {
+    const uint32_t q = EVEN ? wave + u * WAVES : min(wave + u * WAVES, ALL - 1);  // (the last one several times if they do not come out even)
+    const bool isM = EVEN ? u < ALLM / WAVES : q < ALLM;
+    const uint32_t at = (isM ? q : q - ALLM) * 64 + lane, stride = isM ? mStride : nStride;
+    const uint32_t rowM = at / LM::PER, rowN = at / LN::PER, row = isM ? rowM : rowN;
+    const uint32_t piece = isM ? at % LM::PER ^ LM::skew(rowM) : at % LN::PER ^ LN::skew(rowN);
+    const bool across = isM ? MACROSS : NACROSS;
+    const uint32_t lines = across ? along : isM ? m : n, width = across ? (isM ? m : n) : along;
+    source[u] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(isM ? from : with), 0, lines ? ((lines - 1) * stride + width) * (uint32_t)sizeof(T) : 0, 0x00020000);
+    offset[u] = (row * stride + piece * LM::E) * (uint32_t)sizeof(T);
+    kOf[u] = across ? row : piece * LM::E;
+    step[u] = across ? K * stride * (uint32_t)sizeof(T) : 128;
+    place[u] = q * 64;
+  }
+  uint32_t asked = 0, slot = 0;  // tiles that have been asked for, and where the next one goes
+  // Part i of n of the next tile's loads.
+  const auto ask = [&](int i, int n) __attribute__((always_inline)) {
+    Chunk<T>* const ring = lds + slot * PIECES;
 #pragma unroll
-      for (int j = 0; j < FN; j += 4)
+    for (int u = 0; u < (int)LOADS; u++) {
+      if (u * n / (int)LOADS != i) continue;
+      const uint32_t o = kOf[u] + asked * K < along ? offset[u] : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(source[u], (__attribute__((address_space(3))) void*)(ring + place[u]), 16, o, 0, 0, 0);
+      offset[u] += step[u];
+    }
+    if (i == n - 1) {
+      asked++;
+      slot = slot + 1 == R ? 0 : slot + 1;
+    }
+  };
+
+  Acc acc[FM][FN] = {};
+  const uint32_t tiles = (along + K - 1) / K;
+  Fragments<T, MACROSS, BM, FM> fm[2];
+  Fragments<T, NACROSS, BN, FN> fn[2];
+  const auto read = [&](uint32_t at, int s, int i, int n) __attribute__((always_inline)) {
+    fm[s].load(lds + at * PIECES, m0, s, i, n);
+    fn[s].load(lds + at * PIECES + 8 * BM, n0, s, i, n);
+  };
+  // A half tile's products; between them, part by part, what `other` does: there is one wavefront for a SIMD, and what it does not issue while the matrix unit works
+  // is time lost.
+  const auto add = [&](int s, auto other) __attribute__((always_inline)) {
+    Chunk<T> a[FN];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const uint32_t col = n0 + j * 16 + (quarter * 4 + r) * 4;
-          Acc v;
-#pragma unroll
-          for (int x = 0; x < 4; x++) v[x] = acc[i][j + x][r];
-          if (col < n) storeFour(line + col, v, n - col);
-        }
-    } else {
+    for (int i = 0; i < FM; i++) {
+      other(i, FM);
+      const Chunk<T> b = fm[s].at(i);
 #pragma unroll
       for (int j = 0; j < FN; j++) {
-        const uint32_t col = n0 + j * 16 + quarter * 4;
-        if (col < n) storeFour(line + col, acc[i][j], n - col);
+        if (i == 0) a[j] = fn[s].at(j);
+        acc[i][j] = multiply(a[j], b, acc[i][j]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+#pragma unroll
+  for (int r = 0; r < R; r++) ask(0, 1);
+  waitForLoads<(R - 1) * LOADS>();
+  meet();
+  read(0, 0, 0, 1);
+  uint32_t now = 0;
+  for (uint32_t tile = 0; tile < tiles; tile++) {
+    const uint32_t next = now + 1 == R ? 0 : now + 1;
+    waitForLds();  // (before more are under way than the counter counts)
+    add(0, [&](int i, int n) __attribute__((always_inline)) { read(now, 1, i, n); });
+    waitForLoads<(R - 2) * LOADS>();
+    meet();
+    add(1, [&](int i, int n) __attribute__((always_inline)) {
+      read(next, 0, i, n);
+      ask(i, n);  // to where this tile was
+    });
+    now = next;
+  }
+  waitForLoads<0>();
+  meet();
+  storeResults<T, MACROSS, NACROSS, BM, BN>(acc, to, toStride, m0, m, n0, n);
+}
+
+// Items for the workgroups in groups of kNear to an XCD, whose L2 they share.
+constexpr uint32_t kNear = 32;
+__device__ __forceinline__ uint64_t itemOf(uint64_t block) { return block / (8 * kNear) * (8 * kNear) + block % 8 * kNear + block / 8 % kNear; }
+// Which of a group's tiles x strips number `item` is: blocks of kWide strips one after the other, in a block tile by tile, so that items that follow each other share
+// both operands.
+constexpr uint32_t kWide = 8;
+__device__ __forceinline__ void placeOf(uint32_t item, uint32_t tiles, uint32_t strips, uint32_t& tile, uint32_t& strip) {
+  const uint32_t block = item / (tiles * kWide), in = item - block * tiles * kWide, wide = min(strips - block * kWide, kWide);
+  tile = in / wide;
+  strip = block * kWide + in - tile * wide;
+}
+
+template <typename T, bool TRANSPOSED, int BM, int BN, int WM, int WN, int R>
+__global__ __launch_bounds__(WM* WN * 64) void productRingKernel(cuttHipProductArgs a, uint64_t items) {
+  extern __shared__ __attribute__((aligned(16))) char ringLds[];
+  const uint32_t strips = (a.outer + BN - 1) / BN;
+  for (uint64_t block = blockIdx.x; block < items; block += gridDim.x) {
+    const uint64_t item = itemOf(block);
+    Segment s;
+    if (!findTile<BM>(a, (uint32_t)(item / strips), s)) continue;
+    uint32_t tile, strip;
+    placeOf((uint32_t)(item - (uint64_t)s.before * strips), s.tiles, strips, tile, strip);
+    s.first = s.first - ((uint32_t)(item / strips) - s.before) * BM + tile * BM;
+    const uint32_t col = strip * BN;
+    const T* const w = static_cast<const T*>(a.w) + s.group * a.wGroup;
+    productRing<T, false, !TRANSPOSED, BM, BN, WM, WN, R>(static_cast<const T*>(a.x) + s.first * a.xStride, (uint32_t)a.xStride, min(s.end - s.first, (uint32_t)BM),
+                                                       TRANSPOSED ? w + col * a.wRow : w + col, (uint32_t)a.wRow, min(a.outer - col, (uint32_t)BN), a.inner,
+                                                       static_cast<T*>(a.y) + (s.first * a.yStride + col), a.yStride, reinterpret_cast<Chunk<T>*>(ringLds));
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int R>
+__global__ __launch_bounds__(WM* WN * 64) void weightsRingKernel(cuttHipProductArgs a, uint64_t items) {
+  extern __shared__ __attribute__((aligned(16))) char ringLds[];
+  const uint32_t strips = (a.outer + BN - 1) / BN, tiles = (a.inner + BM - 1) / BM;
+  for (uint64_t block = blockIdx.x; block < items; block += gridDim.x) {
+    const uint64_t item = itemOf(block);
+    const uint32_t group = (uint32_t)(item / ((uint64_t)tiles * strips));
+    if (group >= a.groups) continue;
+    uint32_t tile, strip;
+    placeOf((uint32_t)(item - (uint64_t)group * tiles * strips), tiles, strips, tile, strip);
+    const uint32_t row = tile * BM, col = strip * BN;
+    const uint32_t first = boundOf(a, group), end = max(first, boundOf(a, group + 1));
+    productRing<T, true, true, BM, BN, WM, WN, R>(static_cast<const T*>(a.x) + (first * a.xStride + row), (uint32_t)a.xStride, min(a.inner - row, (uint32_t)BM),
+                                               static_cast<const T*>(a.w) + (first * a.wRow + col), (uint32_t)a.wRow, min(a.outer - col, (uint32_t)BN), end - first,
+                                               static_cast<T*>(a.y) + (group * a.wGroup + row * a.yStride + col), a.yStride, reinterpret_cast<Chunk<T>*>(ringLds));
   }
 }
 
@@ -252,20 +431,42 @@ __global__ __launch_bounds__(WM* WN * 64) void weightsKernel(cuttHipProductArgs 
 uint32_t blocksFor(uint64_t items) { return (uint32_t)std::min<uint64_t>(items, kMaxBlocks); }
 uint64_t parts(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
+// Whether `lines` rows of `width` elements every `stride` are on the 16-byte grid, and near enough for 32-bit offsets.
+template <typename T>
+bool inReach(const void* p, uint64_t group, uint64_t stride, uint64_t lines, uint64_t width) {
+  return ((uintptr_t)p | group * sizeof(T) | stride * sizeof(T) | width * sizeof(T)) % 16 == 0 && stride < (1u << 30) &&
+         (lines * stride + width) * sizeof(T) < (1u << 30);
+}
+// (workgroups whose items are handed out kNear to an XCD at a time: whole rounds)
+uint32_t ringBlocks(uint64_t items) { return (uint32_t)std::min<uint64_t>((items + 8 * kNear - 1) / (8 * kNear) * (8 * kNear), kMaxBlocks); }
+
 template <typename T>
 int product(const cuttHipProductArgs& a, bool transposed, void* stream) {
-  constexpr int BM = 128, BN = 128;
   // Tiles that suffice whatever the groups are: whole ones of all rows, and one more for every group that has a row.
-  const uint64_t items = (a.rows / BM + std::min(a.rows, a.groups)) * parts(a.outer, BN);
+  const auto items = [&](uint32_t bm, uint32_t bn) { return (a.rows / bm + std::min(a.rows, a.groups)) * parts(a.outer, bn); };
+  const bool ring = inReach<T>(a.x, 0, a.xStride, 256, a.inner) && (transposed ? inReach<T>(a.w, a.wGroup, a.wRow, 256, a.inner) : inReach<T>(a.w, a.wGroup, a.wRow, a.inner, a.outer));
+  if (ring && sizeof(T) == 2) {
+    constexpr int BM = 256, BN = 256;
+    const uint64_t n = ringBlocks(items(BM, BN));
+    auto kernel = transposed ? productRingKernel<T, true, BM, BN, 2, 2, 2> : productRingKernel<T, false, BM, BN, 2, 2, 2>;
+    return launchRows(kernel, (uint32_t)n, 256, 2 * (BM + BN) * 128, stream, a, n);
+  }
+  constexpr int BM = 128, BN = 128;
   auto kernel = transposed ? productKernel<T, true, BM, BN, 2, 2> : productKernel<T, false, BM, BN, 2, 2>;
-  return launchRows(kernel, blocksFor(items), 256, 0, stream, a, items);
+  return launchRows(kernel, blocksFor(items(BM, BN)), 256, 0, stream, a, items(BM, BN));
 }
 
 template <typename T>
 int weights(const cuttHipProductArgs& a, void* stream) {
+  const auto items = [&](uint32_t bm, uint32_t bn) { return parts(a.inner, bm) * parts(a.outer, bn) * a.groups; };
+  const bool ring = inReach<T>(a.x, 0, a.xStride, a.rows, a.inner) && inReach<T>(a.w, 0, a.wRow, a.rows, a.outer);
+  if (ring && sizeof(T) == 2) {
+    constexpr int BM = 256, BN = 256;
+    const uint64_t n = ringBlocks(items(BM, BN));
+    return launchRows(weightsRingKernel<T, BM, BN, 2, 2, 2>, (uint32_t)n, 256, 2 * (BM + BN) * 128, stream, a, n);
+  }
   constexpr int BM = 128, BN = 128;
-  const uint64_t items = parts(a.inner, BM) * parts(a.outer, BN) * a.groups;
-  return launchRows(weightsKernel<T, BM, BN, 2, 2>, blocksFor(items), 256, 0, stream, a, items);
+  return launchRows(weightsKernel<T, BM, BN, 2, 2>, blocksFor(items(BM, BN)), 256, 0, stream, a, items(BM, BN));
 }
 
 }  // namespace
