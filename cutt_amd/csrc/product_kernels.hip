@@ -66,27 +66,46 @@ struct Tile {
   static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) { return row * PER + (piece ^ skew(row)); }
 };
 
-// An operand's part that a tile is taken from: `along` elements along k and `across` the other way.
+// An operand's part that a tile is taken from: `along` elements along k and `across` the other way.  A lane's 16 bytes that would reach beyond a row's end are loaded from
+// so much further up that they end with it, and moved when they go to LDS.
 template <typename T, bool ACROSS, int B, int THREADS>
 struct Loader {
   using L = Tile<T, ACROSS, B>;
-  static constexpr int N = L::PIECES / THREADS;
-  static_assert(N * THREADS == L::PIECES, "whole rounds");
+  static constexpr int N = (L::PIECES + THREADS - 1) / THREADS;
   Chunk<T> held[N];
+  struct Place {
+    uint32_t row, col;
+    int valid;  // elements of the 16 bytes, 0 to E
+    __device__ __forceinline__ Place(int i, uint32_t along, uint32_t across, uint32_t k) {
+      const uint32_t p = threadIdx.x + i * THREADS, r = p / L::PER, c = p % L::PER * L::E;
+      row = ACROSS ? k + r : r;
+      col = ACROSS ? c : k + c;
+      const uint32_t rows = ACROSS ? along : across, cols = ACROSS ? across : along;
+      valid = p < L::PIECES && row < rows && col < cols ? (int)min(cols - col, (uint32_t)L::E) : 0;
+    }
+  };
   __device__ __forceinline__ void load(const T* from, uint64_t stride, uint32_t along, uint32_t across, uint32_t k) {
+    const bool narrow = (ACROSS ? across : along) < (uint32_t)L::E;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const uint32_t p = threadIdx.x + i * THREADS, row = p / L::PER, col = p % L::PER * L::E;
-      const uint32_t r = ACROSS ? k + row : row, c = ACROSS ? col : k + col;
-      const uint32_t rows = ACROSS ? along : across, cols = ACROSS ? across : along;
-      held[i] = loadChunk(from + (r * stride + c), r < rows && c < cols ? (int)min(cols - c, (uint32_t)L::E) : 0);
+      const Place at(i, along, across, k);
+      const T* const p = from + (at.row * stride + at.col);
+      held[i] = {};
+      if (narrow) held[i] = loadChunk(p, at.valid);
+      else if (at.valid) held[i] = __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Vec<T, L::E>*>(p - (L::E - at.valid)));
     }
   }
-  __device__ __forceinline__ void store(Chunk<T>* lds) const {
+  // With the same arguments as the load.
+  __device__ __forceinline__ void store(Chunk<T>* lds, uint32_t along, uint32_t across, uint32_t k) const {
+    const bool narrow = (ACROSS ? across : along) < (uint32_t)L::E;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const uint32_t p = threadIdx.x + i * THREADS;
-      lds[L::place(p / L::PER, p % L::PER)] = held[i];
+      const Place at(i, along, across, k);
+      Chunk<T> v = held[i];
+      if (!narrow && at.valid && at.valid < L::E)
+        v = __builtin_bit_cast(Chunk<T>, __builtin_bit_cast(unsigned __int128, v) >> (uint32_t)((L::E - at.valid) * 8 * sizeof(T)));
+      if (p < L::PIECES) lds[L::place(p / L::PER, p % L::PER)] = v;
     }
   }
 };
@@ -205,8 +224,8 @@ __device__ __forceinline__ void productTile(const T* from, uint64_t mStride, uin
   constexpr uint32_t K = 128 / sizeof(T);
   for (uint64_t k = 0; k < along; k += K) {
     __syncthreads();
-    loadM.store(lds);
-    loadN.store(ldsN);
+    loadM.store(lds, along, m, (uint32_t)k);
+    loadN.store(ldsN, along, n, (uint32_t)k);
     __syncthreads();
     if (k + K < along) {
       loadM.load(from, mStride, along, m, (uint32_t)k + K);
@@ -440,33 +459,57 @@ bool inReach(const void* p, uint64_t group, uint64_t stride, uint64_t lines, uin
 // (workgroups whose items are handed out kNear to an XCD at a time: whole rounds)
 uint32_t ringBlocks(uint64_t items) { return (uint32_t)std::min<uint64_t>((items + 8 * kNear - 1) / (8 * kNear) * (8 * kNear), kMaxBlocks); }
 
+constexpr uint32_t kRows32 = 4, kRows64 = 48, kRows128 = 320, kRowsWeights = 512;
+
+template <int M, int N, int WAVES_M, int WAVES_N, int PLACES>
+struct Shape {
+  static constexpr int BM = M, BN = N, WM = WAVES_M, WN = WAVES_N, R = PLACES, THREADS = WM * WN * 64;
+};
+
+template <typename T, typename S>
+int productAs(const cuttHipProductArgs& a, bool transposed, bool ring, void* stream) {
+  // Tiles that suffice whatever the groups are: whole ones of all rows, and one more for every group that has a row.
+  const uint64_t items = (a.rows / S::BM + std::min(a.rows, a.groups)) * parts(a.outer, S::BN);
+  if (ring) {
+    auto kernel = transposed ? productRingKernel<T, true, S::BM, S::BN, S::WM, S::WN, S::R> : productRingKernel<T, false, S::BM, S::BN, S::WM, S::WN, S::R>;
+    return launchRows(kernel, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, (uint64_t)ringBlocks(items));
+  }
+  if constexpr (S::BM <= 128) {
+    auto kernel = transposed ? productKernel<T, true, S::BM, S::BN, S::WM, S::WN> : productKernel<T, false, S::BM, S::BN, S::WM, S::WN>;
+    return launchRows(kernel, blocksFor(items), S::THREADS, 0, stream, a, items);
+  }
+  return 0;
+}
+
 template <typename T>
 int product(const cuttHipProductArgs& a, bool transposed, void* stream) {
-  // Tiles that suffice whatever the groups are: whole ones of all rows, and one more for every group that has a row.
-  const auto items = [&](uint32_t bm, uint32_t bn) { return (a.rows / bm + std::min(a.rows, a.groups)) * parts(a.outer, bn); };
   const bool ring = inReach<T>(a.x, 0, a.xStride, 256, a.inner) && (transposed ? inReach<T>(a.w, a.wGroup, a.wRow, 256, a.inner) : inReach<T>(a.w, a.wGroup, a.wRow, a.inner, a.outer));
-  if (ring && sizeof(T) == 2) {
-    constexpr int BM = 256, BN = 256;
-    const uint64_t n = ringBlocks(items(BM, BN));
-    auto kernel = transposed ? productRingKernel<T, true, BM, BN, 2, 2, 2> : productRingKernel<T, false, BM, BN, 2, 2, 2>;
-    return launchRows(kernel, (uint32_t)n, 256, 2 * (BM + BN) * 128, stream, a, n);
+  const uint32_t rows = a.rows / a.groups;
+  if constexpr (sizeof(T) == 4) {
+    if (rows <= 4) return productAs<T, Shape<16, 128, 1, 4, 4>>(a, transposed, ring, stream);
+    if (rows <= 64) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
+    return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
   }
-  constexpr int BM = 128, BN = 128;
-  auto kernel = transposed ? productKernel<T, true, BM, BN, 2, 2> : productKernel<T, false, BM, BN, 2, 2>;
-  return launchRows(kernel, blocksFor(items(BM, BN)), 256, 0, stream, a, items(BM, BN));
+  if (rows <= kRows32) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
+  if (rows <= kRows64) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
+  if (!ring || rows <= kRows128) return productAs<T, Shape<128, 128, 2, 2, 2>>(a, transposed, ring, stream);
+  return productAs<T, Shape<256, 256, 2, 2, 2>>(a, transposed, ring, stream);
+}
+
+template <typename T, typename S>
+int weightsAs(const cuttHipProductArgs& a, bool ring, void* stream) {
+  const uint64_t items = parts(a.inner, S::BM) * parts(a.outer, S::BN) * a.groups;
+  if (ring)
+    return launchRows(weightsRingKernel<T, S::BM, S::BN, S::WM, S::WN, S::R>, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, (uint64_t)ringBlocks(items));
+  if constexpr (S::BM <= 128) return launchRows(weightsKernel<T, S::BM, S::BN, S::WM, S::WN>, blocksFor(items), S::THREADS, 0, stream, a, items);
+  return 0;
 }
 
 template <typename T>
 int weights(const cuttHipProductArgs& a, void* stream) {
-  const auto items = [&](uint32_t bm, uint32_t bn) { return parts(a.inner, bm) * parts(a.outer, bn) * a.groups; };
   const bool ring = inReach<T>(a.x, 0, a.xStride, a.rows, a.inner) && inReach<T>(a.w, 0, a.wRow, a.rows, a.outer);
-  if (ring && sizeof(T) == 2) {
-    constexpr int BM = 256, BN = 256;
-    const uint64_t n = ringBlocks(items(BM, BN));
-    return launchRows(weightsRingKernel<T, BM, BN, 2, 2, 2>, (uint32_t)n, 256, 2 * (BM + BN) * 128, stream, a, n);
-  }
-  constexpr int BM = 128, BN = 128;
-  return launchRows(weightsKernel<T, BM, BN, 2, 2>, blocksFor(items(BM, BN)), 256, 0, stream, a, items(BM, BN));
+  if (!ring || sizeof(T) == 4 || a.rows / a.groups <= kRowsWeights) return weightsAs<T, Shape<128, 128, 2, 2, 2>>(a, ring, stream);
+  return weightsAs<T, Shape<256, 256, 2, 2, 2>>(a, ring, stream);
 }
 
 }  // namespace
