@@ -66,46 +66,67 @@ struct Tile {
   static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) { return row * PER + (piece ^ skew(row)); }
 };
 
-// An operand's part that a tile is taken from: `along` elements along k and `across` the other way.  A lane's 16 bytes that would reach beyond a row's end are loaded from
-// so much further up that they end with it, and moved when they go to LDS.
+// An operand's part that a tile is taken from: `along` elements along k and `across` the other way.  Rows and columns of results that nobody stores are made of whatever is
+// at hand: there the last line is loaded again.  A lane's 16 bytes that would reach beyond a row's end are loaded from so much further up that they end with it, and
+// moved when they go to LDS; rows shorter than 16 bytes are loaded element by element.
 template <typename T, bool ACROSS, int B, int THREADS>
 struct Loader {
   using L = Tile<T, ACROSS, B>;
   static constexpr int N = (L::PIECES + THREADS - 1) / THREADS;
+  static constexpr uint32_t E = L::E, ROWS = THREADS / L::PER;  // of one access of the workgroup
+  static_assert(THREADS % L::PER == 0 && (!ACROSS || L::PIECES % THREADS == 0), "whole rows");
   Chunk<T> held[N];
-  struct Place {
-    uint32_t row, col;
-    int valid;  // elements of the 16 bytes, 0 to E
-    __device__ __forceinline__ Place(int i, uint32_t along, uint32_t across, uint32_t k) {
-      const uint32_t p = threadIdx.x + i * THREADS, r = p / L::PER, c = p % L::PER * L::E;
-      row = ACROSS ? k + r : r;
-      col = ACROSS ? c : k + c;
-      const uint32_t rows = ACROSS ? along : across, cols = ACROSS ? across : along;
-      valid = p < L::PIECES && row < rows && col < cols ? (int)min(cols - col, (uint32_t)L::E) : 0;
-    }
-  };
-  __device__ __forceinline__ void load(const T* from, uint64_t stride, uint32_t along, uint32_t across, uint32_t k) {
-    const bool narrow = (ACROSS ? across : along) < (uint32_t)L::E;
+  const T* from[ACROSS ? 1 : N];
+  uint32_t turn = 0;  // bits to move
+  uint64_t stride;
+  uint32_t along, across;
+  static __device__ __forceinline__ uint32_t row(int i) { return threadIdx.x / L::PER + i * ROWS; }
+  static __device__ __forceinline__ uint32_t column() { return threadIdx.x % L::PER * E; }
+  __device__ __forceinline__ const T* at(int i) const { return ACROSS ? from[0] + i * ROWS * stride : from[i]; }
+  __device__ __forceinline__ Loader(const T* base, uint64_t stride_, uint32_t along_, uint32_t across_) : stride(stride_), along(along_), across(across_) {
+    if constexpr (ACROSS) {
+      const uint32_t col = column() < across ? column() : 0, over = across < E ? 0 : col + E - min(col + E, across);
+      from[0] = base + (row(0) * stride + col - over);
+      turn = over * 8 * sizeof(T);
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const Place at(i, along, across, k);
-      const T* const p = from + (at.row * stride + at.col);
-      held[i] = {};
-      if (narrow) held[i] = loadChunk(p, at.valid);
-      else if (at.valid) held[i] = __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Vec<T, L::E>*>(p - (L::E - at.valid)));
+      for (int i = 0; i < N; i++) from[i] = base + (min(row(i), across - 1) * stride + column());
     }
   }
-  // With the same arguments as the load.
-  __device__ __forceinline__ void store(Chunk<T>* lds, uint32_t along, uint32_t across, uint32_t k) const {
-    const bool narrow = (ACROSS ? across : along) < (uint32_t)L::E;
+  // The tile at k, which is below `along`; the tiles one after the other.
+  __device__ __forceinline__ void load(uint32_t k) {
+    const auto whole = [](const T* p) __attribute__((always_inline)) { return __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Vec<T, E>*>(p)); };
+    if (along - k >= L::K && (!ACROSS || across >= E)) {
+#pragma unroll
+      for (int i = 0; i < N; i++) held[i] = whole(at(i));
+    } else if constexpr (ACROSS) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        held[i] = {};
+        if (row(i) >= along - k) continue;
+        if (across >= E) held[i] = whole(at(i));
+        else if (column() == 0) held[i] = loadChunk(at(i), (int)across);
+      }
+    } else {
+      const uint32_t left = along - k > column() ? min(along - k - column(), E) : 0, over = along < E ? 0 : E - left;
+      turn = over * 8 * sizeof(T) % 128;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        held[i] = {};
+        if (along < E) held[i] = loadChunk(at(i), (int)left);
+        else if (left) held[i] = whole(at(i) - over);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < (ACROSS ? 1 : N); i++) from[i] += ACROSS ? L::K * stride : L::K;
+  }
+  // What the load got.
+  __device__ __forceinline__ void store(Chunk<T>* lds) const {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const uint32_t p = threadIdx.x + i * THREADS;
-      const Place at(i, along, across, k);
       Chunk<T> v = held[i];
-      if (!narrow && at.valid && at.valid < L::E)
-        v = __builtin_bit_cast(Chunk<T>, __builtin_bit_cast(unsigned __int128, v) >> (uint32_t)((L::E - at.valid) * 8 * sizeof(T)));
-      if (p < L::PIECES) lds[L::place(p / L::PER, p % L::PER)] = v;
+      if (turn) v = __builtin_bit_cast(Chunk<T>, __builtin_bit_cast(unsigned __int128, v) >> turn);
+      if (L::PIECES % THREADS == 0 || row(i) < L::PIECES / L::PER) lds[L::place(row(i), threadIdx.x % L::PER)] = v;
     }
   }
 };
@@ -159,14 +180,14 @@ struct Fragments {
   static __device__ __forceinline__ uint32_t rowOf(int t, uint32_t l) { return ACROSS ? t / C * 16 * C + l * C + t % C : t * 16 + l; }
 };
 
-// The first n of N results of a row, side by side.
-template <typename T, int N>
+// The first n of N results of a row, side by side.  ONCE: past the caches.
+template <bool ONCE, typename T, int N>
 __device__ __forceinline__ void storeSome(T* p, const float (&v)[N], uint32_t n) {
   Pack<T, N> o;
 #pragma unroll
   for (int i = 0; i < N; i++) o.set(i, (T)v[i]);
   if (n >= N) {
-    o.store(p);
+    o.template store<ONCE>(p);
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < N; i++)
@@ -174,33 +195,51 @@ __device__ __forceinline__ void storeSome(T* p, const float (&v)[N], uint32_t n)
   }
 }
 
+// A row of results' fragments: those of M's rows b times those of N's rows a.  An instruction's result has one operand's rows along the lanes and four of the other's in each.
+// Whichever a row's neighbouring results come of goes where a lane gets several side by side, and lanes beside each other go on: with N across, N's rows along the lanes.
+// (The 32-bit type's four instructions for the same results wait for each other: others between them.)
+template <bool NACROSS, typename T, int FN>
+__device__ __forceinline__ void addProducts(const Chunk<T> (&a)[FN], const Chunk<T>& b, Acc (&acc)[FN]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) acc[j] = NACROSS ? multiply(b[e], a[j][e], acc[j]) : multiply(a[j][e], b[e], acc[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < FN; j++) acc[j] = NACROSS ? multiply(b, a[j], acc[j]) : multiply(a[j], b, acc[j]);
+  }
+}
+
 // A wavefront's results, rows m0 and columns n0 on of m and n, to `to`.
-template <typename T, bool MACROSS, bool NACROSS, int BM, int BN, int FM, int FN>
+template <typename T, bool MACROSS, bool NACROSS, int BM, int BN, bool ONCE, int FM, int FN>
 __device__ __forceinline__ void storeResults(const Acc (&acc)[FM][FN], T* to, uint64_t stride, uint32_t m0, uint32_t m, uint32_t n0, uint32_t n) {
   using N = Fragments<T, NACROSS, BN, FN>;
   const uint32_t l = threadIdx.x & 15, quarter = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int i = 0; i < FM; i++) {
-    const uint32_t row = m0 + Fragments<T, MACROSS, BM, FM>::rowOf(i, l);
-    if (row >= m) continue;
-    T* const line = to + row * stride;
     if constexpr (NACROSS) {
 #pragma unroll
-      for (int j = 0; j < FN; j += N::C)
+      for (int r = 0; r < 4; r++) {
+        const uint32_t row = m0 + Fragments<T, MACROSS, BM, FM>::rowOf(i, quarter * 4 + r);
+        if (row >= m) continue;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const uint32_t col = n0 + N::rowOf(j, quarter * 4 + r);
+        for (int j = 0; j < FN; j += N::C) {
+          const uint32_t col = n0 + N::rowOf(j, l);
           float v[N::C];
 #pragma unroll
           for (int x = 0; x < N::C; x++) v[x] = acc[i][j + x][r];
-          if (col < n) storeSome(line + col, v, n - col);
+          if (col < n) storeSome<ONCE>(to + (row * stride + col), v, n - col);
         }
+      }
     } else {
+      const uint32_t row = m0 + Fragments<T, MACROSS, BM, FM>::rowOf(i, l);
+      if (row >= m) continue;
 #pragma unroll
       for (int j = 0; j < FN; j++) {
         const uint32_t col = n0 + j * 16 + quarter * 4;
         const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (col < n) storeSome(line + col, v, n - col);
+        if (col < n) storeSome<ONCE>(to + (row * stride + col), v, n - col);
       }
     }
   }
@@ -214,22 +253,22 @@ __device__ __forceinline__ void productTile(const T* from, uint64_t mStride, uin
   const uint32_t wave = threadIdx.x >> 6;
   const uint32_t m0 = wave / WN * (BM / WM), n0 = wave % WN * (BN / WN);
   Chunk<T>* const ldsN = lds + 8 * BM;
-  Loader<T, MACROSS, BM, THREADS> loadM;
-  Loader<T, NACROSS, BN, THREADS> loadN;
+  Loader<T, MACROSS, BM, THREADS> loadM(from, mStride, along, m);
+  Loader<T, NACROSS, BN, THREADS> loadN(with, nStride, along, n);
   Acc acc[FM][FN] = {};
   if (along) {
-    loadM.load(from, mStride, along, m, 0);
-    loadN.load(with, nStride, along, n, 0);
+    loadM.load(0);
+    loadN.load(0);
   }
   constexpr uint32_t K = 128 / sizeof(T);
   for (uint64_t k = 0; k < along; k += K) {
     __syncthreads();
-    loadM.store(lds, along, m, (uint32_t)k);
-    loadN.store(ldsN, along, n, (uint32_t)k);
+    loadM.store(lds);
+    loadN.store(ldsN);
     __syncthreads();
     if (k + K < along) {
-      loadM.load(from, mStride, along, m, (uint32_t)k + K);
-      loadN.load(with, nStride, along, n, (uint32_t)k + K);
+      loadM.load((uint32_t)k + K);
+      loadN.load((uint32_t)k + K);
     }
 #pragma unroll
     for (int s = 0; s < 2; s++) {
@@ -237,13 +276,14 @@ __device__ __forceinline__ void productTile(const T* from, uint64_t mStride, uin
       Fragments<T, NACROSS, BN, FN> fn;
       fm.load(lds, m0, s);
       fn.load(ldsN, n0, s);
+      Chunk<T> a[FN];
 #pragma unroll
-      for (int i = 0; i < FM; i++)
+      for (int j = 0; j < FN; j++) a[j] = fn.at(j);
 #pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = multiply(fn.at(j), fm.at(i), acc[i][j]);
+      for (int i = 0; i < FM; i++) addProducts<NACROSS, T>(a, fm.at(i), acc[i]);
     }
   }
-  storeResults<T, MACROSS, NACROSS, BM, BN>(acc, to, toStride, m0, m, n0, n);
+  storeResults<T, MACROSS, NACROSS, BM, BN, false>(acc, to, toStride, m0, m, n0, n);
 }
 
 // ---------------------------------------------------------------------------
@@ -336,11 +376,10 @@ __device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uin
     for (int i = 0; i < FM; i++) {
       other(i, FM);
       const Chunk<T> b = fm[s].at(i);
+      if (i == 0)
 #pragma unroll
-      for (int j = 0; j < FN; j++) {
-        if (i == 0) a[j] = fn[s].at(j);
-        acc[i][j] = multiply(a[j], b, acc[i][j]);
-      }
+        for (int j = 0; j < FN; j++) a[j] = fn[s].at(j);
+      addProducts<NACROSS, T>(a, b, acc[i]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -364,11 +403,11 @@ __device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uin
   }
   waitForLoads<0>();
   meet();
-  storeResults<T, MACROSS, NACROSS, BM, BN>(acc, to, toStride, m0, m, n0, n);
+  storeResults<T, MACROSS, NACROSS, BM, BN, MACROSS>(acc, to, toStride, m0, m, n0, n);
 }
 
 // Items for the workgroups in groups of kNear to an XCD, whose L2 they share.
-constexpr uint32_t kNear = 32;
+constexpr uint32_t kNear = 16;
 __device__ __forceinline__ uint64_t itemOf(uint64_t block) { return block / (8 * kNear) * (8 * kNear) + block % 8 * kNear + block / 8 % kNear; }
 // Which of a group's tiles x strips number `item` is: blocks of kWide strips one after the other, in a block tile by tile, so that items that follow each other share
 // both operands.
@@ -456,10 +495,11 @@ bool inReach(const void* p, uint64_t group, uint64_t stride, uint64_t lines, uin
   return ((uintptr_t)p | group * sizeof(T) | stride * sizeof(T) | width * sizeof(T)) % 16 == 0 && stride < (1u << 30) &&
          (lines * stride + width) * sizeof(T) < (1u << 30);
 }
-// (workgroups whose items are handed out kNear to an XCD at a time: whole rounds)
-uint32_t ringBlocks(uint64_t items) { return (uint32_t)std::min<uint64_t>((items + 8 * kNear - 1) / (8 * kNear) * (8 * kNear), kMaxBlocks); }
+// (items are handed out kNear to an XCD at a time: whole rounds)
+uint64_t ringItems(uint64_t items) { return parts(items, 8 * kNear) * (8 * kNear); }
+uint32_t ringBlocks(uint64_t items) { return (uint32_t)std::min<uint64_t>(ringItems(items), kMaxBlocks); }
 
-constexpr uint32_t kRows32 = 4, kRows64 = 48, kRows128 = 320, kRowsWeights = 512;
+constexpr uint32_t kRows32 = 8, kRows64 = 48, kRows64Transposed = 80, kRows128 = 320, kRowsWeights = 512;
 
 template <int M, int N, int WAVES_M, int WAVES_N, int PLACES>
 struct Shape {
@@ -472,7 +512,7 @@ int productAs(const cuttHipProductArgs& a, bool transposed, bool ring, void* str
   const uint64_t items = (a.rows / S::BM + std::min(a.rows, a.groups)) * parts(a.outer, S::BN);
   if (ring) {
     auto kernel = transposed ? productRingKernel<T, true, S::BM, S::BN, S::WM, S::WN, S::R> : productRingKernel<T, false, S::BM, S::BN, S::WM, S::WN, S::R>;
-    return launchRows(kernel, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, (uint64_t)ringBlocks(items));
+    return launchRows(kernel, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, ringItems(items));
   }
   if constexpr (S::BM <= 128) {
     auto kernel = transposed ? productKernel<T, true, S::BM, S::BN, S::WM, S::WN> : productKernel<T, false, S::BM, S::BN, S::WM, S::WN>;
@@ -491,7 +531,7 @@ int product(const cuttHipProductArgs& a, bool transposed, void* stream) {
     return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
   }
   if (rows <= kRows32) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
-  if (rows <= kRows64) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
+  if (rows <= (transposed ? kRows64Transposed : kRows64)) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
   if (!ring || rows <= kRows128) return productAs<T, Shape<128, 128, 2, 2, 2>>(a, transposed, ring, stream);
   return productAs<T, Shape<256, 256, 2, 2, 2>>(a, transposed, ring, stream);
 }
@@ -500,7 +540,7 @@ template <typename T, typename S>
 int weightsAs(const cuttHipProductArgs& a, bool ring, void* stream) {
   const uint64_t items = parts(a.inner, S::BM) * parts(a.outer, S::BN) * a.groups;
   if (ring)
-    return launchRows(weightsRingKernel<T, S::BM, S::BN, S::WM, S::WN, S::R>, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, (uint64_t)ringBlocks(items));
+    return launchRows(weightsRingKernel<T, S::BM, S::BN, S::WM, S::WN, S::R>, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, ringItems(items));
   if constexpr (S::BM <= 128) return launchRows(weightsKernel<T, S::BM, S::BN, S::WM, S::WN>, blocksFor(items), S::THREADS, 0, stream, a, items);
   return 0;
 }
@@ -508,8 +548,10 @@ int weightsAs(const cuttHipProductArgs& a, bool ring, void* stream) {
 template <typename T>
 int weights(const cuttHipProductArgs& a, void* stream) {
   const bool ring = inReach<T>(a.x, 0, a.xStride, a.rows, a.inner) && inReach<T>(a.w, 0, a.wRow, a.rows, a.outer);
-  if (!ring || sizeof(T) == 4 || a.rows / a.groups <= kRowsWeights) return weightsAs<T, Shape<128, 128, 2, 2, 2>>(a, ring, stream);
-  return weightsAs<T, Shape<256, 256, 2, 2, 2>>(a, ring, stream);
+  if constexpr (sizeof(T) == 2)
+    if (ring && a.rows / a.groups > kRowsWeights) return weightsAs<T, Shape<256, 256, 2, 2, 2>>(a, ring, stream);
+  if (sizeof(T) == 4 && !ring) return weightsAs<T, Shape<64, 128, 2, 2, 2>>(a, false, stream);
+  return weightsAs<T, Shape<128, 128, 4, 1, 2>>(a, ring, stream);
 }
 
 }  // namespace
