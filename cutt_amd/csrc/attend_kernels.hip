@@ -16,23 +16,25 @@ using Is = std::integral_constant<bool, X>;
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 constexpr uint32_t kColumns = 16;  // of the matrix instructions: query heads of one key head
 constexpr uint32_t kPhase = 1024;  // tokens whose addresses a workgroup works out at a time
-constexpr uint32_t kScan = 2048;   // queries that are shared out evenly
+constexpr uint32_t kScan = 2048;   // queries that are shared out evenly, at most
 constexpr uint32_t kCut = 128;     // queries are cut at multiples of this many tokens: a tile for every wavefront
 constexpr uint32_t kExtra = 128;   // tokens in whose time a workgroup begins a query and ends it
 
 // How the work is shared out.  The tokens that the queries see, with kExtra more for each, lie one behind the other, and are cut into ranges of even lengths, one for each
 // workgroup (of a key head's).  The cuts move to where a query begins or a little further in it, so that a range may take the end of one query's tokens, some whole
 // queries and the begin of another.  Where there are many more workgroups than queries, each query has ranges of its own instead, and no workgroup has two to begin.
+// Where there are many queries none looks at the others: each is a range, or a few of a length that is known before.
 struct Attend {
   cuttHipAttendArgs a;
   uint32_t group, headTiles;  // query heads per key head, and workgroups that share them
   uint32_t most;              // neighbouring queries of one request that a workgroup takes together, a power of two: their heads share its columns
-  uint32_t ranges;            // 0: each query is a range
+  uint32_t ranges;            // 0: each query has `pieces` of its own, of `length` tokens (the last one what is left)
+  uint32_t pieces, length;
   uint32_t each;              // each query is cut into ranges of its own
   float perRange;             // what length of a range, by all tokens, makes no more than `ranges`
-  cuttHipDivisor byPage, byTiles, byHeads, byShares;  // divisions by pageSize, headTiles, the heads in a column tile and eight times all workgroups of a range
-  float* partial;             // [2 * ranges][most][heads][width]: of what begins within a query, and of what ends in one
-  float* tops;                // [2 * ranges][most][heads][2]: the largest score or near it, and the sum of the exponentials that it was taken off
+  cuttHipDivisor byPage, byTiles, byHeads, byShares;  // divisions by pageSize, headTiles, the heads in a column tile and all workgroups of a range
+  float* partial;             // [2 * ranges][most][heads][width]: of what begins within a query, and of what ends in one; or [queries][pieces][heads][width]
+  float* tops;                // [2 * ranges][most][heads][2] or likewise: the largest score or near it, and the sum of the exponentials that it was taken off
   uint32_t* cuts;             // [queries][4]: first range, number of ranges, place among the queries that are taken together
 };
 
@@ -79,7 +81,7 @@ struct ScanLds {
   Cut cut[2];
   Seen seen;          // what the range's first queries see, and how many they are
   uint32_t queries;   // (0: they are the ones behind those that the cut was in)
-  uint64_t before;    // tokens before them; where each query is cut by itself, its pieces
+  uint64_t before;    // tokens before them; where each query is cut by itself, its ranges
 };
 
 __device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y) { return x + y; }
@@ -89,7 +91,7 @@ struct Range {
   Cut from, to;
   Seen seen;
   uint32_t queries;
-  uint64_t before, length;  // length: of all ranges, before the cuts move
+  uint64_t before, length;  // length: of all ranges, before the cuts move.  (Queries that are cut by themselves: `before` is how many ranges this one has.)
 };
 
 // A cut that would come before token `at` of a query's `tokens` moves to the nearest multiple of kCut, or to the query's end (returned as ~0) if there would be little left.
@@ -104,10 +106,15 @@ __device__ __forceinline__ uint64_t cutsEnd(uint32_t tokens) { return tokens < k
 __device__ __forceinline__ bool findRange(const Attend& p, uint32_t index, ScanLds& s, Range& r) {
   const cuttHipAttendArgs& a = p.a;
   if (!p.ranges) {
-    if (index >= a.queries || follows(p, index)) return false;
-    r.from = {index, 0};
-    r.queries = together(p, index, r.seen);
-    r.to = {index + r.queries, 0};
+    const uint32_t query = index / p.pieces, piece = index - query * p.pieces;
+    if (query >= a.queries || follows(p, query)) return false;
+    r.queries = together(p, query, r.seen);
+    const uint32_t tokens = r.seen.end - r.seen.first, begin = piece * p.length;
+    if (piece && begin >= tokens) return false;
+    const bool last = piece + 1 == p.pieces || tokens - begin <= p.length;
+    r.from = {query, begin};
+    r.to = {last ? query + r.queries : query, last ? 0 : begin + p.length};
+    if (!last) r.before = min((tokens - 1) / p.length + 1, p.pieces);
     return true;
   }
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -270,9 +277,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
   const uint32_t lane = threadIdx.x & 63, l = lane & 15, quarter = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int width = (int)a.width;
   const float scale = a.scale * kLog2e;
-  // Workgroups that follow each other go to the XCDs in turn: eight ranges at a time, all heads of a range to one XCD.
-  const uint32_t shares = a.keyHeads * p.headTiles, eights = divide(blockIdx.x, p.byShares), in = blockIdx.x - eights * shares * 8;
-  const uint32_t index = firstRange + eights * 8 + in % 8, share = in / 8;
+  // Workgroups that follow each other go to the XCDs in turn: so that none has much more to do than another, a range's heads follow each other, and the eight ranges that
+  // do are turned on from eight to eight (every fourth range may be all that has work, as drafted tokens are taken together).
+  const uint32_t shares = a.keyHeads * p.headTiles, at = divide(blockIdx.x, p.byShares), share = blockIdx.x - at * shares;
+  const uint32_t index = firstRange + (at & ~7u) + ((at + at / 8) & 7);
   const uint32_t keyHead = divide(share, p.byTiles), headTile = share - keyHead * p.headTiles;
   const uint32_t head0 = keyHead * p.group + headTile * kColumns, nHeads = min(p.group - headTile * kColumns, kColumns);
   const T* const kHead = static_cast<const T*>(a.k) + keyHead * a.cacheHead;
@@ -603,7 +611,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
 #pragma unroll
     for (uint32_t w = 0; w < kWaves; w++) of += sums[w * kColumns + c] * exp2Of(tops[w * kColumns + c] - baseOf(m));
     const bool none = of == 0 && m == -INFINITY;
-    const uint64_t row = ((uint64_t)slot * p.most + n) * a.heads + h, to = range.from.query + n;
+    const uint64_t to = range.from.query + n;
+    const uint64_t row = (p.ranges ? (uint64_t)slot * p.most + n : to * p.pieces + (index - range.from.query * p.pieces)) * a.heads + h;
     for (uint32_t d = lane; d < a.width; d += 64) {
       float o = 0;
 #pragma unroll
@@ -619,10 +628,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
     }
   }
 
-  if (p.ranges && range.from.from == 0 && share == 0 && threadIdx.x < queries) {
+  if ((p.ranges || p.pieces > 1) && range.from.from == 0 && share == 0 && threadIdx.x < queries) {
     uint32_t* const to = p.cuts + (range.from.query + threadIdx.x) * 4;
     to[0] = index;
-    to[1] = ends ? 1 : p.each ? (uint32_t)range.before : (uint32_t)((range.before + cutsEnd(tokensInAll) + range.length - 1) / range.length) - index;
+    to[1] = ends ? 1 : p.each || !p.ranges ? (uint32_t)range.before : (uint32_t)((range.before + cutsEnd(tokensInAll) + range.length - 1) / range.length) - index;
     to[2] = threadIdx.x;
   }
   range.from = {range.from.query + queries, 0};
@@ -645,9 +654,10 @@ __global__ __launch_bounds__(kThreads) void joinKernel(Attend p) {
     const uint32_t* const cut = p.cuts + query * 4;
     const uint32_t first = cut[0], ranges = cut[1];
     if (ranges <= 1) continue;
-    const uint64_t step = (uint64_t)p.most * a.heads, place = (uint64_t)cut[2] * a.heads + head;
     // Its first range ends in it, the others begin in it.
-    const auto rowOf = [&](uint32_t i) __attribute__((always_inline)) { return (2 * ((uint64_t)first + i) + (i == 0)) * step + place; };
+    const auto rowOf = [&](uint32_t i) __attribute__((always_inline)) {
+      return (p.ranges ? (2 * ((uint64_t)first + i) + (i == 0)) * p.most + cut[2] : (uint64_t)query * p.pieces + i) * a.heads + head;
+    };
     // A wavefront joins every kWaves-th of them, AT at a time, whose loads go out together.
     constexpr uint32_t AT = 4, PER = CUTT_MAX_HEAD_WIDTH / 64;
     float m = -INFINITY, n = 0, o[PER] = {};
@@ -704,22 +714,34 @@ __global__ __launch_bounds__(kThreads) void joinKernel(Attend p) {
 
 constexpr uint32_t kMaxBlocks = 1u << 22;
 
-Attend planAttend(uint32_t queries, uint32_t heads, uint32_t keyHeads, uint32_t width, uint32_t pageSize) {
+constexpr uint32_t kManyBlocks = 256, kShort = 256, kPieces = 8, kLeastPiece = 2048, kPieceBlocks = 16384;
+
+Attend planAttend(uint32_t queries, uint32_t heads, uint32_t keyHeads, uint32_t width, uint32_t pageSize, uint32_t tableWidth, uint32_t window) {
   Attend p = {};
   p.group = heads / keyHeads;
   p.headTiles = (p.group + kColumns - 1) / kColumns;
   for (p.most = 1; p.most * 2 * p.group <= kColumns;) p.most *= 2;
   p.byPage = cuttHipMakeDivisor(pageSize);
   p.byTiles = cuttHipMakeDivisor(p.headTiles);
-  p.byShares = cuttHipMakeDivisor(keyHeads * p.headTiles * 8);
+  p.byShares = cuttHipMakeDivisor(keyHeads * p.headTiles);
   p.byHeads = cuttHipMakeDivisor(std::min(p.group, kColumns));
+  const uint64_t shares = (uint64_t)keyHeads * p.headTiles, blocks = queries * shares;
+  const uint64_t reach = std::min((uint64_t)tableWidth * pageSize, window ? (uint64_t)window + p.most : (uint64_t)1 << 31);
+  if (queries > kScan || blocks / p.most >= kManyBlocks || reach <= kShort) {
+    p.pieces = (uint32_t)std::max<uint64_t>(std::min({(uint64_t)kPieces, kPieceBlocks / std::max<uint64_t>(blocks, 1), reach / kLeastPiece}), 1);
+    p.length = (uint32_t)((reach + p.pieces * kCut - 1) / (p.pieces * kCut) * kCut);
+    return p;
+  }
   // As many workgroups as run at a time.
-  if (queries <= kScan) p.ranges = std::max(1u, (width <= 64 ? 768 : width <= 128 ? 512 : 256) / (keyHeads * p.headTiles));
+  p.ranges = std::max(1u, (width <= 64 ? 768 : width <= 128 ? 512 : 256) / (uint32_t)shares);
   // (each query's last range may be a short one; and there are kThreads queries at most, one for each thread that looks)
   p.each = queries <= kThreads && queries * 4 <= p.ranges;
   p.perRange = p.ranges ? 1.0001f / (p.each ? p.ranges - queries : p.ranges) : 0.0f;
   return p;
 }
+
+// Parts of queries that the workspace has room for.
+size_t rowsOf(const Attend& p, uint32_t queries) { return p.ranges ? 2 * (size_t)p.ranges * p.most : p.pieces > 1 ? (size_t)queries * p.pieces : 0; }
 
 template <typename T, int DP, bool DIRECT>
 int attend(const Attend& p, void* stream) {
@@ -727,12 +749,12 @@ int attend(const Attend& p, void* stream) {
   const size_t lds = std::max({space, sizeof(ScanLds), join});
   const uint32_t shares = p.a.keyHeads * p.headTiles;
   const uint32_t most = std::max(1u, (1u << 20) / shares) * 8;  // (a launch's lanes stay below 2^32)
-  const uint64_t ranges = p.ranges ? p.ranges : p.a.queries;
+  const uint64_t ranges = p.ranges ? p.ranges : (uint64_t)p.a.queries * p.pieces;
   for (uint64_t first = 0; first < ranges; first += most) {
     const uint32_t blocks = ((uint32_t)std::min<uint64_t>(ranges - first, most) + 7) / 8 * 8 * shares;
     if (int e = launchRows(attendKernel<T, DP, DIRECT>, blocks, kThreads, lds, stream, p, (uint32_t)first)) return e;
   }
-  if (!p.ranges) return 0;
+  if (!p.ranges && p.pieces == 1) return 0;
   return launchRows(joinKernel<T>, (uint32_t)std::min<uint64_t>((uint64_t)p.a.queries * p.a.heads, kMaxBlocks), kThreads, 0, stream, p);
 }
 
@@ -750,19 +772,20 @@ int attendType(const Attend& p, void* stream) {
 
 }  // namespace
 
-extern "C" size_t cuttHipAttendWorkspace(uint32_t queries, uint32_t heads, uint32_t keyHeads, uint32_t width, uint32_t pageSize, uint32_t, uint32_t) {
-  const Attend p = planAttend(queries, heads, keyHeads, width, pageSize);
-  return p.ranges ? (2 * (size_t)p.ranges * p.most * heads * (width + 2) + 4 * (size_t)queries) * 4 : 0;
+extern "C" size_t cuttHipAttendWorkspace(uint32_t queries, uint32_t heads, uint32_t keyHeads, uint32_t width, uint32_t pageSize, uint32_t tableWidth, uint32_t window) {
+  const Attend p = planAttend(queries, heads, keyHeads, width, pageSize, tableWidth, window);
+  const size_t rows = rowsOf(p, queries) * heads;
+  return rows ? (rows * (width + 2) + 4 * (size_t)queries) * 4 : 0;
 }
 
 extern "C" int cuttHipAttend(const cuttHipAttendArgs* a, int type, void* stream) {
-  Attend p = planAttend(a->queries, a->heads, a->keyHeads, a->width, a->pageSize);
+  Attend p = planAttend(a->queries, a->heads, a->keyHeads, a->width, a->pageSize, a->tableWidth, a->window);
   p.a = *a;
   float* const space = static_cast<float*>(a->workspace);
-  const size_t slots = 2 * (size_t)p.ranges * p.most * a->heads;
+  const size_t rows = rowsOf(p, a->queries) * a->heads;
   p.tops = space;
-  p.partial = space + 2 * slots;
-  p.cuts = reinterpret_cast<uint32_t*>(p.partial + slots * a->width);
+  p.partial = space + 2 * rows;
+  p.cuts = reinterpret_cast<uint32_t*>(p.partial + rows * a->width);
   switch (type) {
     case CUTT_ROW_F32: return attendType<float>(p, stream);
     case CUTT_ROW_F16: return attendType<_Float16>(p, stream);

@@ -383,6 +383,30 @@ def test_attend(lengths, page, heads, key_heads, width, window, layout, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("requests,drafts,longest,heads,key_heads,width,window,idle", [
+    (40, 1, 700, 16, 8, 64, 0, 5),       # ranges that begin and end within queries
+    (30, 3, 500, 8, 8, 128, 0, 7),       # drafted tokens, taken together
+    (50, 2, 900, 12, 12, 80, 300, 9),
+    (256, 1, 4500, 16, 1, 64, 0, 3),     # queries in two pieces of their own
+    (700, 3, 4500, 2, 1, 64, 0, 50),     # and drafted ones
+    (700, 3, 4500, 2, 1, 64, 2300, 50),
+    (300, 4, 200, 8, 8, 64, 0, 4),       # a workgroup for each
+])
+def test_shares(requests, drafts, longest, heads, key_heads, width, window, idle, dtype):
+    """Many queries of long and short requests, every `idle`-th of which has no token."""
+    g = generator(18)
+    lengths = torch.randint(1, min(longest, 300), (requests,), generator=g, device="cuda").tolist()
+    lengths[::idle] = [0] * len(lengths[::idle])
+    lengths[1], lengths[requests // 2 | 1], lengths[-1] = longest, longest - 1, longest // 2 + 5
+    cache = Cache(lengths, 32, key_heads, width, dtype, "slot", g)
+    owners = ints([b for b in range(requests) for _ in range(drafts)])
+    positions = ints([n - drafts + i if n else -1 for n in lengths for i in range(drafts)])
+    q = (2 * torch.randn(requests * drafts, heads, width, generator=g, device="cuda")).to(dtype)
+    out, logs = run_attend(q, cache, owners, positions, window, width ** -0.5)
+    check_attend(q, cache, owners, positions, window, width ** -0.5, out, logs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 @pytest.mark.parametrize("window", [0, 10])
 def test_owners_and_positions(window, dtype):
     """Several queries of one request, queries of nobody, positions beyond the table, before the first token and far ones."""
