@@ -1,5 +1,13 @@
 /*
  * product_kernels.hip - rows grouped by expert times their experts' weights, and the weights' gradient (cutt_products.h).
+ *
+ * A group's product is cut into tiles of results, one for a workgroup.  The groups' sizes are known on the GPU alone: the host launches as many workgroups as any sizes can
+ * need, each finds its tile in the offsets, and those that are too many end.  No sum crosses a workgroup, so the results do not depend on timing, and an
+ * expert's sums run over all its rows in 32 bits, rounded once.
+ *
+ * What bounds it: with few rows per group the weights, read once (512 rows of 4096 x 1536 over 128 groups, bfloat16: 242 us, 6.6 TB/s); with many the matrix
+ * instructions and what feeds them (131072 rows of the same: 1640 us, 1.0 PFLOP/s; one group of 8192 rows and 8192 x 8192 weights 1.2, transposed 1.33, its gradient
+ * 0.95); the gradient of few rows writes its result (64 experts of 2048 x 1536, 16 rows each: 110 us, 3.7 TB/s).
  */
 #include <algorithm>
 
@@ -66,10 +74,18 @@ struct Tile {
   static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) { return row * PER + (piece ^ skew(row)); }
 };
 
+// A workgroup's tile of M x N results, made by WAVES_M x WAVES_N wavefronts, or by PARTS that share the k's; PLACES tiles of the operands in LDS.
+template <int M, int N, int WAVES_M, int WAVES_N, int PLACES, int PARTS = 1>
+struct Shape {
+  static constexpr int BM = M, BN = N, WM = WAVES_M, WN = WAVES_N, R = PLACES, SPLIT = PARTS, THREADS = WM * WN * SPLIT * 64;
+  static_assert(SPLIT == 1 || WM * WN == 1, "one or the other");
+  static constexpr uint32_t LDS = R * SPLIT * (BM + BN) * 128;
+};
+
 // An operand's part that a tile is taken from: `along` elements along k and `across` the other way.  Rows and columns of results that nobody stores are made of whatever is
 // at hand: there the last line is loaded again.  A lane's 16 bytes that would reach beyond a row's end are loaded from so much further up that they end with it, and
 // moved when they go to LDS; rows shorter than 16 bytes are loaded element by element.
-template <typename T, bool ACROSS, int B, int THREADS>
+template <typename T, bool ACROSS, int B, int THREADS, int EVERY>
 struct Loader {
   using L = Tile<T, ACROSS, B>;
   static constexpr int N = (L::PIECES + THREADS - 1) / THREADS;
@@ -80,7 +96,7 @@ struct Loader {
   uint32_t turn = 0;  // bits to move
   uint64_t stride;
   uint32_t along, across;
-  static __device__ __forceinline__ uint32_t row(int i) { return threadIdx.x / L::PER + i * ROWS; }
+  static __device__ __forceinline__ uint32_t row(int i) { return threadIdx.x % THREADS / L::PER + i * ROWS; }
   static __device__ __forceinline__ uint32_t column() { return threadIdx.x % L::PER * E; }
   __device__ __forceinline__ const T* at(int i) const { return ACROSS ? from[0] + i * ROWS * stride : from[i]; }
   __device__ __forceinline__ Loader(const T* base, uint64_t stride_, uint32_t along_, uint32_t across_) : stride(stride_), along(along_), across(across_) {
@@ -93,7 +109,7 @@ struct Loader {
       for (int i = 0; i < N; i++) from[i] = base + (min(row(i), across - 1) * stride + column());
     }
   }
-  // The tile at k, which is below `along`; the tiles one after the other.
+  // The tile at k, which is below `along`; every EVERY-th of the tiles, one after the other.
   __device__ __forceinline__ void load(uint32_t k) {
     const auto whole = [](const T* p) __attribute__((always_inline)) { return __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Vec<T, E>*>(p)); };
     if (along - k >= L::K && (!ACROSS || across >= E)) {
@@ -118,7 +134,7 @@ struct Loader {
       }
     }
 #pragma unroll
-    for (int i = 0; i < (ACROSS ? 1 : N); i++) from[i] += ACROSS ? L::K * stride : L::K;
+    for (int i = 0; i < (ACROSS ? 1 : N); i++) from[i] += EVERY * (ACROSS ? L::K * stride : L::K);
   }
   // What the load got.
   __device__ __forceinline__ void store(Chunk<T>* lds) const {
@@ -245,36 +261,59 @@ __device__ __forceinline__ void storeResults(const Acc (&acc)[FM][FN], T* to, ui
   }
 }
 
-// One tile of results: M [m rows] times N [n rows] over `along` k's, to `to`.
-template <typename T, bool MACROSS, bool NACROSS, int BM, int BN, int WM, int WN>
+// The sums that SPLIT wavefronts have made of the same results, each of its share of the k's, together in the first one, in the order of the wavefronts.
+template <int SPLIT, int FM, int FN>
+__device__ __forceinline__ void joinSums(Acc (&acc)[FM][FN], void* lds) {
+  Acc* const sums = static_cast<Acc*>(lds) + (threadIdx.x & 63);
+  const uint32_t wave = threadIdx.x >> 6;
+  __syncthreads();
+  if (wave)
+#pragma unroll
+    for (int i = 0; i < FM * FN; i++) sums[((wave - 1) * FM * FN + i) * 64] = acc[i / FN][i % FN];
+  __syncthreads();
+  if (!wave)
+#pragma unroll
+    for (int w = 0; w + 1 < SPLIT; w++)
+#pragma unroll
+      for (int i = 0; i < FM * FN; i++) acc[i / FN][i % FN] += sums[(w * FM * FN + i) * 64];
+}
+
+// One tile of results: M [m rows] times N [n rows] over `along` k's, to `to`.  SPLIT wavefronts share the k's, tile by tile, each with a part of LDS of its own.
+template <typename T, bool MACROSS, bool NACROSS, typename S>
 __device__ __forceinline__ void productTile(const T* from, uint64_t mStride, uint32_t m, const T* with, uint64_t nStride, uint32_t n, uint32_t along, T* to,
                                             uint64_t toStride, Chunk<T>* lds) {
-  constexpr int THREADS = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16;
-  const uint32_t wave = threadIdx.x >> 6;
-  const uint32_t m0 = wave / WN * (BM / WM), n0 = wave % WN * (BN / WN);
-  Chunk<T>* const ldsN = lds + 8 * BM;
-  Loader<T, MACROSS, BM, THREADS> loadM(from, mStride, along, m);
-  Loader<T, NACROSS, BN, THREADS> loadN(with, nStride, along, n);
+  constexpr int BM = S::BM, BN = S::BN, SPLIT = S::SPLIT, THREADS = S::THREADS / SPLIT, FM = BM / S::WM / 16, FN = BN / S::WN / 16;
+  constexpr uint32_t K = 128 / sizeof(T);
+  const uint32_t wave = threadIdx.x >> 6, part = SPLIT > 1 ? wave : 0;
+  const uint32_t m0 = SPLIT > 1 ? 0 : wave / S::WN * (BM / S::WM), n0 = SPLIT > 1 ? 0 : wave % S::WN * (BN / S::WN);
+  const uint32_t rest = along - min(along, part * K);
+  Chunk<T>* const ldsM = lds + part * 8 * (BM + BN);
+  Chunk<T>* const ldsN = ldsM + 8 * BM;
+  Loader<T, MACROSS, BM, THREADS, SPLIT> loadM(from + part * K * (MACROSS ? mStride : 1), mStride, rest, m);
+  Loader<T, NACROSS, BN, THREADS, SPLIT> loadN(with + part * K * (NACROSS ? nStride : 1), nStride, rest, n);
+  const auto meet = [] __attribute__((always_inline)) {
+    if constexpr (SPLIT > 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a wavefront's accesses to LDS are in order)
+    else __syncthreads();
+  };
   Acc acc[FM][FN] = {};
-  if (along) {
+  if (rest) {
     loadM.load(0);
     loadN.load(0);
   }
-  constexpr uint32_t K = 128 / sizeof(T);
-  for (uint64_t k = 0; k < along; k += K) {
-    __syncthreads();
-    loadM.store(lds);
+  for (uint64_t k = 0; k < rest; k += K * SPLIT) {
+    meet();
+    loadM.store(ldsM);
     loadN.store(ldsN);
-    __syncthreads();
-    if (k + K < along) {
-      loadM.load((uint32_t)k + K);
-      loadN.load((uint32_t)k + K);
+    meet();
+    if (k + K * SPLIT < rest) {
+      loadM.load((uint32_t)k + K * SPLIT);
+      loadN.load((uint32_t)k + K * SPLIT);
     }
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       Fragments<T, MACROSS, BM, FM> fm;
       Fragments<T, NACROSS, BN, FN> fn;
-      fm.load(lds, m0, s);
+      fm.load(ldsM, m0, s);
       fn.load(ldsN, n0, s);
       Chunk<T> a[FN];
 #pragma unroll
@@ -282,6 +321,11 @@ __device__ __forceinline__ void productTile(const T* from, uint64_t mStride, uin
 #pragma unroll
       for (int i = 0; i < FM; i++) addProducts<NACROSS, T>(a, fm.at(i), acc[i]);
     }
+  }
+  if constexpr (SPLIT > 1) {
+    joinSums<SPLIT>(acc, lds);
+    __syncthreads();  // (the next item's tiles go to the same places)
+    if (wave) return;
   }
   storeResults<T, MACROSS, NACROSS, BM, BN, false>(acc, to, toStride, m0, m, n0, n);
 }
@@ -305,25 +349,26 @@ __device__ __forceinline__ void waitForLds() {
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt alone
   asm volatile("" ::: "memory");
 }
-// It has, and all wavefronts are here.
-__device__ __forceinline__ void meet() {
-  waitForLds();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // All wavefronts of the workgroup.  The operands' parts are below 2^30 bytes each, from the first to the last element.
-template <typename T, bool MACROSS, bool NACROSS, int BM, int BN, int WM, int WN, int R>
+template <typename T, bool MACROSS, bool NACROSS, typename S>
 __device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uint32_t m, const T* with, uint32_t nStride, uint32_t n, uint32_t along, T* to,
-                                            uint64_t toStride, Chunk<T>* lds) {
+                                            uint64_t toStride, Chunk<T>* all) {
+  constexpr int BM = S::BM, BN = S::BN, R = S::R, SPLIT = S::SPLIT, FM = BM / S::WM / 16, FN = BN / S::WN / 16;
   using LM = Tile<T, MACROSS, BM>;
   using LN = Tile<T, NACROSS, BN>;
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr uint32_t WAVES = WM * WN, K = LM::K, PIECES = 8 * (BM + BN);
+  constexpr uint32_t WAVES = S::WM * S::WN, K = LM::K, PIECES = 8 * (BM + BN);
   constexpr uint32_t ALLM = BM / 8, ALL = (BM + BN) / 8, LOADS = (ALL + WAVES - 1) / WAVES;  // a wavefront's load: 64 pieces
   constexpr bool EVEN = ALLM % WAVES == 0 && ALL % WAVES == 0;  // (then it is known which load is of which operand)
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const uint32_t m0 = wave / WN * (BM / WM), n0 = wave % WN * (BN / WN);
+  static_assert(R * LOADS < 64, "as the counter of loads counts");
+  const uint32_t number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t part = SPLIT > 1 ? number : 0, wave = SPLIT > 1 ? 0 : number;  // of SPLIT wavefronts each has a share of the k's, tile by tile, and a ring of its own
+  const uint32_t m0 = wave / S::WN * (BM / S::WM), n0 = wave % S::WN * (BN / S::WN);
+  Chunk<T>* const lds = all + part * R * PIECES;
+  const auto meet = [] __attribute__((always_inline)) {
+    waitForLds();
+    if constexpr (SPLIT == 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
 
   // This wavefront's loads of a tile.
   __amdgpu_buffer_rsrc_t source[LOADS];
@@ -338,9 +383,10 @@ __device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uin
     const bool across = isM ? MACROSS : NACROSS;
     const uint32_t lines = across ? along : isM ? m : n, width = across ? (isM ? m : n) : along;
     source[u] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(isM ? from : with), 0, lines ? ((lines - 1) * stride + width) * (uint32_t)sizeof(T) : 0, 0x00020000);
-    offset[u] = (row * stride + piece * LM::E) * (uint32_t)sizeof(T);
-    kOf[u] = across ? row : piece * LM::E;
-    step[u] = across ? K * stride * (uint32_t)sizeof(T) : 128;
+    const uint32_t tile = across ? K * stride * (uint32_t)sizeof(T) : 128;
+    offset[u] = (row * stride + piece * LM::E) * (uint32_t)sizeof(T) + part * tile;
+    kOf[u] = (across ? row : piece * LM::E) + part * K;
+    step[u] = SPLIT * tile;
     place[u] = q * 64;
   }
   uint32_t asked = 0, slot = 0;  // tiles that have been asked for, and where the next one goes
@@ -350,7 +396,7 @@ __device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uin
 #pragma unroll
     for (int u = 0; u < (int)LOADS; u++) {
       if (u * n / (int)LOADS != i) continue;
-      const uint32_t o = kOf[u] + asked * K < along ? offset[u] : kOutside;
+      const uint32_t o = kOf[u] + asked * (K * SPLIT) < along ? offset[u] : kOutside;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(source[u], (__attribute__((address_space(3))) void*)(ring + place[u]), 16, o, 0, 0, 0);
       offset[u] += step[u];
     }
@@ -361,7 +407,7 @@ __device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uin
   };
 
   Acc acc[FM][FN] = {};
-  const uint32_t tiles = (along + K - 1) / K;
+  const uint32_t tiles = (along + K * SPLIT - 1 - part * K) / (K * SPLIT);
   Fragments<T, MACROSS, BM, FM> fm[2];
   Fragments<T, NACROSS, BN, FN> fn[2];
   const auto read = [&](uint32_t at, int s, int i, int n) __attribute__((always_inline)) {
@@ -403,12 +449,19 @@ __device__ __forceinline__ void productRing(const T* from, uint32_t mStride, uin
   }
   waitForLoads<0>();
   meet();
+  if constexpr (SPLIT > 1) {
+    joinSums<SPLIT>(acc, all);
+    __syncthreads();  // (the next item's loads go to the same places)
+    if (number) return;
+  }
   storeResults<T, MACROSS, NACROSS, BM, BN, MACROSS>(acc, to, toStride, m0, m, n0, n);
 }
 
-// Items for the workgroups in groups of kNear to an XCD, whose L2 they share.
-constexpr uint32_t kNear = 16;
-__device__ __forceinline__ uint64_t itemOf(uint64_t block) { return block / (8 * kNear) * (8 * kNear) + block % 8 * kNear + block / 8 % kNear; }
+// Items for the workgroups in groups of 2^near to an XCD, whose L2 they share.
+constexpr uint32_t kNear = 4;
+__device__ __forceinline__ uint64_t itemOf(uint64_t block, uint32_t near) {
+  return (block >> (near + 3) << (near + 3)) + ((block & 7) << near) + (block >> 3 & ((1u << near) - 1));
+}
 // Which of a group's tiles x strips number `item` is: blocks of kWide strips one after the other, in a block tile by tile, so that items that follow each other share
 // both operands.
 constexpr uint32_t kWide = 8;
@@ -418,12 +471,13 @@ __device__ __forceinline__ void placeOf(uint32_t item, uint32_t tiles, uint32_t 
   strip = block * kWide + in - tile * wide;
 }
 
-template <typename T, bool TRANSPOSED, int BM, int BN, int WM, int WN, int R>
-__global__ __launch_bounds__(WM* WN * 64) void productRingKernel(cuttHipProductArgs a, uint64_t items) {
+template <typename T, bool TRANSPOSED, typename S>
+__global__ __launch_bounds__(S::THREADS) void productRingKernel(cuttHipProductArgs a, uint64_t items, uint32_t near) {
+  constexpr int BM = S::BM, BN = S::BN;
   extern __shared__ __attribute__((aligned(16))) char ringLds[];
   const uint32_t strips = (a.outer + BN - 1) / BN;
   for (uint64_t block = blockIdx.x; block < items; block += gridDim.x) {
-    const uint64_t item = itemOf(block);
+    const uint64_t item = itemOf(block, near);
     Segment s;
     if (!findTile<BM>(a, (uint32_t)(item / strips), s)) continue;
     uint32_t tile, strip;
@@ -431,25 +485,26 @@ __global__ __launch_bounds__(WM* WN * 64) void productRingKernel(cuttHipProductA
     s.first = s.first - ((uint32_t)(item / strips) - s.before) * BM + tile * BM;
     const uint32_t col = strip * BN;
     const T* const w = static_cast<const T*>(a.w) + s.group * a.wGroup;
-    productRing<T, false, !TRANSPOSED, BM, BN, WM, WN, R>(static_cast<const T*>(a.x) + s.first * a.xStride, (uint32_t)a.xStride, min(s.end - s.first, (uint32_t)BM),
+    productRing<T, false, !TRANSPOSED, S>(static_cast<const T*>(a.x) + s.first * a.xStride, (uint32_t)a.xStride, min(s.end - s.first, (uint32_t)BM),
                                                        TRANSPOSED ? w + col * a.wRow : w + col, (uint32_t)a.wRow, min(a.outer - col, (uint32_t)BN), a.inner,
                                                        static_cast<T*>(a.y) + (s.first * a.yStride + col), a.yStride, reinterpret_cast<Chunk<T>*>(ringLds));
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int R>
-__global__ __launch_bounds__(WM* WN * 64) void weightsRingKernel(cuttHipProductArgs a, uint64_t items) {
+template <typename T, typename S>
+__global__ __launch_bounds__(S::THREADS) void weightsRingKernel(cuttHipProductArgs a, uint64_t items, uint32_t near) {
+  constexpr int BM = S::BM, BN = S::BN;
   extern __shared__ __attribute__((aligned(16))) char ringLds[];
   const uint32_t strips = (a.outer + BN - 1) / BN, tiles = (a.inner + BM - 1) / BM;
   for (uint64_t block = blockIdx.x; block < items; block += gridDim.x) {
-    const uint64_t item = itemOf(block);
+    const uint64_t item = itemOf(block, near);
     const uint32_t group = (uint32_t)(item / ((uint64_t)tiles * strips));
     if (group >= a.groups) continue;
     uint32_t tile, strip;
     placeOf((uint32_t)(item - (uint64_t)group * tiles * strips), tiles, strips, tile, strip);
     const uint32_t row = tile * BM, col = strip * BN;
     const uint32_t first = boundOf(a, group), end = max(first, boundOf(a, group + 1));
-    productRing<T, true, true, BM, BN, WM, WN, R>(static_cast<const T*>(a.x) + (first * a.xStride + row), (uint32_t)a.xStride, min(a.inner - row, (uint32_t)BM),
+    productRing<T, true, true, S>(static_cast<const T*>(a.x) + (first * a.xStride + row), (uint32_t)a.xStride, min(a.inner - row, (uint32_t)BM),
                                                static_cast<const T*>(a.w) + (first * a.wRow + col), (uint32_t)a.wRow, min(a.outer - col, (uint32_t)BN), end - first,
                                                static_cast<T*>(a.y) + (group * a.wGroup + row * a.yStride + col), a.yStride, reinterpret_cast<Chunk<T>*>(ringLds));
   }
@@ -457,30 +512,32 @@ __global__ __launch_bounds__(WM* WN * 64) void weightsRingKernel(cuttHipProductA
 
 constexpr uint32_t kMaxBlocks = 1u << 22;
 
-template <typename T, bool TRANSPOSED, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void productKernel(cuttHipProductArgs a, uint64_t items) {
-  __shared__ Chunk<T> lds[8 * (BM + BN)];
+template <typename T, bool TRANSPOSED, typename S>
+__global__ __launch_bounds__(S::THREADS) void productKernel(cuttHipProductArgs a, uint64_t items) {
+  constexpr int BM = S::BM, BN = S::BN;
+  __shared__ Chunk<T> lds[S::SPLIT * 8 * (BM + BN)];
   const uint32_t strips = (uint32_t)(((uint64_t)a.outer + BN - 1) / BN);
   for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
     Segment s;
     if (!findTile<BM>(a, (uint32_t)(item / strips), s)) return;  // (nor are there later ones)
     const uint32_t col = (uint32_t)(item % strips) * BN;
     const T* const w = static_cast<const T*>(a.w) + s.group * a.wGroup;
-    productTile<T, false, !TRANSPOSED, BM, BN, WM, WN>(static_cast<const T*>(a.x) + s.first * a.xStride, a.xStride, min(s.end - s.first, (uint32_t)BM),
+    productTile<T, false, !TRANSPOSED, S>(static_cast<const T*>(a.x) + s.first * a.xStride, a.xStride, min(s.end - s.first, (uint32_t)BM),
                                                        TRANSPOSED ? w + col * a.wRow : w + col, a.wRow, min(a.outer - col, (uint32_t)BN), a.inner,
                                                        static_cast<T*>(a.y) + (s.first * a.yStride + col), a.yStride, lds);
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void weightsKernel(cuttHipProductArgs a, uint64_t items) {
+template <typename T, typename S>
+__global__ __launch_bounds__(S::THREADS) void weightsKernel(cuttHipProductArgs a, uint64_t items) {
+  constexpr int BM = S::BM, BN = S::BN;
   __shared__ Chunk<T> lds[8 * (BM + BN)];
   const uint32_t strips = (uint32_t)(((uint64_t)a.outer + BN - 1) / BN), tiles = (uint32_t)(((uint64_t)a.inner + BM - 1) / BM);
   for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const uint64_t q = item / strips;
     const uint32_t group = (uint32_t)(q / tiles), row = (uint32_t)(q % tiles) * BM, col = (uint32_t)(item % strips) * BN;
     const uint32_t first = boundOf(a, group), end = max(first, boundOf(a, group + 1));
-    productTile<T, true, true, BM, BN, WM, WN>(static_cast<const T*>(a.x) + (first * a.xStride + row), a.xStride, min(a.inner - row, (uint32_t)BM),
+    productTile<T, true, true, S>(static_cast<const T*>(a.x) + (first * a.xStride + row), a.xStride, min(a.inner - row, (uint32_t)BM),
                                                static_cast<const T*>(a.w) + (first * a.wRow + col), a.wRow, min(a.outer - col, (uint32_t)BN), end - first,
                                                static_cast<T*>(a.y) + (group * a.wGroup + row * a.yStride + col), a.yStride, lds);
   }
@@ -495,27 +552,46 @@ bool inReach(const void* p, uint64_t group, uint64_t stride, uint64_t lines, uin
   return ((uintptr_t)p | group * sizeof(T) | stride * sizeof(T) | width * sizeof(T)) % 16 == 0 && stride < (1u << 30) &&
          (lines * stride + width) * sizeof(T) < (1u << 30);
 }
-// (items are handed out kNear to an XCD at a time: whole rounds)
-uint64_t ringItems(uint64_t items) { return parts(items, 8 * kNear) * (8 * kNear); }
+// How many items to an XCD at a time: few enough that all XCDs have some; and what makes whole rounds of these.
+uint32_t nearOf(uint64_t items) {
+  uint32_t near = kNear;
+  while (near && items >> near < 64) near--;
+  return near;
+}
+uint64_t ringItems(uint64_t items) { return parts(items, 8u << nearOf(items)) * (8u << nearOf(items)); }
 uint32_t ringBlocks(uint64_t items) { return (uint32_t)std::min<uint64_t>(ringItems(items), kMaxBlocks); }
 
-constexpr uint32_t kRows32 = 8, kRows64 = 48, kRows64Transposed = 80, kRows128 = 320, kRowsWeights = 512;
+// Tiles of `of` rows that suffice whatever the groups are: whole ones of all rows, and one more for every group that has a row.
+uint64_t tilesOf(const cuttHipProductArgs& a, uint32_t of) { return a.rows / of + std::min(a.rows, a.groups); }
 
-template <int M, int N, int WAVES_M, int WAVES_N, int PLACES>
-struct Shape {
-  static constexpr int BM = M, BN = N, WM = WAVES_M, WN = WAVES_N, R = PLACES, THREADS = WM * WN * 64;
-};
+// Which shape, by what the host knows: how many rows a group has in the mean.  A larger tile reads its operands less often from the caches and feeds more products with each; a group's
+// last tile is a partial one.  Measured with 64 groups of 4096 x 1536 weights, random routing, bfloat16, us (transposed weights in brackets):
+//     rows per group       2          8         16         48         64         80         96        256        320        512
+//     tiles of  32       123 (128)  141 (154)  162 (162)  217 (195)  242 (212)
+//               64       126 (130)  139 (154)  149 (167)  169 (165)  191 (179)  216 (195)  232 (212)
+//              128       152 (159)  160 (183)  165 (192)  177 (194)  180 (192)  186 (191)  191 (194)  319 (311)  388 (371)  550 (525)
+//              256                                                              234 (233)  235 (235)  341 (331)  359 (356)  492 (476)
+// (Up to 8 rows tiles of 32 take as long on the 16-byte grid as those of 64, and off it 175 us instead of 204.  The mean counts the rows that fill segments up, hence 80 and not 72.)
+constexpr uint32_t kRows32 = 8, kRows64 = 48, kRows64Transposed = 80, kRows128 = 288;
+// float, 2048 x 1536: 4 rows 132 with tiles of 16, 144 with 32; 8 rows 153 and 145; 96 rows 417 with tiles of 32, 465 with 64; 256 rows 962 and 927.
+constexpr uint32_t kRows16Float = 4, kRows32Float = 128;
+// The weights' gradient, 64 groups of 2048 x 1536: 256 rows 222 with tiles of 128, 231 with 256; 512 rows 379 and 366; 1024 rows 627 and 614.
+constexpr uint32_t kRowsWeights = 384;
+// Fewer workgroups than these and the chip waits for memory: narrow tiles then, whose k's four wavefronts share.  One token of 8 experts, 4096 x 1536 (96 tiles of 128 columns): 30 -> 24 us
+// (28 -> 21 transposed); 4 experts of 4096 x 1408 (44): 22.7 -> 12.9; one group of 1024 rows of 1024 x 512: 30.9 -> 7.7; 16 experts (192): 42 -> 52, so not there.
+// Off the 16-byte grid, where a wavefront has one tile on its way and not a ring of them: 2047 x 1023, 8 tokens of 8 experts (512) 67 -> 57 (52 -> 44), 16 tokens in float (1024) 122 -> 160.
+constexpr uint32_t kFewRows = 4;
+constexpr uint64_t kFew = 176, kFewUnaligned = 768;
 
 template <typename T, typename S>
 int productAs(const cuttHipProductArgs& a, bool transposed, bool ring, void* stream) {
-  // Tiles that suffice whatever the groups are: whole ones of all rows, and one more for every group that has a row.
-  const uint64_t items = (a.rows / S::BM + std::min(a.rows, a.groups)) * parts(a.outer, S::BN);
+  const uint64_t items = tilesOf(a, S::BM) * parts(a.outer, S::BN);
   if (ring) {
-    auto kernel = transposed ? productRingKernel<T, true, S::BM, S::BN, S::WM, S::WN, S::R> : productRingKernel<T, false, S::BM, S::BN, S::WM, S::WN, S::R>;
-    return launchRows(kernel, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, ringItems(items));
+    auto kernel = transposed ? productRingKernel<T, true, S> : productRingKernel<T, false, S>;
+    return launchRows(kernel, ringBlocks(items), S::THREADS, S::LDS, stream, a, ringItems(items), nearOf(items));
   }
   if constexpr (S::BM <= 128) {
-    auto kernel = transposed ? productKernel<T, true, S::BM, S::BN, S::WM, S::WN> : productKernel<T, false, S::BM, S::BN, S::WM, S::WN>;
+    auto kernel = transposed ? productKernel<T, true, S> : productKernel<T, false, S>;
     return launchRows(kernel, blocksFor(items), S::THREADS, 0, stream, a, items);
   }
   return 0;
@@ -525,33 +601,44 @@ template <typename T>
 int product(const cuttHipProductArgs& a, bool transposed, void* stream) {
   const bool ring = inReach<T>(a.x, 0, a.xStride, 256, a.inner) && (transposed ? inReach<T>(a.w, a.wGroup, a.wRow, 256, a.inner) : inReach<T>(a.w, a.wGroup, a.wRow, a.inner, a.outer));
   const uint32_t rows = a.rows / a.groups;
+  const bool few = tilesOf(a, 32) * parts(a.outer, 128) < (ring ? kFew : kFewUnaligned);
   if constexpr (sizeof(T) == 4) {
-    if (rows <= 4) return productAs<T, Shape<16, 128, 1, 4, 4>>(a, transposed, ring, stream);
-    if (rows <= 64) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
+    if (few && rows <= kFewRows) return productAs<T, Shape<16, 32, 1, 1, 4, 4>>(a, transposed, ring, stream);
+    if (few) return productAs<T, Shape<32, 32, 1, 1, 4, 4>>(a, transposed, ring, stream);
+    if (rows <= kRows16Float) return productAs<T, Shape<16, 128, 1, 4, 4>>(a, transposed, ring, stream);
+    if (rows <= kRows32Float) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
     return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
+  } else {
+    if (few && rows <= kFewRows) return productAs<T, Shape<16, 64, 1, 1, 3, 4>>(a, transposed, ring, stream);
+    if (few) return productAs<T, Shape<32, 64, 1, 1, 3, 4>>(a, transposed, ring, stream);
+    if (rows <= kRows32) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
+    if (rows <= (transposed ? kRows64Transposed : kRows64)) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
+    if (!ring || rows <= kRows128) return productAs<T, Shape<128, 128, 2, 2, 2>>(a, transposed, ring, stream);
+    return productAs<T, Shape<256, 256, 2, 2, 2>>(a, transposed, ring, stream);
   }
-  if (rows <= kRows32) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
-  if (rows <= (transposed ? kRows64Transposed : kRows64)) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
-  if (!ring || rows <= kRows128) return productAs<T, Shape<128, 128, 2, 2, 2>>(a, transposed, ring, stream);
-  return productAs<T, Shape<256, 256, 2, 2, 2>>(a, transposed, ring, stream);
 }
 
+template <typename S>
+uint64_t weightsItems(const cuttHipProductArgs& a) { return parts(a.inner, S::BM) * parts(a.outer, S::BN) * a.groups; }
 template <typename T, typename S>
-int weightsAs(const cuttHipProductArgs& a, bool ring, void* stream) {
-  const uint64_t items = parts(a.inner, S::BM) * parts(a.outer, S::BN) * a.groups;
-  if (ring)
-    return launchRows(weightsRingKernel<T, S::BM, S::BN, S::WM, S::WN, S::R>, ringBlocks(items), S::THREADS, S::R * (S::BM + S::BN) * 128, stream, a, ringItems(items));
-  if constexpr (S::BM <= 128) return launchRows(weightsKernel<T, S::BM, S::BN, S::WM, S::WN>, blocksFor(items), S::THREADS, 0, stream, a, items);
-  return 0;
+int weightsInRings(const cuttHipProductArgs& a, void* stream) {
+  const uint64_t items = weightsItems<S>(a);
+  return launchRows(weightsRingKernel<T, S>, ringBlocks(items), S::THREADS, S::LDS, stream, a, ringItems(items), nearOf(items));
+}
+template <typename T, typename S>
+int weightsAnyhow(const cuttHipProductArgs& a, void* stream) {
+  return launchRows(weightsKernel<T, S>, blocksFor(weightsItems<S>(a)), S::THREADS, 0, stream, a, weightsItems<S>(a));
 }
 
 template <typename T>
 int weights(const cuttHipProductArgs& a, void* stream) {
   const bool ring = inReach<T>(a.x, 0, a.xStride, a.rows, a.inner) && inReach<T>(a.w, 0, a.wRow, a.rows, a.outer);
-  if constexpr (sizeof(T) == 2)
-    if (ring && a.rows / a.groups > kRowsWeights) return weightsAs<T, Shape<256, 256, 2, 2, 2>>(a, ring, stream);
-  if (sizeof(T) == 4 && !ring) return weightsAs<T, Shape<64, 128, 2, 2, 2>>(a, false, stream);
-  return weightsAs<T, Shape<128, 128, 4, 1, 2>>(a, ring, stream);
+  if constexpr (sizeof(T) == 4)
+    // (off the grid 8188 rows, 60 groups, 2050 x 690: 334 us with these, 359 with tiles of 128)
+    return ring ? weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream) : weightsAnyhow<T, Shape<64, 128, 2, 2, 2>>(a, stream);
+  else if (!ring) return weightsAnyhow<T, Shape<128, 128, 4, 1, 2>>(a, stream);
+  else if (a.rows / a.groups <= kRowsWeights) return weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream);
+  else return weightsInRings<T, Shape<256, 256, 2, 2, 2>>(a, stream);
 }
 
 }  // namespace

@@ -204,6 +204,25 @@ def test_neighbours_do_not_leak(dtype):
             assert torch.equal(run_weights(xs[1], ds[1], offsets, torch.zeros_like(wants))[e], wants[e])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("counts,inner,outer", [
+    ([3, 0, 1, 2], 1000, 64), ([1, 0, 0, 1, 0, 2], 1, 40), ([2, 1], 4103, 30),   # few rows: k's shared by wavefronts, fewer tiles of k's than wavefronts
+    ([90, 1, 33], 264, 136), ([300], 640, 200), ([70, 20], 65, 67),
+    ([9] * 40, 136, 520), ([2] * 100, 130, 515),                                 # many groups
+    ([400, 390, 0, 420, 380], 200, 2056), ([130] * 60, 72, 512)])
+def test_shapes(counts, inner, outer, transposed, dtype):
+    """Whole numbers, whose sums are exact: few and many rows to a group, few and many tiles."""
+    g = generator(10)
+    rows, offsets = sum(counts) + 2, offsets_of(counts)
+    x, w = made((rows, inner), dtype, True, g, 2), made((len(counts), outer, inner) if transposed else (len(counts), inner, outer), dtype, True, g, 2)
+    y = torch.full((rows, outer), 7, dtype=dtype, device="cuda")
+    before = np64(y)
+    got = np64(run_product(x, w, offsets, transposed, y))
+    want, _ = oracle.grouped(np64(x), np64(w), offsets.cpu().numpy(), transposed, before)
+    assert np.array_equal(got, np64(torch.from_numpy(want).to(dtype)))
+
+
 def test_offsets_out_of_range():
     """Offsets beyond the rows count as the nearer end, groups whose end is not above their start are empty; a guard behind y stays."""
     g, rows, inner, outer = generator(6), 200, 40, 72
