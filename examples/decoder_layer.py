@@ -1,11 +1,12 @@
-"""A small decoder layer with paged keys and values and routed experts, on the row operators of cutt_rows.h.
+"""A small decoder layer with paged keys and values and routed experts, on the row operators of cutt_rows.h and the products of cutt_products.h.
 
     python examples/decoder_layer.py
 
 Serving: prompts of several requests, then one token each, step by step.  cuttPageTables takes pages for the new tokens and names their
-slots, cuttPageStore puts their keys and values there, cuttPageLoad brings a request's keys and values back head by head, a transpose
-plan turns the keys for the scores, and the tokens go to their experts and back (cuttExpertSort, cuttExpertDispatch,
-cuttExpertCombine).  Training: the same experts with the operators' gradients as autograd functions.  Both are compared with the same layer in
+slots, and cuttPageStore puts their keys and values there.  For a prompt cuttPageLoad brings a request's keys and values back head by head and a transpose
+plan turns the keys for the scores; a step's single tokens look at the pages where they are (cuttAttendPages).  The tokens go to their experts and
+back (cuttExpertSort, cuttExpertDispatch, cuttExpertCombine), and there through the experts' weights (cuttGroupedProduct), no segment's end leaving the device.
+Training: the same experts with the operators' gradients (cuttGroupedProductWeights among them) as autograd functions.  Both are compared with the same layer in
 plain torch operations.
 """
 import math
@@ -134,6 +135,51 @@ class CombineGradients(torch.autograd.Function):
         return drows, dweights, sum(ddout[1:], ddout[0]), None, None, None
 
 
+class Product(torch.autograd.Function):
+    """rows [routing.rows, inner], every segment's times its expert's weights: [experts, inner, outer], or transposed [experts, outer, inner].  What is behind
+    the last segment is not written: no row comes from there."""
+
+    @staticmethod
+    def forward(ctx, rows, weights, routing, transposed):
+        rows, weights = rows.contiguous(), weights.contiguous()
+        ctx.routing, ctx.transposed = routing, transposed
+        ctx.save_for_backward(rows, weights)
+        experts, outer = weights.shape[0], weights.shape[1 if transposed else 2]
+        out = torch.empty(routing.rows, outer, dtype=rows.dtype, device=rows.device)
+        check(cutt.cuttGroupedProduct(routing.rows, experts, rows.shape[1], outer, row_type(rows), transposed, stream(), routing.offsets.data_ptr(),
+                                      rows.data_ptr(), rows.stride(0), weights.data_ptr(), weights.stride()[:2], out.data_ptr(), out.stride(0)),
+              "cuttGroupedProduct")
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        rows, weights = ctx.saved_tensors
+        drows = Product.apply(dout, weights, ctx.routing, not ctx.transposed) if ctx.needs_input_grad[0] else None
+        sides = (dout, rows) if ctx.transposed else (rows, dout)
+        return drows, WeightsGradient.apply(*sides, ctx.routing) if ctx.needs_input_grad[1] else None, None, None
+
+
+class WeightsGradient(torch.autograd.Function):
+    """rows [routing.rows, inner], dout [routing.rows, outer] -> [experts, inner, outer], the sums of a segment's outer products: Product's gradient for its
+    weights, and Product gives its own."""
+
+    @staticmethod
+    def forward(ctx, rows, dout, routing):
+        rows, dout = rows.contiguous(), dout.contiguous()
+        ctx.routing = routing
+        ctx.save_for_backward(rows, dout)
+        dw = torch.empty(routing.counts.numel(), rows.shape[1], dout.shape[1], dtype=rows.dtype, device=rows.device)
+        check(cutt.cuttGroupedProductWeights(routing.rows, dw.shape[0], dw.shape[1], dw.shape[2], row_type(rows), stream(), routing.offsets.data_ptr(),
+                                             rows.data_ptr(), rows.stride(0), dout.data_ptr(), dout.stride(0), dw.data_ptr(), dw.stride()[:2]),
+              "cuttGroupedProductWeights")
+        return dw
+
+    @staticmethod
+    def backward(ctx, g):
+        rows, dout = ctx.saved_tensors
+        return Product.apply(dout, g, ctx.routing, True), Product.apply(rows, g, ctx.routing, False), None
+
+
 class Experts:
     """A router and its experts, each two products with a nonlinearity between."""
 
@@ -154,11 +200,8 @@ class Experts:
     def __call__(self, x):
         ids, weights = self.route(x)
         routing = Routing(ids, self.experts, self.align)
-        rows = Dispatch.apply(x, routing)
-        ends = routing.offsets.tolist()
-        done = [torch.nn.functional.gelu(rows[ends[e]:ends[e + 1]] @ self.up[e]) @ self.down[e] for e in range(self.experts)]
-        done.append(rows[ends[-1]:])  # beyond the last segment: no row comes from there
-        return Combine.apply(torch.cat(done), weights, routing)
+        inside = torch.nn.functional.gelu(Product.apply(Dispatch.apply(x, routing), self.up, routing, False))
+        return Combine.apply(Product.apply(inside, self.down, routing, False), weights, routing)
 
     def plain(self, x):
         ids, weights = self.route(x)
@@ -217,6 +260,19 @@ class PagedCache:
         return k, v
 
 
+    def attend(self, q, owners, positions):
+        """q [tokens, heads, width] of requests `owners` at `positions`, over the pages: [tokens, heads, width]."""
+        tokens, heads, width = q.shape
+        out = torch.empty(tokens, heads, width, device="cuda")
+        space = cutt.cuttAttendPagesWorkspace(tokens, heads, self.heads, width, self.page, self.tables.shape[1], 0)
+        workspace = torch.empty(space, dtype=torch.uint8, device="cuda")
+        check(cutt.cuttAttendPages(tokens, self.tables.shape[0], heads, self.heads, width, cutt.CUTT_F32, self.pages, self.page, self.tables.shape[1], 0,
+                                   1 / math.sqrt(width), stream(), self.tables.data_ptr(), owners.data_ptr(), positions.data_ptr(), q.data_ptr(),
+                                   q.stride()[:2], self.k.data_ptr(), self.v.data_ptr(), self.strides, out.data_ptr(), out.stride()[:2], 0,
+                                   workspace.data_ptr(), space), "cuttAttendPages")
+        return out
+
+
 def turned(k):
     """[heads, length, width] -> [heads, width, length], by a transpose of the library."""
     heads, length, width = k.shape
@@ -249,9 +305,13 @@ class DecoderLayer:
     def step(self, x, cache, added):
         """x [tokens, width]: the new tokens of all requests, `added` of each (a list)."""
         before = cache.lengths.tolist()
-        slots, _ = cache.extend(torch.tensor(added, dtype=torch.int32, device="cuda"), x.shape[0])
+        slots, positions = cache.extend(torch.tensor(added, dtype=torch.int32, device="cuda"), x.shape[0])
         q, k, v = self.project(x)
         cache.store(slots, k, v)
+        if max(added) == 1:
+            owners = torch.tensor([b for b, n in enumerate(added) if n], dtype=torch.int32, device="cuda")
+            x = x + cache.attend(q, owners, positions).reshape(x.shape[0], -1) @ self.out
+            return x + self.experts(x)
         parts, at = [], 0
         for b, n in enumerate(added):
             if n:
