@@ -626,3 +626,92 @@ def test_two_streams_at_once():
     for (_, results, _), want in zip(steps, wants):
         for a, b in zip(results, want):
             assert torch.equal(a, b)
+
+
+def test_a_step_of_all():
+    """Prompts into empty pages, attention over them, and the rows to their experts, through these and back: captured, and replayed with other lengths and choices.
+    Tolerance: a chain of ten operations of up to 512 terms in 32 bits, 10 * 512 * 2^-24 = 3e-4 of the largest value."""
+    g = generator(41)
+    tokens, requests, heads, key_heads, size, page, table, experts, choices, hidden = 60, 7, 6, 2, 32, 8, 9, 8, 3, 96
+    width, kv = heads * size, key_heads * size
+
+    def floats(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+
+    def zeros(*shape, dtype=torch.int32):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+    qkv, up, down = floats(tokens, width + 2 * kv), floats(experts, width, hidden) / width ** 0.5, floats(experts, width, hidden) / hidden ** 0.5
+    added, owners, ids, weights = zeros(requests), zeros(tokens), zeros(tokens, choices, dtype=torch.int64), zeros(tokens, choices, dtype=torch.float32)
+    pages = requests + tokens // page + 1
+    lengths, free, tables = zeros(requests), torch.randperm(pages, generator=g, device="cuda").to(torch.int32), torch.full((requests, table), -1, dtype=torch.int32, device="cuda")
+    starts, used, slots, positions = zeros(requests + 1), zeros(1), zeros(tokens, dtype=torch.int64), zeros(tokens)
+    k, v = floats(pages, page, key_heads, size), floats(pages, page, key_heads, size)
+    mixed, out = zeros(tokens, width, dtype=torch.float32), zeros(tokens, width, dtype=torch.float32)
+    rows = cutt.cuttExpertRows(tokens, choices, experts, 4)
+    counts, offsets, position, source = zeros(experts), zeros(experts + 1), zeros(tokens, choices), zeros(rows)
+    x, inside, y = zeros(rows, width, dtype=torch.float32), zeros(rows, hidden, dtype=torch.float32), zeros(rows, width, dtype=torch.float32)
+    sort_space = cutt.cuttExpertSortWorkspace(tokens, choices, experts)
+    space = cutt.cuttAttendPagesWorkspace(tokens, heads, key_heads, size, page, table, 0)
+    workspace = torch.empty(max(space, sort_space) + 4, dtype=torch.uint8, device="cuda")
+    pitch, cache = qkv.stride(0), k.stride()[:3]
+
+    def step():
+        ok(cutt.cuttPageTables(requests, page, table, pages, tokens, stream(), lengths.data_ptr(), added.data_ptr(), free.data_ptr(), tables.data_ptr(),
+                               starts.data_ptr(), used.data_ptr(), slots.data_ptr(), positions.data_ptr()))
+        ok(cutt.cuttPageStore(tokens, key_heads, size, 4, pages, page, stream(), slots.data_ptr(), qkv[:, width:].data_ptr(), qkv[:, width + kv:].data_ptr(), (pitch, size),
+                              k.data_ptr(), v.data_ptr(), cache))
+        ok(cutt.cuttAttendPages(tokens, requests, heads, key_heads, size, cutt.CUTT_F32, pages, page, table, 0, size ** -0.5, stream(), tables.data_ptr(),
+                                owners.data_ptr(), positions.data_ptr(), qkv.data_ptr(), (pitch, size), k.data_ptr(), v.data_ptr(), cache, mixed.data_ptr(),
+                                (width, size), 0, workspace.data_ptr(), space))
+        ok(cutt.cuttExpertSort(tokens, choices, 0, experts, 4, rows, 8, stream(), ids.data_ptr(), counts.data_ptr(), offsets.data_ptr(), position.data_ptr(),
+                               source.data_ptr(), workspace.data_ptr(), sort_space))
+        ok(cutt.cuttExpertDispatch(tokens, choices, rows, width, 4, stream(), position.data_ptr(), source.data_ptr(), mixed.data_ptr(), width, x.data_ptr(), width))
+        run_product(x, up, offsets, False, inside)
+        inside.tanh_()
+        run_product(inside, down, offsets, True, y)
+        ok(cutt.cuttExpertCombine(tokens, choices, rows, width, cutt.CUTT_F32, stream(), position.data_ptr(), weights.data_ptr(), y.data_ptr(), width, out.data_ptr(),
+                                  width))
+
+    def draw():
+        cuts = torch.sort(torch.randperm(tokens + 1, generator=g, device="cuda")[:requests - 1])[0].tolist()
+        share = [b - a for a, b in zip([0] + cuts, cuts + [tokens])]
+        added.copy_(ints(share))
+        owners.copy_(ints([b for b, n in enumerate(share) for _ in range(n)]))
+        qkv.copy_(floats(*qkv.shape))
+        ids.copy_(torch.topk(floats(tokens, experts), choices, dim=1)[1])
+        weights.copy_(torch.softmax(floats(tokens, choices), dim=1))
+
+    def plain():
+        wide = qkv.double()
+        q, keys, values = wide[:, :width].view(tokens, heads, size), wide[:, width:width + kv].view(tokens, key_heads, size), wide[:, width + kv:].view(tokens, key_heads, size)
+        at = torch.arange(tokens, device="cuda")
+        sees = (owners[:, None] == owners[None]) & (at[None] <= at[:, None])
+        done = []
+        for h in range(heads):
+            score = (q[:, h] @ keys[:, h // (heads // key_heads)].t().contiguous() * size ** -0.5).masked_fill(~sees, float("-inf"))
+            done.append(torch.softmax(score, dim=1) @ values[:, h // (heads // key_heads)].contiguous())
+        one = torch.cat(done, dim=1)
+        two = torch.zeros_like(one)
+        for c in range(choices):
+            for e in range(experts):
+                mine = ids[:, c] == e
+                two[mine] += weights[mine, c, None].double() * (torch.tanh(one[mine] @ up[e].double()) @ down[e].double().t().contiguous())
+        return one, two
+
+    draw()
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(4):
+        draw()
+        step()
+        eager = [mixed.clone(), out.clone()]
+        for got, want in zip(eager, plain()):
+            assert float((got - want).abs().max()) <= 3e-4 * float(want.abs().max())
+        mixed.fill_(7), out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(mixed, eager[0]) and torch.equal(out, eager[1])
