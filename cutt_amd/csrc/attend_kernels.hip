@@ -288,357 +288,356 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
   Range range;
   if (!findRange(p, index, *reinterpret_cast<ScanLds*>(lds), range)) return;
   for (;;) {
+    // Of the range's next queries, the part of their tokens that is in it.
+    const uint32_t queries = range.queries, tokensInAll = range.seen.end - range.seen.first;
+    const bool ends = range.from.query != range.to.query;  // with the queries' last token
+    const bool cut = range.from.from > 0 || !ends;
+    const uint32_t slot = 2 * index + (range.from.from == 0);
+    Seen seen = range.seen;
+    if (!ends) seen.end = seen.first + range.to.from;
+    seen.first += range.from.from;
+    const int32_t* const table = a.tables + (uint64_t)seen.request * a.tableWidth;
 
-  // Of the range's next queries, the part of their tokens that is in it.
-  const uint32_t queries = range.queries, tokensInAll = range.seen.end - range.seen.first;
-  const bool ends = range.from.query != range.to.query;  // with the queries' last token
-  const bool cut = range.from.from > 0 || !ends;
-  const uint32_t slot = 2 * index + (range.from.from == 0);
-  Seen seen = range.seen;
-  if (!ends) seen.end = seen.first + range.to.from;
-  seen.first += range.from.from;
-  const int32_t* const table = a.tables + (uint64_t)seen.request * a.tableWidth;
+    // The pages of a phase's tokens: lane i of wavefront w has token (w + j * kWaves) * 64 + i.
+    constexpr uint32_t PER = kPhase / kThreads;
+    int32_t page[PER];
+    const auto askPages = [&](uint32_t phase) __attribute__((always_inline)) {
+#pragma unroll
+      for (uint32_t j = 0; j < PER; j++) {
+        const uint32_t t = phase + (j * kWaves + wave) * 64 + lane;  // (below 2^32: positions are below 2^31)
+        page[j] = -1;
+        if (t < seen.end) page[j] = table[divide(t, p.byPage)];
+      }
+    };
+    const auto placeTokens = [&](uint32_t phase) __attribute__((always_inline)) {
+#pragma unroll
+      for (uint32_t j = 0; j < PER; j++) {
+        const uint32_t block = j * kWaves + wave, t = phase + block * 64 + lane;
+        const bool is = (uint32_t)page[j] < a.pages;
+        const uint64_t there = __ballot(is);
+        const uint64_t to = is ? (uint64_t)(uint32_t)page[j] * a.pageStride + (t - divide(t, p.byPage) * a.pageSize) * a.slotStride : 0;
+        const uint32_t some = there ? __builtin_ctzll(there) : 0;  // a token that is there stands in for one that is not, whose value counts nothing
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(to >> 32), some) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)to, some);
+        tokens.offset[block * 64 + lane] = is ? to : other;
+        if (lane == 0) tokens.there[block] = there;
+      }
+    };
+    askPages(seen.first);
 
-  // The pages of a phase's tokens: lane i of wavefront w has token (w + j * kWaves) * 64 + i.
-  constexpr uint32_t PER = kPhase / kThreads;
-  int32_t page[PER];
-  const auto askPages = [&](uint32_t phase) __attribute__((always_inline)) {
+    // This lane's column: a head of one of the queries, and what that sees.
+    const uint32_t place = p.most > 1 ? divide(l, p.byHeads) : 0, head = head0 + l - place * nHeads;
+    const bool column = place < queries && l - place * nHeads < nHeads;
+    const uint32_t query = range.from.query + (column ? place : 0);
+    Seen own = range.seen;
+    uint32_t from = own.first, till = own.end;  // what all columns see
+    if (queries > 1) {
+      own = Seen(a, query);
+      from = column ? own.first : 0;
+      till = column ? own.end : 0xffffffffu;
 #pragma unroll
-    for (uint32_t j = 0; j < PER; j++) {
-      const uint32_t t = phase + (j * kWaves + wave) * 64 + lane;  // (below 2^32: positions are below 2^31)
-      page[j] = -1;
-      if (t < seen.end) page[j] = table[divide(t, p.byPage)];
+      for (int i = 1; i < 16; i *= 2) {
+        from = max(from, (uint32_t)__shfl_xor(from, i));
+        till = min(till, (uint32_t)__shfl_xor(till, i));
+      }
+      from = __builtin_amdgcn_readfirstlane(from);
+      till = __builtin_amdgcn_readfirstlane(till);
     }
-  };
-  const auto placeTokens = [&](uint32_t phase) __attribute__((always_inline)) {
+    if (!column) own.first = own.end = 0;
+    Chunk<T> q[STEPS];
+    {
+      const T* const line = static_cast<const T*>(a.q) + query * a.qStride + (column ? head : head0) * a.qHead;
 #pragma unroll
-    for (uint32_t j = 0; j < PER; j++) {
-      const uint32_t block = j * kWaves + wave, t = phase + block * 64 + lane;
-      const bool is = (uint32_t)page[j] < a.pages;
-      const uint64_t there = __ballot(is);
-      const uint64_t to = is ? (uint64_t)(uint32_t)page[j] * a.pageStride + (t - divide(t, p.byPage) * a.pageSize) * a.slotStride : 0;
-      const uint32_t some = there ? __builtin_ctzll(there) : 0;  // a token that is there stands in for one that is not, whose value counts nothing
-      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(to >> 32), some) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)to, some);
-      tokens.offset[block * 64 + lane] = is ? to : other;
-      if (lane == 0) tokens.there[block] = there;
-    }
-  };
-  askPages(seen.first);
-
-  // This lane's column: a head of one of the queries, and what that sees.
-  const uint32_t place = p.most > 1 ? divide(l, p.byHeads) : 0, head = head0 + l - place * nHeads;
-  const bool column = place < queries && l - place * nHeads < nHeads;
-  const uint32_t query = range.from.query + (column ? place : 0);
-  Seen own = range.seen;
-  uint32_t from = own.first, till = own.end;  // what all columns see
-  if (queries > 1) {
-    own = Seen(a, query);
-    from = column ? own.first : 0;
-    till = column ? own.end : 0xffffffffu;
-#pragma unroll
-    for (int i = 1; i < 16; i *= 2) {
-      from = max(from, (uint32_t)__shfl_xor(from, i));
-      till = min(till, (uint32_t)__shfl_xor(till, i));
-    }
-    from = __builtin_amdgcn_readfirstlane(from);
-    till = __builtin_amdgcn_readfirstlane(till);
-  }
-  if (!column) own.first = own.end = 0;
-  Chunk<T> q[STEPS];
-  {
-    const T* const line = static_cast<const T*>(a.q) + query * a.qStride + (column ? head : head0) * a.qHead;
-#pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-      const int d = (s * 4 + quarter) * E;
-      q[s] = loadChunk(line + d, column ? width - d : 0);
-    }
-  }
-  float top = -INFINITY, sum = 0;  // of this lane's column: what scores are taken off from (times log2 e), the exponentials of this quarter's tokens
-  Acc acc[VD] = {};
-
-  // DIRECT: the wavefront's tiles in LDS.
-  Chunk<T>* const keys = reinterpret_cast<Chunk<T>*>(lds + sizeof(PhaseLds) + wave * S::BYTES);
-  Chunk<T>* const values = keys + TILE * S::PIECES;
-  Chunk<T> k[DIRECT ? 1 : SUB][DIRECT ? 1 : STEPS];
-  AlignedVec<T, VE> v[DIRECT ? 1 : VT][VC];
-  const auto toLds = [&](const T* head, Chunk<T>* to, uint32_t tile, auto place) __attribute__((always_inline)) {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // (lgkmcnt: what was in this place has been read)
-#pragma unroll
-    for (int n = 0; n < S::LOADS; n++) {
-      // The lane's place in LDS is fixed; what it loads is the piece that belongs there.
-      const uint32_t row = n * S::ROWS + lane / S::PIECES, at = lane % S::PIECES, piece = place(row, at) - row * S::PIECES;
-      const T* const from = head + (tokens.offset[tile * TILE + row] + piece * E);
-      loadToLds(piece * E < (uint32_t)width ? (const void*)from : (const void*)&kZeros, to + n * 64);
-    }
-    asm volatile("" ::: "memory");
-  };
-  const auto loadKeys = [&](uint32_t tile) __attribute__((always_inline)) {
-    if constexpr (DIRECT) {
-      toLds(kHead, keys, tile, S::keyPlace);
-    } else {
-#pragma unroll
-      for (int i = 0; i < SUB; i++) {
-        const T* const line = kHead + tokens.offset[tile * TILE + i * 16 + l];
-#pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-          const int d = (s * 4 + quarter) * E;
-          k[i][s] = loadChunk(line + d, width - d);
-        }
+      for (int s = 0; s < STEPS; s++) {
+        const int d = (s * 4 + quarter) * E;
+        q[s] = loadChunk(line + d, column ? width - d : 0);
       }
     }
-  };
-  const auto loadValues = [&](uint32_t tile) __attribute__((always_inline)) {
-    if constexpr (DIRECT) {
-      toLds(vHead, values, tile, S::valuePlace);
-    } else {
+    float top = -INFINITY, sum = 0;  // of this lane's column: what scores are taken off from (times log2 e), the exponentials of this quarter's tokens
+    Acc acc[VD] = {};
+
+    // DIRECT: the wavefront's tiles in LDS.
+    Chunk<T>* const keys = reinterpret_cast<Chunk<T>*>(lds + sizeof(PhaseLds) + wave * S::BYTES);
+    Chunk<T>* const values = keys + TILE * S::PIECES;
+    Chunk<T> k[DIRECT ? 1 : SUB][DIRECT ? 1 : STEPS];
+    AlignedVec<T, VE> v[DIRECT ? 1 : VT][VC];
+    const auto toLds = [&](const T* head, Chunk<T>* to, uint32_t tile, auto place) __attribute__((always_inline)) {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // (lgkmcnt: what was in this place has been read)
 #pragma unroll
-      for (int t = 0; t < VT; t++) {
-        const T* const line = vHead + tokens.offset[tile * TILE + t / 4 * 16 + quarter * 4 + t % 4];
+      for (int n = 0; n < S::LOADS; n++) {
+        // The lane's place in LDS is fixed; what it loads is the piece that belongs there.
+        const uint32_t row = n * S::ROWS + lane / S::PIECES, at = lane % S::PIECES, piece = place(row, at) - row * S::PIECES;
+        const T* const from = head + (tokens.offset[tile * TILE + row] + piece * E);
+        loadToLds(piece * E < (uint32_t)width ? (const void*)from : (const void*)&kZeros, to + n * 64);
+      }
+      asm volatile("" ::: "memory");
+    };
+    const auto loadKeys = [&](uint32_t tile) __attribute__((always_inline)) {
+      if constexpr (DIRECT) {
+        toLds(kHead, keys, tile, S::keyPlace);
+      } else {
 #pragma unroll
-        for (int c = 0; c < VC; c++) {
-          const int d = (int)l * VD + c * VE;
-          if (d + VE <= width) {
-            v[t][c] = __builtin_bit_cast(AlignedVec<T, VE>, *reinterpret_cast<const Vec<T, VE>*>(line + d));
-          } else {
-            v[t][c] = {};
+        for (int i = 0; i < SUB; i++) {
+          const T* const line = kHead + tokens.offset[tile * TILE + i * 16 + l];
 #pragma unroll
-            for (int e = 0; e < VE; e++)
-              if (d + e < width) v[t][c][e] = line[d + e];
+          for (int s = 0; s < STEPS; s++) {
+            const int d = (s * 4 + quarter) * E;
+            k[i][s] = loadChunk(line + d, width - d);
           }
         }
       }
-    }
-  };
-  Acc score[SUB];
-  const auto scores = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < SUB; i++) score[i] = Acc(0);
-#pragma unroll
-    for (int s = 0; s < STEPS; s++)
-#pragma unroll
-      for (int i = 0; i < SUB; i++) {
-        if constexpr (DIRECT) score[i] = multiply(keys[S::keyPlace(i * 16 + l, s * 4 + quarter)], q[s], score[i]);
-        else score[i] = multiply(k[i][s], q[s], score[i]);
-      }
-  };
-  // Weighted values added to the sums; with a mask those of the lane's tokens t with bit t of it, for the columns that `mine` says.
-  const auto addWeighted = [&](auto masked, uint32_t mask, bool mine) __attribute__((always_inline)) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int j = 0; j < VD; j += VE) {
-        Acc o[VE];
-#pragma unroll
-        for (int e = 0; e < VE; e++) o[e] = acc[j + e];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          AlignedVec<T, VE> line;
-          if constexpr (DIRECT) line = values[S::valuePlace(quarter * 4 + r, j / 4 * 16 + l)];
-          else line = v[r][j / VE];
-#pragma unroll
-          for (int e = 0; e < VE; e++) o[e] = multiply(!masked || mask >> r & 1 ? line[e] : 0.0f, score[0][r], o[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < VE; e++) acc[j + e] = !masked || mine ? o[e] : acc[j + e];
-      }
-    } else {
-      // Exponentials in two parts, what the type rounds and what it leaves, so that they count with 16 bits and more.  (The matrix unit has the time: with the first
-      // part alone a pass takes as long.)
-      Chunk<T> high, low;
-#pragma unroll
-      for (int t = 0; t < 8; t++) {
-        high[t] = (T)score[t / 4][t % 4];
-        low[t] = (T)(score[t / 4][t % 4] - (float)high[t]);
-      }
-      typedef uint32_t Words __attribute__((ext_vector_type(4)));
-      Words keep;
-      if constexpr (masked)
-#pragma unroll
-        for (int i = 0; i < 4; i++) keep[i] = (mask >> (2 * i) & 1 ? 0xffffu : 0u) | (mask >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
-#pragma unroll
-      for (int j = 0; j < VD; j++) {
-        // Values turned: of eight tokens one element of each, two tokens to a word.
-        Words turned;
-        if constexpr (DIRECT) {
-          // Sixteen lanes load 16 elements of 4 tokens, 8 bytes each, and get one element of the four.
-          typedef short Four __attribute__((ext_vector_type(4)));
-          typedef __attribute__((address_space(3))) Four* Lds;
-          union {
-            Four four[2];
-            Words whole;
-          } u;
-#pragma unroll
-          for (int h = 0; h < 2; h++)
-            u.four[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(reinterpret_cast<char*>(values + S::valuePlace(h * 16 + quarter * 4 + l / 4, j * 2 + (l & 3) / 2)) + (l & 1) * 8));
-          turned = u.whole;
-        } else {
-          typedef uint32_t Piece __attribute__((ext_vector_type(VE / 2)));
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t even = __builtin_bit_cast(Piece, v[2 * i][j / VE])[j % VE / 2], odd = __builtin_bit_cast(Piece, v[2 * i + 1][j / VE])[j % VE / 2];
-            turned[i] = __builtin_amdgcn_perm(odd, even, j % 2 ? 0x07060302 : 0x05040100);
-          }
-        }
-        if constexpr (masked) turned &= keep;
-        const Chunk<T> of = __builtin_bit_cast(Chunk<T>, turned);
-        const Acc o = multiply(of, low, multiply(of, high, acc[j]));
-        acc[j] = !masked || mine ? o : acc[j];
-      }
-    }
-  };
-  // A tile's part of the sums: tokens `first` on; full: all of them have a page.
-  const auto addValues = [&](uint32_t tile, uint32_t first, bool full) __attribute__((always_inline)) {
-    const bool whole = full && first >= from && first + TILE <= till;  // every column sees every token
-    uint32_t mine = 0;  // of the lane's tokens t those that have a page
-#pragma unroll
-    for (int i = 0; i < SUB; i++) score[i] *= scale;
-    if (!whole) {
-      const uint32_t there = (uint32_t)(tokens.there[tile * TILE / 64] >> (tile * TILE % 64));
-#pragma unroll
-      for (int t = 0; t < VT; t++) {
-        const uint32_t at = t / 4 * 16 + quarter * 4 + t % 4;
-        mine |= (there >> at & 1) << t;
-        const bool is = (there >> at & 1) & (first + at >= own.first) & (first + at < own.end);
-        score[t / 4][t % 4] = is ? score[t / 4][t % 4] : -INFINITY;
-      }
-    }
-    float most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < SUB; i++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) most = fmaxf(most, score[i][r]);
-    if (__any(most > top + kSlack)) {
-      most = overQuarters(most, [](float x, float y) { return fmaxf(x, y); });
-      const float next = fmaxf(most, top), less = exp2Of(top - baseOf(next));
-      top = next;
-      sum *= less;
-#pragma unroll
-      for (int j = 0; j < VD; j++) acc[j] *= less;
-    }
-    const float base = baseOf(top);
-#pragma unroll
-    for (int i = 0; i < SUB; i++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        score[i][r] = exp2Of(score[i][r] - base);
-        sum += score[i][r];
-      }
-    if (whole) {
-      addWeighted(Is<false>{}, 0, true);
-    } else {
-      // What a column does not see must not meet its exponential of 0, which an infinity would make NaN: one query after the other takes the values that it sees,
-      // and the columns of the others stay as they were.
-#pragma unroll 1
-      for (uint32_t n = 0; n < queries; n++) {
-        const uint32_t begin = __builtin_amdgcn_readlane(own.first, n * nHeads), end = __builtin_amdgcn_readlane(own.end, n * nHeads);
-        uint32_t with = 0;
+    };
+    const auto loadValues = [&](uint32_t tile) __attribute__((always_inline)) {
+      if constexpr (DIRECT) {
+        toLds(vHead, values, tile, S::valuePlace);
+      } else {
 #pragma unroll
         for (int t = 0; t < VT; t++) {
-          const uint32_t at = first + t / 4 * 16 + quarter * 4 + t % 4;
-          with |= (uint32_t)((at >= begin) & (at < end)) << t;
+          const T* const line = vHead + tokens.offset[tile * TILE + t / 4 * 16 + quarter * 4 + t % 4];
+#pragma unroll
+          for (int c = 0; c < VC; c++) {
+            const int d = (int)l * VD + c * VE;
+            if (d + VE <= width) {
+              v[t][c] = __builtin_bit_cast(AlignedVec<T, VE>, *reinterpret_cast<const Vec<T, VE>*>(line + d));
+            } else {
+              v[t][c] = {};
+#pragma unroll
+              for (int e = 0; e < VE; e++)
+                if (d + e < width) v[t][c][e] = line[d + e];
+            }
+          }
         }
-        addWeighted(Is<true>{}, with & mine, place == n);
       }
-    }
-  };
-
-  for (uint32_t phase = seen.first; phase < seen.end; phase += kPhase) {
-    __syncthreads();
-    placeTokens(phase);
-    __syncthreads();
-    askPages(phase + kPhase);
-    // The wavefront's tiles: every kWaves-th of those that have a token.
-    static_assert(kPhase / TILE <= 64, "a lane for every tile");
-    uint32_t there = 0;
-    if (lane < kPhase / TILE) there = (uint32_t)(tokens.there[lane * TILE / 64] >> (lane * TILE % 64)) & ALL;
-    uint64_t left = __ballot(there != 0) & (0x1111111111111111ull << wave);
-    const uint64_t full = __ballot(there == ALL);
-    if (!left) continue;
-    uint32_t tile = __builtin_ctzll(left);
-    loadKeys(tile);
-    loadValues(tile);
-    // The next tile's keys are asked for as soon as this one's have been used, its values likewise; behind the last tile the same ones again, which nobody waits
-    // for: with a condition around loads to registers the compiler, which counts the loads that it waits for, would have to wait for all.
-    for (;;) {
-      if constexpr (DIRECT) waitForLoads<S::LOADS>();  // (the values' loads may be under way)
-      scores();
-      left &= left - 1;
-      const uint32_t next = left ? __builtin_ctzll(left) : tile;
-      if constexpr (DIRECT) {
-        if (left) {
-          loadKeys(next);
-          waitForLoads<S::LOADS>();
-        } else {
-          waitForLoads<0>();
+    };
+    Acc score[SUB];
+    const auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < SUB; i++) score[i] = Acc(0);
+#pragma unroll
+      for (int s = 0; s < STEPS; s++)
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+          if constexpr (DIRECT) score[i] = multiply(keys[S::keyPlace(i * 16 + l, s * 4 + quarter)], q[s], score[i]);
+          else score[i] = multiply(k[i][s], q[s], score[i]);
+        }
+    };
+    // Weighted values added to the sums; with a mask those of the lane's tokens t with bit t of it, for the columns that `mine` says.
+    const auto addWeighted = [&](auto masked, uint32_t mask, bool mine) __attribute__((always_inline)) {
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < VD; j += VE) {
+          Acc o[VE];
+#pragma unroll
+          for (int e = 0; e < VE; e++) o[e] = acc[j + e];
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            AlignedVec<T, VE> line;
+            if constexpr (DIRECT) line = values[S::valuePlace(quarter * 4 + r, j / 4 * 16 + l)];
+            else line = v[r][j / VE];
+#pragma unroll
+            for (int e = 0; e < VE; e++) o[e] = multiply(!masked || mask >> r & 1 ? line[e] : 0.0f, score[0][r], o[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < VE; e++) acc[j + e] = !masked || mine ? o[e] : acc[j + e];
         }
       } else {
-        loadKeys(next);
+        // Exponentials in two parts, what the type rounds and what it leaves, so that they count with 16 bits and more.  (The matrix unit has the time: with the first
+        // part alone a pass takes as long.)
+        Chunk<T> high, low;
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+          high[t] = (T)score[t / 4][t % 4];
+          low[t] = (T)(score[t / 4][t % 4] - (float)high[t]);
+        }
+        typedef uint32_t Words __attribute__((ext_vector_type(4)));
+        Words keep;
+        if constexpr (masked)
+#pragma unroll
+          for (int i = 0; i < 4; i++) keep[i] = (mask >> (2 * i) & 1 ? 0xffffu : 0u) | (mask >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int j = 0; j < VD; j++) {
+          // Values turned: of eight tokens one element of each, two tokens to a word.
+          Words turned;
+          if constexpr (DIRECT) {
+            // Sixteen lanes load 16 elements of 4 tokens, 8 bytes each, and get one element of the four.
+            typedef short Four __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) Four* Lds;
+            union {
+              Four four[2];
+              Words whole;
+            } u;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+              u.four[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(reinterpret_cast<char*>(values + S::valuePlace(h * 16 + quarter * 4 + l / 4, j * 2 + (l & 3) / 2)) + (l & 1) * 8));
+            turned = u.whole;
+          } else {
+            typedef uint32_t Piece __attribute__((ext_vector_type(VE / 2)));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t even = __builtin_bit_cast(Piece, v[2 * i][j / VE])[j % VE / 2], odd = __builtin_bit_cast(Piece, v[2 * i + 1][j / VE])[j % VE / 2];
+              turned[i] = __builtin_amdgcn_perm(odd, even, j % 2 ? 0x07060302 : 0x05040100);
+            }
+          }
+          if constexpr (masked) turned &= keep;
+          const Chunk<T> of = __builtin_bit_cast(Chunk<T>, turned);
+          const Acc o = multiply(of, low, multiply(of, high, acc[j]));
+          acc[j] = !masked || mine ? o : acc[j];
+        }
       }
-      addValues(tile, phase + tile * TILE, full >> tile & 1);
-      if (!left) break;
-      loadValues(next);
-      tile = next;
-    }
-  }
+    };
+    // A tile's part of the sums: tokens `first` on; full: all of them have a page.
+    const auto addValues = [&](uint32_t tile, uint32_t first, bool full) __attribute__((always_inline)) {
+      const bool whole = full && first >= from && first + TILE <= till;  // every column sees every token
+      uint32_t mine = 0;  // of the lane's tokens t those that have a page
+#pragma unroll
+      for (int i = 0; i < SUB; i++) score[i] *= scale;
+      if (!whole) {
+        const uint32_t there = (uint32_t)(tokens.there[tile * TILE / 64] >> (tile * TILE % 64));
+#pragma unroll
+        for (int t = 0; t < VT; t++) {
+          const uint32_t at = t / 4 * 16 + quarter * 4 + t % 4;
+          mine |= (there >> at & 1) << t;
+          const bool is = (there >> at & 1) & (first + at >= own.first) & (first + at < own.end);
+          score[t / 4][t % 4] = is ? score[t / 4][t % 4] : -INFINITY;
+        }
+      }
+      float most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) most = fmaxf(most, score[i][r]);
+      if (__any(most > top + kSlack)) {
+        most = overQuarters(most, [](float x, float y) { return fmaxf(x, y); });
+        const float next = fmaxf(most, top), less = exp2Of(top - baseOf(next));
+        top = next;
+        sum *= less;
+#pragma unroll
+        for (int j = 0; j < VD; j++) acc[j] *= less;
+      }
+      const float base = baseOf(top);
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          score[i][r] = exp2Of(score[i][r] - base);
+          sum += score[i][r];
+        }
+      if (whole) {
+        addWeighted(Is<false>{}, 0, true);
+      } else {
+        // What a column does not see must not meet its exponential of 0, which an infinity would make NaN: one query after the other takes the values that it sees,
+        // and the columns of the others stay as they were.
+#pragma unroll 1
+        for (uint32_t n = 0; n < queries; n++) {
+          const uint32_t begin = __builtin_amdgcn_readlane(own.first, n * nHeads), end = __builtin_amdgcn_readlane(own.end, n * nHeads);
+          uint32_t with = 0;
+#pragma unroll
+          for (int t = 0; t < VT; t++) {
+            const uint32_t at = first + t / 4 * 16 + quarter * 4 + t % 4;
+            with |= (uint32_t)((at >= begin) & (at < end)) << t;
+          }
+          addWeighted(Is<true>{}, with & mine, place == n);
+        }
+      }
+    };
 
-  // The wavefronts' parts together.
-  sum = overQuarters(sum, [](float x, float y) { return x + y; });
-  __syncthreads();
-  float* const tops = reinterpret_cast<float*>(lds);            // [waves][columns]
-  float* const sums = tops + kWaves * kColumns;
-  float* const parts = sums + kWaves * kColumns;                // [waves][columns][DP + 4]
-  constexpr uint32_t PITCH = DP + 4;
-  if (quarter == 0) {
-    tops[wave * kColumns + l] = top;
-    sums[wave * kColumns + l] = sum;
-  }
-  __syncthreads();
-  float all = -INFINITY;
-#pragma unroll
-  for (uint32_t w = 0; w < kWaves; w++) all = fmaxf(all, tops[w * kColumns + l]);
-  const float mine = exp2Of(top - baseOf(all));
-  if (column)
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-      for (int j = 0; j < VD; j++) parts[(wave * kColumns + l) * PITCH + S::elementOf(j, quarter * 4 + r)] = acc[j][r] * mine;
-  __syncthreads();
-  for (uint32_t c = wave; c < queries * nHeads; c += kWaves) {
-    const uint32_t n = p.most > 1 ? divide(c, p.byHeads) : 0, h = head0 + c - n * nHeads;
-    float m = -INFINITY, of = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; w++) m = fmaxf(m, tops[w * kColumns + c]);
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; w++) of += sums[w * kColumns + c] * exp2Of(tops[w * kColumns + c] - baseOf(m));
-    const bool none = of == 0 && m == -INFINITY;
-    const uint64_t to = range.from.query + n;
-    const uint64_t row = (p.ranges ? (uint64_t)slot * p.most + n : to * p.pieces + (index - range.from.query * p.pieces)) * a.heads + h;
-    for (uint32_t d = lane; d < a.width; d += 64) {
-      float o = 0;
-#pragma unroll
-      for (uint32_t w = 0; w < kWaves; w++) o += parts[(w * kColumns + c) * PITCH + d];
-      if (cut) p.partial[row * a.width + d] = o;
-      else static_cast<T*>(a.out)[to * a.outStride + h * a.outHead + d] = (T)(none ? 0.0f : o / of);
+    for (uint32_t phase = seen.first; phase < seen.end; phase += kPhase) {
+      __syncthreads();
+      placeTokens(phase);
+      __syncthreads();
+      askPages(phase + kPhase);
+      // The wavefront's tiles: every kWaves-th of those that have a token.
+      static_assert(kPhase / TILE <= 64, "a lane for every tile");
+      uint32_t there = 0;
+      if (lane < kPhase / TILE) there = (uint32_t)(tokens.there[lane * TILE / 64] >> (lane * TILE % 64)) & ALL;
+      uint64_t left = __ballot(there != 0) & (0x1111111111111111ull << wave);
+      const uint64_t full = __ballot(there == ALL);
+      if (!left) continue;
+      uint32_t tile = __builtin_ctzll(left);
+      loadKeys(tile);
+      loadValues(tile);
+      // The next tile's keys are asked for as soon as this one's have been used, its values likewise; behind the last tile the same ones again, which nobody waits
+      // for: with a condition around loads to registers the compiler, which counts the loads that it waits for, would have to wait for all.
+      for (;;) {
+        if constexpr (DIRECT) waitForLoads<S::LOADS>();  // (the values' loads may be under way)
+        scores();
+        left &= left - 1;
+        const uint32_t next = left ? __builtin_ctzll(left) : tile;
+        if constexpr (DIRECT) {
+          if (left) {
+            loadKeys(next);
+            waitForLoads<S::LOADS>();
+          } else {
+            waitForLoads<0>();
+          }
+        } else {
+          loadKeys(next);
+        }
+        addValues(tile, phase + tile * TILE, full >> tile & 1);
+        if (!left) break;
+        loadValues(next);
+        tile = next;
+      }
     }
-    if (lane == 0) {
-      if (cut) {
-        p.tops[row * 2] = m;
-        p.tops[row * 2 + 1] = of;
-      } else if (a.logSums) a.logSums[to * a.heads + h] = none ? -INFINITY : (m + __log2f(of)) * kLn2;
-    }
-  }
 
-  if ((p.ranges || p.pieces > 1) && range.from.from == 0 && share == 0 && threadIdx.x < queries) {
-    uint32_t* const to = p.cuts + (range.from.query + threadIdx.x) * 4;
-    to[0] = index;
-    to[1] = ends ? 1 : p.each || !p.ranges ? (uint32_t)range.before : (uint32_t)((range.before + cutsEnd(tokensInAll) + range.length - 1) / range.length) - index;
-    to[2] = threadIdx.x;
-  }
-  range.from = {range.from.query + queries, 0};
-  if (!ends || range.from.query >= a.queries || (range.from.query == range.to.query && range.to.from == 0)) break;
-  range.before += tokensInAll + kExtra;
-  range.queries = together(p, range.from.query, range.seen);
-  __syncthreads();  // (the next query's tokens take the place of what has been joined)
+    // The wavefronts' parts together.
+    sum = overQuarters(sum, [](float x, float y) { return x + y; });
+    __syncthreads();
+    float* const tops = reinterpret_cast<float*>(lds);            // [waves][columns]
+    float* const sums = tops + kWaves * kColumns;
+    float* const parts = sums + kWaves * kColumns;                // [waves][columns][DP + 4]
+    constexpr uint32_t PITCH = DP + 4;
+    if (quarter == 0) {
+      tops[wave * kColumns + l] = top;
+      sums[wave * kColumns + l] = sum;
+    }
+    __syncthreads();
+    float all = -INFINITY;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; w++) all = fmaxf(all, tops[w * kColumns + l]);
+    const float mine = exp2Of(top - baseOf(all));
+    if (column)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int j = 0; j < VD; j++) parts[(wave * kColumns + l) * PITCH + S::elementOf(j, quarter * 4 + r)] = acc[j][r] * mine;
+    __syncthreads();
+    for (uint32_t c = wave; c < queries * nHeads; c += kWaves) {
+      const uint32_t n = p.most > 1 ? divide(c, p.byHeads) : 0, h = head0 + c - n * nHeads;
+      float m = -INFINITY, of = 0;
+#pragma unroll
+      for (uint32_t w = 0; w < kWaves; w++) m = fmaxf(m, tops[w * kColumns + c]);
+#pragma unroll
+      for (uint32_t w = 0; w < kWaves; w++) of += sums[w * kColumns + c] * exp2Of(tops[w * kColumns + c] - baseOf(m));
+      const bool none = of == 0 && m == -INFINITY;
+      const uint64_t to = range.from.query + n;
+      const uint64_t row = (p.ranges ? (uint64_t)slot * p.most + n : to * p.pieces + (index - range.from.query * p.pieces)) * a.heads + h;
+      for (uint32_t d = lane; d < a.width; d += 64) {
+        float o = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) o += parts[(w * kColumns + c) * PITCH + d];
+        if (cut) p.partial[row * a.width + d] = o;
+        else static_cast<T*>(a.out)[to * a.outStride + h * a.outHead + d] = (T)(none ? 0.0f : o / of);
+      }
+      if (lane == 0) {
+        if (cut) {
+          p.tops[row * 2] = m;
+          p.tops[row * 2 + 1] = of;
+        } else if (a.logSums) a.logSums[to * a.heads + h] = none ? -INFINITY : (m + __log2f(of)) * kLn2;
+      }
+    }
+
+    if ((p.ranges || p.pieces > 1) && range.from.from == 0 && share == 0 && threadIdx.x < queries) {
+      uint32_t* const to = p.cuts + (range.from.query + threadIdx.x) * 4;
+      to[0] = index;
+      to[1] = ends ? 1 : p.each || !p.ranges ? (uint32_t)range.before : (uint32_t)((range.before + cutsEnd(tokensInAll) + range.length - 1) / range.length) - index;
+      to[2] = threadIdx.x;
+    }
+    range.from = {range.from.query + queries, 0};
+    if (!ends || range.from.query >= a.queries || (range.from.query == range.to.query && range.to.from == 0)) break;
+    range.before += tokensInAll + kExtra;
+    range.queries = together(p, range.from.query, range.seen);
+    __syncthreads();  // (the next query's tokens take the place of what has been joined)
   }
 }
 
