@@ -8,7 +8,7 @@ benchmarks written in Python.
 from .api import (  # noqa: F401
     CUTT_SUCCESS, CUTT_INVALID_PLAN, CUTT_INVALID_PARAMETER, CUTT_INVALID_DEVICE,
     CUTT_INTERNAL_ERROR, CUTT_UNDEFINED_ERROR,
-    CUTT_F32, CUTT_F16, CUTT_BF16, CUTT_MAX_EXPERTS, CUTT_MAX_HEAD_WIDTH,
+    CUTT_F32, CUTT_F16, CUTT_BF16, CUTT_MAX_EXPERTS, CUTT_MAX_HEAD_WIDTH, CUTT_MAX_HEADS,
     METHOD_NAMES, METHOD_TRIVIAL, METHOD_PACKED, METHOD_PACKEDSPLIT, METHOD_TILED, METHOD_TILEDCOPY,
     CuttError, PlanInfo, StreamCounts, lib, lib_path,
     cuttPlan, cuttPlanMeasure, cuttPlanFromCandidate, cuttExecute, cuttExecuteNoAlloc, cuttDestroy,

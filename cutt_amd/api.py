@@ -30,6 +30,7 @@ METHOD_NAMES = {0: "Unknown", 1: "Trivial", 2: "Packed", 3: "PackedSplit", 4: "T
 CUTT_F32, CUTT_F16, CUTT_BF16 = 0, 1, 2
 CUTT_MAX_EXPERTS = 1024
 CUTT_MAX_HEAD_WIDTH = 256
+CUTT_MAX_HEADS = 65536
 
 
 class CuttError(RuntimeError):

@@ -1,5 +1,13 @@
 /*
  * attend_kernels.hip - attention of new tokens' queries over keys and values in pages (cutt_products.h).
+ *
+ * With s_t = scale q.k_t, what is wanted is sum exp(s_t) v_t / sum exp(s_t) over the tokens t that a query sees.  It is had in one pass: scores are taken off from a number `top` near
+ * the largest so far, and what has been summed is scaled when that is raised.  Parts of a query's tokens, each with its `top`, are joined by the same scaling, first a workgroup's four
+ * wavefronts', then, in a second launch, those of the workgroups that share the query.  All of this is in 32 bits; only the products' operands have 16 where the type has.
+ *
+ * Every cached element is read once, and takes two operations for each of the query heads that share it: memory bounds it, and where there is little of it the chain
+ * offsets -> page -> keys -> scores -> values -> joined parts.  64 requests of up to 8192 tokens, 32 heads on 8 key heads of 128 bfloat16 (1075 MB): 194 us, 5.5 TB/s, where a pure
+ * read of as much reaches 6.2 (6.9 past the caches); 256 requests of 2048 each: 338 us, 6.4 TB/s; one request of 128 tokens: 7.3 us.
  */
 #include <algorithm>
 
@@ -18,19 +26,17 @@ constexpr uint32_t kColumns = 16;  // of the matrix instructions: query heads of
 constexpr uint32_t kPhase = 1024;  // tokens whose addresses a workgroup works out at a time
 constexpr uint32_t kScan = 2048;   // queries that are shared out evenly, at most
 constexpr uint32_t kCut = 128;     // queries are cut at multiples of this many tokens: a tile for every wavefront
-constexpr uint32_t kExtra = 128;   // tokens in whose time a workgroup begins a query and ends it
+constexpr uint32_t kExtra = 128;   // tokens in whose time a workgroup begins a query and ends it (with 320 the 24 drafting requests take 67 us and not 62)
 
 // How the work is shared out.  The tokens that the queries see, with kExtra more for each, lie one behind the other, and are cut into ranges of even lengths, one for each
 // workgroup (of a key head's).  The cuts move to where a query begins or a little further in it, so that a range may take the end of one query's tokens, some whole
-// queries and the begin of another.  Where there are many more workgroups than queries, each query has ranges of its own instead, and no workgroup has two to begin.
-// Where there are many queries none looks at the others: each is a range, or a few of a length that is known before.
+// queries and the begin of another.  Where there are many queries none looks at the others: each is a range, or a few of a length that is known before.
 struct Attend {
   cuttHipAttendArgs a;
   uint32_t group, headTiles;  // query heads per key head, and workgroups that share them
   uint32_t most;              // neighbouring queries of one request that a workgroup takes together, a power of two: their heads share its columns
   uint32_t ranges;            // 0: each query has `pieces` of its own, of `length` tokens (the last one what is left)
   uint32_t pieces, length;
-  uint32_t each;              // each query is cut into ranges of its own
   float perRange;             // what length of a range, by all tokens, makes no more than `ranges`
   cuttHipDivisor byPage, byTiles, byHeads, byShares;  // divisions by pageSize, headTiles, the heads in a column tile and all workgroups of a range
   float* partial;             // [2 * ranges][most][heads][width]: of what begins within a query, and of what ends in one; or [queries][pieces][heads][width]
@@ -77,11 +83,11 @@ struct Cut {
 };
 
 struct ScanLds {
-  uint32_t low[kWaves], high[kWaves], pieces[kWaves];
+  uint32_t low[kWaves], high[kWaves];
   Cut cut[2];
   Seen seen;          // what the range's first queries see, and how many they are
   uint32_t queries;   // (0: they are the ones behind those that the cut was in)
-  uint64_t before;    // tokens before them; where each query is cut by itself, its ranges
+  uint64_t before;    // tokens before them
 };
 
 __device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y) { return x + y; }
@@ -127,7 +133,7 @@ __device__ __forceinline__ bool findRange(const Attend& p, uint32_t index, ScanL
     queries = 0;
     if (follows(p, i)) continue;
     queries = together(p, i, seen);
-    const uint32_t n = seen.end - seen.first + (p.each ? 0 : kExtra);
+    const uint32_t n = seen.end - seen.first + kExtra;
     low += n & 0xffff;
     high += n >> 16;
   }
@@ -145,29 +151,10 @@ __device__ __forceinline__ bool findRange(const Attend& p, uint32_t index, ScanL
     all += n;
     if (w < wave) before += n;
   }
-  if (p.each) {
-    // Each query by itself in pieces of even lengths.  (Its tokens and the rounding to whole pieces: no more than p.ranges are needed.)
-    const uint32_t tokens = queries ? seen.end - seen.first : 0;
-    r.length = min(((uint64_t)((float)all * p.perRange) + kCut) / kCut * kCut, (uint64_t)1 << 31);
-    const uint32_t length = (uint32_t)r.length, pieces = queries ? max((tokens + length - 1) / length, 1u) : 0;
-    const uint32_t upTo = scanOverWave(pieces, plus);
-    if (lane == 63) s.pieces[wave] = upTo;
-    __syncthreads();
-    uint32_t at = upTo - pieces;
-    for (uint32_t w = 0; w < wave; w++) at += s.pieces[w];
-    if (index >= at && index < at + pieces) {
-      const uint32_t piece = index - at;
-      s.cut[0] = {from, piece * length};
-      s.cut[1] = {piece + 1 < pieces ? from : from + queries, piece + 1 < pieces ? (piece + 1) * length : 0};
-      s.seen = seen;
-      s.queries = queries;
-      s.before = pieces;
-    }
-  }
-  r.length = p.each ? r.length : max((uint64_t)((float)all * p.perRange) + 1, (uint64_t)kCut);  // (two cuts do not move to the same place within a query)
+  r.length = max((uint64_t)((float)all * p.perRange) + 1, (uint64_t)kCut);  // (two cuts do not move to the same place within a query)
   const uint64_t begin = index * r.length, end = begin + r.length;
 #pragma unroll 1
-  for (uint32_t i = p.each ? to : from; i < to; i++) {
+  for (uint32_t i = from; i < to; i++) {
     if (i != from) {
       if (follows(p, i)) continue;
       queries = together(p, i, seen);
@@ -208,8 +195,12 @@ __device__ __forceinline__ bool findRange(const Attend& p, uint32_t index, ScanL
 // The tokens' scores and their weighted values, a tile of tokens at a time: keys times queries give the scores, heads along the instruction's columns, and each lane
 // then holds the exponentials of its head's tokens just as the second product, values turned times exponentials, wants them.
 //
+// Keys and values are the instructions' A operands, 16 tokens or 16 elements, queries and exponentials their B operands: up to 16 heads that share the keys, so that few heads leave columns idle
+// but no more is read, and no product waits for another wavefront.
+//
 // DIRECT: a wavefront's tiles go from memory to its own part of LDS, token by token, 16-byte pieces of a row exchanged so that a fragment's lanes find theirs in different banks.  Else (rows
-// off the 16-byte grid) they go to registers, keys as the fragments want them and of a token's values VD neighbouring elements to each lane.
+// off the 16-byte grid) they go to registers, keys as the fragments want them and of a token's values VD neighbouring elements to each lane.  So much as is on its way to registers has to
+// have its registers: with aligned rows too the 64 requests above take 229 us this way, not 194, 72 queries of 80 floats 83 and not 50.
 template <typename T, int DP, bool DIRECT>
 struct Tokens {
   static constexpr int E = kPer16<T>;
@@ -630,7 +621,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
     if ((p.ranges || p.pieces > 1) && range.from.from == 0 && share == 0 && threadIdx.x < queries) {
       uint32_t* const to = p.cuts + (range.from.query + threadIdx.x) * 4;
       to[0] = index;
-      to[1] = ends ? 1 : p.each || !p.ranges ? (uint32_t)range.before : (uint32_t)((range.before + cutsEnd(tokensInAll) + range.length - 1) / range.length) - index;
+      to[1] = ends ? 1 : !p.ranges ? (uint32_t)range.before : (uint32_t)((range.before + cutsEnd(tokensInAll) + range.length - 1) / range.length) - index;
       to[2] = threadIdx.x;
     }
     range.from = {range.from.query + queries, 0};
@@ -713,6 +704,10 @@ __global__ __launch_bounds__(kThreads) void joinKernel(Attend p) {
 
 constexpr uint32_t kMaxBlocks = 1u << 22;
 
+// Queries are cut by themselves if they are enough for all CUs even when kColumns / group of them are taken together (256 requests of 2048 tokens, 8 key heads: 338 us, with even ranges
+// 360; of up to 256 tokens 48 and 53; but 24 requests of three drafted tokens, 12 heads: 104 and 50), or have so few tokens that a part of them is no less time (8 requests, 8 key heads:
+// 256 tokens 9.9 and 12.9 us, 512 tokens 14.3 and 13.3).  Their pieces are long, so that what a workgroup does before and after its tokens (5 us) is little of its time (16 pieces of 1024
+// tokens at least: the 338 become 370), and there are no more than kPieceBlocks workgroups, which also bounds the workspace.
 constexpr uint32_t kManyBlocks = 256, kShort = 256, kPieces = 8, kLeastPiece = 2048, kPieceBlocks = 16384;
 
 Attend planAttend(uint32_t queries, uint32_t heads, uint32_t keyHeads, uint32_t width, uint32_t pageSize, uint32_t tableWidth, uint32_t window) {
@@ -731,11 +726,9 @@ Attend planAttend(uint32_t queries, uint32_t heads, uint32_t keyHeads, uint32_t 
     p.length = (uint32_t)((reach + p.pieces * kCut - 1) / (p.pieces * kCut) * kCut);
     return p;
   }
-  // As many workgroups as run at a time.
+  // As many workgroups as run at a time: two to a CU, which LDS and registers allow, three of narrow heads, one of wide ones.  (Half as many: the 64 requests above 250 us, twice as many 207.)
   p.ranges = std::max(1u, (width <= 64 ? 768 : width <= 128 ? 512 : 256) / (uint32_t)shares);
-  // (each query's last range may be a short one; and there are kThreads queries at most, one for each thread that looks)
-  p.each = queries <= kThreads && queries * 4 <= p.ranges;
-  p.perRange = p.ranges ? 1.0001f / (p.each ? p.ranges - queries : p.ranges) : 0.0f;
+  p.perRange = 1.0001f / p.ranges;
   return p;
 }
 
@@ -762,6 +755,7 @@ int attendWide(const Attend& p, void* stream) {
   return p.a.width <= 64 ? attend<T, 64, DIRECT>(p, stream) : p.a.width <= 128 ? attend<T, 128, DIRECT>(p, stream) : attend<T, 256, DIRECT>(p, stream);
 }
 
+// (what both ways cost is said where Tokens is)
 template <typename T>
 int attendType(const Attend& p, void* stream) {
   const cuttHipAttendArgs& a = p.a;

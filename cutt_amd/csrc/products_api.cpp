@@ -19,7 +19,7 @@ bool productSizes(int rows, int groups, int inner, int outer) {
 uint64_t strideOf(long long stride, int n) { return n > 1 ? (uint64_t)stride : 0; }
 
 bool attendSizes(int queries, int heads, int keyHeads, int width, int pageSize, int tableWidth, int window) {
-  return queries >= 0 && heads >= 1 && keyHeads >= 1 && heads % keyHeads == 0 && (long long)queries * heads <= INT_MAX && width >= 1 &&
+  return queries >= 0 && heads >= 1 && heads <= CUTT_MAX_HEADS && keyHeads >= 1 && heads % keyHeads == 0 && (long long)queries * heads <= INT_MAX && width >= 1 &&
          width <= CUTT_MAX_HEAD_WIDTH && pageSize >= 1 && tableWidth >= 1 && window >= 0;
 }
 

@@ -59,6 +59,7 @@ cuttResult cuttGroupedProductWeights(int rows, int groups, int inner, int outer,
 /* ---- attention over pages ---------------------------------------------------- */
 
 #define CUTT_MAX_HEAD_WIDTH 256
+#define CUTT_MAX_HEADS 65536
 
 /* Bytes of workspace that cuttAttendPages needs for these sizes (0: none, or arguments out of range). */
 size_t cuttAttendPagesWorkspace(int queries, int heads, int keyHeads, int width, int pageSize, int tableWidth, int window);
@@ -74,7 +75,8 @@ size_t cuttAttendPagesWorkspace(int queries, int heads, int keyHeads, int width,
  * A query that sees nothing (a position below 0, an owner not in 0 .. requests - 1), or whose scores are all -infinity, gets zeros, and -infinity.  Keys and
  * values that are not seen have no part in it, whatever they hold.
  *
- *   queries, requests, pages >= 0, heads a multiple of keyHeads >= 1, 1 <= width <= CUTT_MAX_HEAD_WIDTH, pageSize, tableWidth >= 1, scale finite
+ *   queries, requests, pages >= 0, keyHeads >= 1, heads <= CUTT_MAX_HEADS a multiple of it, queries * heads < 2^31
+ *   1 <= width <= CUTT_MAX_HEAD_WIDTH, pageSize, tableWidth >= 1, scale finite
  *   window            tokens that a query sees at most, itself among them; 0: all
  *   tables            [requests, tableWidth]
  *   owners            [queries], or NULL: query i belongs to request i

@@ -25,6 +25,7 @@ def test_every_declared_function_is_exported_and_bound(cutt):
     lib = ctypes.CDLL(cutt.lib_path())
     for n in names:
         assert hasattr(lib, n) and callable(getattr(cutt, n)), n
+    assert cutt.CUTT_MAX_HEADS == 65536 and re.search(r"CUTT_MAX_HEADS\s+65536", text)
     assert cutt.CUTT_MAX_HEAD_WIDTH == 256 and re.search(r"CUTT_MAX_HEAD_WIDTH\s+256", text)
 
 
@@ -66,7 +67,8 @@ def test_weights_refuse(cutt, change):
                                     dict(tables=0), dict(tables=A + 2), dict(owners=I + 1), dict(positions=0), dict(positions=B + 2), dict(q=0), dict(q=C + 1), dict(qs=None),
                                     dict(qs=(-128, 16)), dict(k=0), dict(v=0), dict(v=E + 1), dict(cs=None), dict(cs=(512, -32, 16)), dict(out=0), dict(out=F + 1),
                                     dict(os=None), dict(os=(128, 15)), dict(os=(127, 16)), dict(logs=G + 2), dict(out=C), dict(out=D + 64), dict(out=E), dict(logs=A),
-                                    dict(logs=F), dict(logs=B), dict(out=A), dict(owners=F), dict(queries=2 ** 30), dict(cs=(2 ** 62, 32, 16))])
+                                    dict(logs=F), dict(logs=B), dict(out=A), dict(owners=F), dict(queries=2 ** 30), dict(cs=(2 ** 62, 32, 16)),
+                                    dict(heads=65538, os=(2 ** 21, 16), qs=(2 ** 21, 16))])
 def test_attend_refuses(cutt, change):
     assert cutt.cuttAttendPages(*{**ATTEND, **change}.values()) == BAD
 
@@ -80,7 +82,7 @@ def test_strides_are_as_many_as_axes(cutt):
 
 def test_workspace_of_sizes_out_of_range(cutt):
     for bad in ((-1, 8, 2, 16, 16, 8, 0), (4, 8, 3, 16, 16, 8, 0), (4, 8, 2, 257, 16, 8, 0), (4, 8, 2, 16, 0, 8, 0), (4, 8, 2, 16, 16, 0, 0), (4, 8, 2, 16, 16, 8, -1),
-                (2 ** 31, 8, 2, 16, 16, 8, 0)):
+                (2 ** 31, 8, 2, 16, 16, 8, 0), (4, 65538, 2, 16, 16, 8, 0)):
         assert cutt.cuttAttendPagesWorkspace(*bad) == 0
 
 
