@@ -633,8 +633,8 @@ template <typename T>
 int weights(const cuttHipProductArgs& a, void* stream) {
   const bool ring = inReach<T>(a.x, 0, a.xStride, a.rows, a.inner) && inReach<T>(a.w, 0, a.wRow, a.rows, a.outer);
   if constexpr (sizeof(T) == 4)
-    // (off the grid 8188 rows, 60 groups, 2050 x 690: 334 us with these, 359 with tiles of 128)
-    return ring ? weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream) : weightsAnyhow<T, Shape<64, 128, 2, 2, 2>>(a, stream);
+    // (off the grid 8188 rows, 60 groups, 2050 x 690: 308 us with these, 334 with tiles of 64 x 128, 359 with 128 x 128)
+    return ring ? weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream) : weightsAnyhow<T, Shape<64, 64, 4, 1, 2>>(a, stream);
   else if (!ring) return weightsAnyhow<T, Shape<128, 128, 4, 1, 2>>(a, stream);
   else if (a.rows / a.groups <= kRowsWeights) return weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream);
   else return weightsInRings<T, Shape<256, 256, 2, 2, 2>>(a, stream);
