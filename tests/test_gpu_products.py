@@ -261,6 +261,18 @@ def test_no_rows():
     assert bool((dw == 0).all())
 
 
+@pytest.mark.parametrize("outer", [2 ** 28, 2 ** 28 + 1])
+def test_more_tiles_than_workgroups(outer):
+    """Results of 13 GB, in more tiles than a launch has workgroups; single products, which are exact in 32 bits and rounded once."""
+    g = generator(9)
+    x, dy = made((3, 8), torch.bfloat16, True, g), made((3, outer), torch.bfloat16, True, g)
+    dw = torch.full((3, 8, outer), 7, dtype=torch.bfloat16, device="cuda")
+    run_weights(x, dy, offsets_of([1, 1, 1]), dw)
+    for e in range(3):
+        for i in range(8):
+            assert torch.equal(dw[e, i], x[e, i] * dy[e])
+
+
 def test_small_numbers():
     """Halves below the normal range count in full: products are exact."""
     x = torch.full((3, 64), 2.0 ** -24, dtype=torch.float16, device="cuda")
