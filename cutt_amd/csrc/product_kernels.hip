@@ -575,8 +575,16 @@ uint64_t tilesOf(const cuttHipProductArgs& a, uint32_t of) { return a.rows / of 
 constexpr uint32_t kRows32 = 8, kRows64 = 48, kRows64Transposed = 80, kRows128 = 288;
 // float, 2048 x 1536: 4 rows 132 with tiles of 16, 144 with 32; 8 rows 153 and 145; 96 rows 417 with tiles of 32, 465 with 64; 256 rows 962 and 927.
 constexpr uint32_t kRows16Float = 4, kRows32Float = 128;
-// The weights' gradient, 64 groups of 2048 x 1536: 256 rows 222 with tiles of 128, 231 with 256; 512 rows 379 and 366; 1024 rows 627 and 614.
+// Large tiles need many of them besides, or CUs have none: bfloat16, 8 groups of 512 rows, 1024 x 1024 (96 tiles of 256, 320 of 128) 32.6 us with 256, 20.7 with 128, 28.3 with 64; 8 groups of 328 rows, 320 x 448
+// 18.8, 8.6 and 6.4; but 64 groups of 512 rows, 1024 x 1024 (768 of 256) 111, 117, 135.
+constexpr uint64_t kFew128 = 256, kFew256 = 700;
+// The weights' gradient, 64 groups of 2048 x 1536: 256 rows 222 with tiles of 128, 231 with 256; 512 rows 379 and 366; 1024 rows 627 and 614; (tiles of 128 by 4 x 1 wavefronts: 3 % less than by 2 x 2).
 constexpr uint32_t kRowsWeights = 384;
+// Each of its tiles goes over all of a group's rows, so that with few the longest group is all there is to wait for.  By tiles of 128 x 128, 1024 rows to a group, bfloat16, us with tiles of 64, 128, 256:
+//     64 12.0, 20.0, 41.6;   256 37, 45, 95;   512 57, 50, 96;   1024 104, 67, 97;   4096 -, 234, 240;   8192 -, 433, 430
+// float 64 28, 81 (with 128);   256 115, 204;   512 177, 254;   1024 341, 383;   708 tiles, groups of very unequal lengths 239, 531.  Off the 16-byte grid, bfloat16, 512: 66 with 64, 86 with 128;
+// 2898: 477, 264; there 64 x 64 by 2 x 2 wavefronts where tiles are few (512 of float 200, 226 with 4 x 1), 4 x 1 where they are many (308 and 328 for 8188 rows, 60 groups, 2050 x 690).
+constexpr uint64_t kFewWeights = 384, kFewWeightsUnaligned = 768, kFewWeightsFloat = 1536, kManyWeights = 6144;
 // Fewer workgroups than these and the chip waits for memory: narrow tiles then, whose k's four wavefronts share.  One token of 8 experts, 4096 x 1536 (96 tiles of 128 columns): 30 -> 24 us
 // (28 -> 21 transposed); 4 experts of 4096 x 1408 (44): 22.7 -> 12.9; one group of 1024 rows of 1024 x 512: 30.9 -> 7.7; 16 experts (192): 42 -> 52, so not there.
 // Off the 16-byte grid, where a wavefront has one tile on its way and not a ring of them: 2047 x 1023, 8 tokens of 8 experts (512) 67 -> 57 (52 -> 44), 16 tokens in float (1024) 122 -> 160.
@@ -601,7 +609,8 @@ template <typename T>
 int product(const cuttHipProductArgs& a, bool transposed, void* stream) {
   const bool ring = inReach<T>(a.x, 0, a.xStride, 256, a.inner) && (transposed ? inReach<T>(a.w, a.wGroup, a.wRow, 256, a.inner) : inReach<T>(a.w, a.wGroup, a.wRow, a.inner, a.outer));
   const uint32_t rows = a.rows / a.groups;
-  const bool few = tilesOf(a, 32) * parts(a.outer, 128) < (ring ? kFew : kFewUnaligned);
+  const auto items = [&](uint32_t m, uint32_t n) { return tilesOf(a, m) * parts(a.outer, n); };
+  const bool few = items(32, 128) < (ring ? kFew : kFewUnaligned);
   if constexpr (sizeof(T) == 4) {
     if (few && rows <= kFewRows) return productAs<T, Shape<16, 32, 1, 1, 4, 4>>(a, transposed, ring, stream);
     if (few) return productAs<T, Shape<32, 32, 1, 1, 4, 4>>(a, transposed, ring, stream);
@@ -612,8 +621,8 @@ int product(const cuttHipProductArgs& a, bool transposed, void* stream) {
     if (few && rows <= kFewRows) return productAs<T, Shape<16, 64, 1, 1, 3, 4>>(a, transposed, ring, stream);
     if (few) return productAs<T, Shape<32, 64, 1, 1, 3, 4>>(a, transposed, ring, stream);
     if (rows <= kRows32) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
-    if (rows <= (transposed ? kRows64Transposed : kRows64)) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
-    if (!ring || rows <= kRows128) return productAs<T, Shape<128, 128, 2, 2, 2>>(a, transposed, ring, stream);
+    if (rows <= (transposed ? kRows64Transposed : kRows64) || items(128, 128) < kFew128) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
+    if (!ring || rows <= kRows128 || items(256, 256) < kFew256) return productAs<T, Shape<128, 128, 2, 2, 2>>(a, transposed, ring, stream);
     return productAs<T, Shape<256, 256, 2, 2, 2>>(a, transposed, ring, stream);
   }
 }
@@ -633,12 +642,16 @@ int weightsAnyhow(const cuttHipProductArgs& a, void* stream) {
 template <typename T>
 int weights(const cuttHipProductArgs& a, void* stream) {
   const bool ring = inReach<T>(a.x, 0, a.xStride, a.rows, a.inner) && inReach<T>(a.w, 0, a.wRow, a.rows, a.outer);
-  if constexpr (sizeof(T) == 4)
-    // (off the grid 8188 rows, 60 groups, 2050 x 690: 308 us with these, 334 with tiles of 64 x 128, 359 with 128 x 128)
-    return ring ? weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream) : weightsAnyhow<T, Shape<64, 64, 4, 1, 2>>(a, stream);
-  else if (!ring) return weightsAnyhow<T, Shape<128, 128, 4, 1, 2>>(a, stream);
-  else if (a.rows / a.groups <= kRowsWeights) return weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream);
-  else return weightsInRings<T, Shape<256, 256, 2, 2, 2>>(a, stream);
+  const uint64_t items = weightsItems<Shape<128, 128, 4, 1, 2>>(a);
+  if constexpr (sizeof(T) == 4) {
+    if (ring) return items < kFewWeightsFloat ? weightsInRings<T, Shape<64, 64, 4, 1, 4>>(a, stream) : weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream);
+    return items < kFewWeightsFloat ? weightsAnyhow<T, Shape<64, 64, 2, 2, 2>>(a, stream) : weightsAnyhow<T, Shape<64, 64, 4, 1, 2>>(a, stream);
+  } else {
+    if (!ring) return items < kFewWeightsUnaligned ? weightsAnyhow<T, Shape<64, 64, 2, 2, 2>>(a, stream) : weightsAnyhow<T, Shape<128, 128, 4, 1, 2>>(a, stream);
+    if (items < kFewWeights) return weightsInRings<T, Shape<64, 64, 2, 2, 4>>(a, stream);
+    if (a.rows / a.groups <= kRowsWeights || items < kManyWeights) return weightsInRings<T, Shape<128, 128, 4, 1, 2>>(a, stream);
+    return weightsInRings<T, Shape<256, 256, 2, 2, 2>>(a, stream);
+  }
 }
 
 }  // namespace

@@ -223,6 +223,24 @@ def test_shapes(counts, inner, outer, transposed, dtype):
     assert np.array_equal(got, np64(torch.from_numpy(want).to(dtype)))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("counts,inner,outer", [
+    ([300, 0, 1100], 136, 200), ([2000], 64, 64), ([513, 64, 65], 65, 131),   # few results of many rows
+    ([500] * 16, 264, 1032), ([40, 3] * 8, 500, 777),                            # more
+    ([420] * 12, 2048, 4096)])
+def test_gradients_of_all_shapes(counts, inner, outer, dtype):
+    """Whole numbers, whose sums are exact."""
+    g = generator(8)
+    rows, offsets = sum(counts) + 5, offsets_of(counts)
+    x, dy = made((rows, inner), dtype, True, g, 2), made((rows, outer), dtype, True, g, 2)
+    dw = run_weights(x, dy, offsets, torch.full((len(counts), inner, outer), 7, dtype=dtype, device="cuda"))
+    at = 0
+    for e, n in enumerate(counts):
+        want = x[at:at + n].float().t().contiguous() @ dy[at:at + n].float()
+        assert torch.equal(dw[e], want.to(dtype))
+        at += n
+
+
 def test_offsets_out_of_range():
     """Offsets beyond the rows count as the nearer end, groups whose end is not above their start are empty; a guard behind y stays."""
     g, rows, inner, outer = generator(6), 200, 40, 72
