@@ -37,6 +37,7 @@ struct Attend {
   uint32_t most;              // neighbouring queries of one request that a workgroup takes together, a power of two: their heads share its columns
   uint32_t ranges;            // 0: each query has `pieces` of its own, of `length` tokens (the last one what is left)
   uint32_t pieces, length;
+  float scale, scaleRest;     // of scores that are exponents of 2, and what it is off by: an error that all scores share does not average out
   float perRange;             // what length of a range, by all tokens, makes no more than `ranges`
   cuttHipDivisor byPage, byTiles, byHeads, byShares;  // divisions by pageSize, headTiles, the heads in a column tile and all workgroups of a range
   float* partial;             // [2 * ranges][most][heads][width]: of what begins within a query, and of what ends in one; or [queries][pieces][heads][width]
@@ -245,7 +246,7 @@ __device__ __forceinline__ void waitForLoads() {
   asm volatile("" ::: "memory");
 }
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLn2 = 0.69314718055994530942f;
 // Scores may exceed what they are taken off from by this much (times log2 e) before it is raised: exponentials stay below 2^8, within the range of half.
 constexpr float kSlack = 8.0f;
 __device__ __forceinline__ float exp2Of(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
   PhaseLds& tokens = *reinterpret_cast<PhaseLds*>(lds);
   const uint32_t lane = threadIdx.x & 63, l = lane & 15, quarter = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int width = (int)a.width;
-  const float scale = a.scale * kLog2e;
+  const float scale = p.scale, scaleRest = p.scaleRest;
   // Workgroups that follow each other go to the XCDs in turn: so that none has much more to do than another, a range's heads follow each other, and the eight ranges that
   // do are turned on from eight to eight (every fourth range may be all that has work, as drafted tokens are taken together).
   const uint32_t shares = a.keyHeads * p.headTiles, at = divide(blockIdx.x, p.byShares), share = blockIdx.x - at * shares;
@@ -402,15 +403,28 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
     };
     Acc score[SUB];
     const auto scores = [&]() __attribute__((always_inline)) {
+      const auto keysOf = [&](int i, int s) __attribute__((always_inline)) -> Chunk<T> {
+        if constexpr (DIRECT) return keys[S::keyPlace(i * 16 + l, s * 4 + quarter)];
+        else return k[i][s];
+      };
+      if constexpr (sizeof(T) == 4) {
+        // Four sums of a quarter of the terms each: their roundings add up to half as much, and no instruction waits for the one before it.
+        Acc part[4] = {};
 #pragma unroll
-      for (int i = 0; i < SUB; i++) score[i] = Acc(0);
+        for (int s = 0; s < STEPS; s++) {
+          const Chunk<T> of = keysOf(0, s);
 #pragma unroll
-      for (int s = 0; s < STEPS; s++)
-#pragma unroll
-        for (int i = 0; i < SUB; i++) {
-          if constexpr (DIRECT) score[i] = multiply(keys[S::keyPlace(i * 16 + l, s * 4 + quarter)], q[s], score[i]);
-          else score[i] = multiply(k[i][s], q[s], score[i]);
+          for (int e = 0; e < 4; e++) part[e] = multiply(of[e], q[s][e], part[e]);
         }
+        score[0] = (part[0] + part[1]) + (part[2] + part[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < SUB; i++) score[i] = Acc(0);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+          for (int i = 0; i < SUB; i++) score[i] = multiply(keysOf(i, s), q[s], score[i]);
+      }
     };
     // Weighted values added to the sums; with a mask those of the lane's tokens t with bit t of it, for the columns that `mine` says.
     const auto addWeighted = [&](auto masked, uint32_t mask, bool mine) __attribute__((always_inline)) {
@@ -481,7 +495,9 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
       const bool whole = full && first >= from && first + TILE <= till;  // every column sees every token
       uint32_t mine = 0;  // of the lane's tokens t those that have a page
 #pragma unroll
-      for (int i = 0; i < SUB; i++) score[i] *= scale;
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) score[i][r] = fmaf(score[i][r], scale, score[i][r] * scaleRest);
       if (!whole) {
         const uint32_t there = (uint32_t)(tokens.there[tile * TILE / 64] >> (tile * TILE % 64));
 #pragma unroll
@@ -774,6 +790,9 @@ extern "C" size_t cuttHipAttendWorkspace(uint32_t queries, uint32_t heads, uint3
 extern "C" int cuttHipAttend(const cuttHipAttendArgs* a, int type, void* stream) {
   Attend p = planAttend(a->queries, a->heads, a->keyHeads, a->width, a->pageSize, a->tableWidth, a->window);
   p.a = *a;
+  const double scale = a->scale * 1.44269504088896340736;
+  p.scale = (float)scale;
+  p.scaleRest = (float)(scale - p.scale);
   float* const space = static_cast<float*>(a->workspace);
   const size_t rows = rowsOf(p, a->queries) * a->heads;
   p.tops = space;
