@@ -10,6 +10,7 @@
  * read of as much reaches 6.2 (6.9 past the caches); 256 requests of 2048 each: 338 us, 6.4 TB/s; one request of 128 tokens: 7.3 us.
  */
 #include <algorithm>
+#include <cfloat>
 
 #include "product_device.h"
 #include "product_layer.h"
@@ -497,7 +498,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
 #pragma unroll
       for (int i = 0; i < SUB; i++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) score[i][r] = fmaf(score[i][r], scale, score[i][r] * scaleRest);
+        for (int r = 0; r < 4; r++)  // (what the rest adds to a score of infinity must not be the other infinity)
+          score[i][r] = fmaf(score[i][r], scale, __builtin_amdgcn_fmed3f(score[i][r] * scaleRest, -FLT_MAX, FLT_MAX));
       if (!whole) {
         const uint32_t there = (uint32_t)(tokens.there[tile * TILE / 64] >> (tile * TILE % 64));
 #pragma unroll

@@ -1,0 +1,103 @@
+"""Attention over pages where scores or values are infinite, and where weights are small, against the definition in 64 bits.
+
+Tolerances as for the products' other tests: a score is off by d = (width + 4) * 2^-23 times its terms' sizes, an exponential by that relative to itself and a few steps, numerator
+and denominator alike, and the result by half a step of its type.  Terms and sizes are those of the finite tokens: the others have the weight 0, or make their element infinite."""
+import numpy as np
+import pytest
+import torch
+
+import product_oracle as oracle
+from test_gpu_products import HALF, LEAST, TYPES, UNIT, Cache, generator, ids_of, ints, np64, run_attend
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+# What a weight can be off by: 16-bit types keep an exponential in two parts.  Half's smallest step is 2^-24, and the largest exponential is 2^15 at least.
+PART = {torch.float32: 0.0, torch.float16: 2.0 ** -22, torch.bfloat16: 2.0 ** -16}
+FLOOR = {torch.float32: 0.0, torch.float16: 2.0 ** -40, torch.bfloat16: 0.0}
+
+
+def tolerance(want, size, terms, count, most, width, dtype):
+    """Of out, and of the log sums without what is relative to these."""
+    score, n = terms * (width + 4) * UNIT + 8 * UNIT, count[:, None]
+    out = size * (2 * np.expm1(2 * score) + (2 * n + 40) * UNIT + PART[dtype])[:, :, None] + n[:, :, None] * most * FLOOR[dtype] + np.abs(want) * HALF[dtype] * 1.01 + LEAST[dtype]
+    return out, 2 * score + (n + 10) * UNIT
+
+
+def check(q, cache, owners, positions, window, scale, out, logs):
+    """Keys of infinity or the lowest value count as 1e30, whose scores' exponentials are 0 in 64 bits; a query with no others sees nothing that counts."""
+    who = np.arange(q.shape[0]) if owners is None else owners.cpu().numpy()
+    rest = (cache.tables.cpu().numpy(), who, positions.cpu().numpy(), window, scale)
+    k, v = np64(cache.k), np64(cache.v)
+    far = np.abs(k) > 1e30
+    with np.errstate(all="ignore"):
+        want, want_logs, size, _, count, most = oracle.attend(np64(q), np.where(far, np.sign(k) * 1e30, k), v, *rest)
+        terms = oracle.attend(np64(q), np.where(far, 0, k), np.zeros(v.shape), *rest)[3]
+        off, off_logs = tolerance(want, size, terms, count, most, q.shape[2], q.dtype)
+        out, logs = np64(out), np64(logs)
+        none = want_logs < -1e25
+        want[none] = 0
+        odd = ~np.isfinite(want)
+        wrong = np.isfinite(out) == odd
+        assert not wrong.any(), (np.argwhere(wrong)[:5], out[wrong][:5], want[wrong][:5])
+        assert np.array_equal(out[odd], want[odd], equal_nan=True)
+        bad = ~odd & ~(np.abs(out - want) <= off)
+        assert not bad.any(), (int(bad.sum()), out[bad][:5], want[bad][:5], off[bad][:5])
+        assert np.array_equal(np.isneginf(logs), none)
+        bad = ~none & ~(np.abs(logs - want_logs) <= off_logs + 4 * np.abs(np.where(none, 0, want_logs)) * UNIT)
+        assert not bad.any(), (logs[bad][:5], want_logs[bad][:5])
+
+
+def cell(cache, b, t):
+    """The page and slot of request b's token t."""
+    return int(cache.tables[b, t // cache.page]), t % cache.page
+
+
+# Requests of one and two tiles and their edges; cut into ranges; drafted tokens whose windows end within tiles.
+FORMS = {
+    "short": ([1, 16, 33, 100, 256], 1, 0),
+    "long": ([6000, 40], 1, 0),
+    "drafts": ([90, 300, 31], 3, 50),
+}
+
+
+def form(name, dtype, width, key_heads=2, shared=2, seed=51):
+    lengths, drafts, window = FORMS[name]
+    g = generator(seed)
+    cache = Cache(lengths, 16, key_heads, width, dtype, "slot", g)
+    owners = ints([b for b in range(len(lengths)) for _ in range(drafts)])
+    positions = ints([n - drafts + i for n in lengths for i in range(drafts)])
+    q = torch.randn(len(lengths) * drafts, key_heads * shared, width, generator=g, device="cuda").to(dtype)
+    return cache, q, owners, positions, window, lengths, g
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("name", FORMS)
+@pytest.mark.parametrize("width,scale", [(32, 32 ** -0.5), (64, 64 ** -0.5), (96, 96 ** -0.5), (128, 128 ** -0.5), (64, 0.1), (64, 0.2), (64, 0.3), (80, 1.0), (256, -0.1),
+                                         (40, -0.3)])
+def test_scores_of_minus_infinity(width, scale, name, dtype):
+    """Tokens with a score of -infinity, every third one, count nothing, whatever the scale's rounding; where there are no others, zeros and -infinity."""
+    cache, q, owners, positions, window, lengths, g = form(name, dtype, width)
+    q[:, :, 0] = 4.0
+    low = -INF if scale > 0 else INF
+    for b, n in enumerate(lengths):
+        for t in range(0, n, 3):
+            cache.k[cell(cache, b, t)][:, 0] = low
+    out, logs = run_attend(q, cache, owners, positions, window, scale)
+    check(q, cache, owners, positions, window, scale, out, logs)
+    cache.k[..., 0] = low
+    out, logs = run_attend(q, cache, owners, positions, window, scale)
+    assert bool((out == 0).all()) and bool((logs == -INF).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [128 ** -0.5, 0.1, 0.3])
+def test_keys_of_the_lowest_value(scale, dtype):
+    """Their scores leave the range of 32 bits."""
+    cache, q, owners, positions, window, lengths, g = form("short", dtype, 128)
+    q[:, :, 0] = 4.0
+    for b, n in enumerate(lengths):
+        for t in range(0, n - 1, 2):
+            cache.k[cell(cache, b, t)][:, 0] = torch.finfo(dtype).min
+    out, logs = run_attend(q, cache, owners, positions, window, scale)
+    check(q, cache, owners, positions, window, scale, out, logs)
