@@ -793,7 +793,7 @@ extern "C" int cuttHipAttend(const cuttHipAttendArgs* a, int type, void* stream)
   Attend p = planAttend(a->queries, a->heads, a->keyHeads, a->width, a->pageSize, a->tableWidth, a->window);
   p.a = *a;
   const double scale = a->scale * 1.44269504088896340736;
-  p.scale = (float)scale;
+  p.scale = (float)std::max(std::min(scale, (double)FLT_MAX), -(double)FLT_MAX);  // (the rest has what the largest scales exceed that by)
   p.scaleRest = (float)(scale - p.scale);
   float* const space = static_cast<float*>(a->workspace);
   const size_t rows = rowsOf(p, a->queries) * a->heads;

@@ -101,3 +101,23 @@ def test_keys_of_the_lowest_value(scale, dtype):
             cache.k[cell(cache, b, t)][:, 0] = torch.finfo(dtype).min
     out, logs = run_attend(q, cache, owners, positions, window, scale)
     check(q, cache, owners, positions, window, scale, out, logs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("scale", [3.4e38, -3.4e38, 2.5e38])
+def test_largest_scales(scale, dtype):
+    """Scales whose product with log2 e leaves the range of 32 bits: scores of 0 stay 0, and one that is higher takes all of the weight."""
+    cache, q, owners, positions, window, lengths, g = form("short", dtype, 64)
+    q.zero_()
+    out, logs = run_attend(q, cache, owners, positions, window, scale)
+    check(q, cache, owners, positions, window, scale, out, logs)
+    q[:, :, 0] = 2.0 ** -24
+    cache.k.zero_()
+    for b, n in enumerate(lengths):
+        cache.k[cell(cache, b, n // 2)][:, 0] = -2.0 ** -20 if scale < 0 else 2.0 ** -20
+    out, logs = run_attend(q, cache, owners, positions, window, scale)
+    assert float((logs / (abs(scale) * 2.0 ** -44) - 1).abs().max()) <= 2.0 ** -20
+    for i, b in enumerate(owners.tolist()):
+        v = cache.v[cell(cache, b, lengths[b] // 2)]
+        for h in range(4):
+            assert torch.equal(out[i, h], v[h // 2])
