@@ -673,11 +673,12 @@ __global__ __launch_bounds__(kThreads) void joinKernel(Attend p) {
       float top[AT], sum[AT], part[AT][PER];
 #pragma unroll
       for (uint32_t u = 0; u < AT; u++) {
-        const uint64_t row = rowOf(min(i + u * kWaves, ranges - 1));
-        top[u] = i + u * kWaves < ranges ? p.tops[row * 2] : -INFINITY;
-        sum[u] = p.tops[row * 2 + 1];
+        const bool is = i + u * kWaves < ranges;  // (behind the last one nothing, which its infinities must not meet)
+        const uint64_t row = rowOf(is ? i + u * kWaves : ranges - 1);
+        top[u] = is ? p.tops[row * 2] : -INFINITY;
+        sum[u] = is ? p.tops[row * 2 + 1] : 0.0f;
 #pragma unroll
-        for (uint32_t j = 0; j < PER; j++) part[u][j] = lane + j * 64 < a.width ? p.partial[row * a.width + lane + j * 64] : 0.0f;
+        for (uint32_t j = 0; j < PER; j++) part[u][j] = is && lane + j * 64 < a.width ? p.partial[row * a.width + lane + j * 64] : 0.0f;
       }
       float next = m;
 #pragma unroll
@@ -688,7 +689,7 @@ __global__ __launch_bounds__(kThreads) void joinKernel(Attend p) {
       for (uint32_t j = 0; j < PER; j++) o[j] *= less;
 #pragma unroll
       for (uint32_t u = 0; u < AT; u++) {
-        const float share = exp2Of(top[u] - baseOf(next));  // (0 behind the last one)
+        const float share = exp2Of(top[u] - baseOf(next));
         n += share * sum[u];
 #pragma unroll
         for (uint32_t j = 0; j < PER; j++) o[j] += share * part[u][j];

@@ -121,3 +121,21 @@ def test_largest_scales(scale, dtype):
         v = cache.v[cell(cache, b, lengths[b] // 2)]
         for h in range(4):
             assert torch.equal(out[i, h], v[h // 2])
+
+
+@pytest.mark.parametrize("dtype", TYPES[:1], ids=ids_of[:1])
+@pytest.mark.parametrize("queries", [1, 2, 5])
+def test_infinite_values_at_the_end_of_cut_queries(queries, dtype):
+    """Where the last part of a query's tokens, and of every other part too, holds infinities: as many parts as there are, none of them counts twice or as nothing."""
+    for longest in (1000, 2100, 2900, 5000):
+        g = generator(61)
+        cache = Cache([longest - 100 * i for i in range(queries)], 16, 1, 64, dtype, "slot", g)
+        q = torch.randn(queries, 2, 64, generator=g, device="cuda").to(dtype)
+        positions = ints([longest - 100 * i - 1 for i in range(queries)])
+        for b in range(queries):
+            n = longest - 100 * b
+            for d in range(8):
+                cache.v[cell(cache, b, (n - 1) * d // 7)][0, d] = INF
+            cache.v[cell(cache, b, n - 1)][0, 9] = -INF
+        out, logs = run_attend(q, cache, None, positions, 0, 0.125)
+        check(q, cache, None, positions, 0, 0.125, out, logs)
