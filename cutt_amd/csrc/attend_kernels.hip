@@ -251,8 +251,8 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // Scores may exceed what they are taken off from by this much (times log2 e) before it is raised: exponentials stay below 2^8, within the range of half.
 constexpr float kSlack = 8.0f;
 __device__ __forceinline__ float exp2Of(float x) { return __builtin_amdgcn_exp2f(x); }
-// What scores are taken off from before they are exponents, unless there are only scores of -infinity.
-__device__ __forceinline__ float baseOf(float top) { return top == -INFINITY ? 0.0f : top; }
+// What scores are taken off from before they are exponents, unless there are only scores of -infinity.  (Finite: a score of +infinity has the exponential +infinity.)
+__device__ __forceinline__ float baseOf(float top) { return top == -INFINITY ? 0.0f : fminf(top, FLT_MAX); }
 
 struct PhaseLds {
   uint64_t offset[kPhase];      // of the phase's tokens in the caches, in elements

@@ -72,8 +72,8 @@ size_t cuttAttendPagesWorkspace(int queries, int heads, int keyHeads, int width,
  * Head h uses the keys and values of key head h / (heads / keyHeads).  With s_t = scale * (q[i, h, :] . k[t, :]) over the tokens t that it sees:
  *   logSums[i, h]     log of the sum of exp(s_t)
  *   out[i, h, :]      sum of exp(s_t - logSums[i, h]) * v[t, :]
- * A query that sees nothing (a position below 0, an owner not in 0 .. requests - 1), or whose scores are all -infinity, gets zeros, and -infinity.  Keys and
- * values that are not seen have no part in it, whatever they hold.
+ * A query that sees nothing (a position below 0, an owner not in 0 .. requests - 1), or whose scores are all -infinity, gets zeros, and -infinity; one with a score of
+ * +infinity NaN, and +infinity.  Keys and values that are not seen have no part in it, whatever they hold.
  *
  *   queries, requests, pages >= 0, keyHeads >= 1, heads <= CUTT_MAX_HEADS a multiple of it, queries * heads < 2^31
  *   1 <= width <= CUTT_MAX_HEAD_WIDTH, pageSize, tableWidth >= 1, scale finite

@@ -123,6 +123,27 @@ def test_largest_scales(scale, dtype):
             assert torch.equal(out[i, h], v[h // 2])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("name", FORMS)
+def test_scores_of_plus_infinity(name, dtype):
+    """A score of +infinity: the log sum is +infinity, and out, infinity over infinity, is no number; other heads are as without it.  A score that is no number: neither."""
+    cache, q, owners, positions, window, lengths, g = form(name, dtype, 64)
+    want, want_logs = run_attend(q, cache, owners, positions, window, 0.125)
+    for bad in (INF, float("nan")):
+        other = Cache.__new__(Cache)
+        other.__dict__.update(cache.__dict__, k=cache.k.clone())
+        other.k[cell(cache, 0, lengths[0] - 1 if len(owners) == len(lengths) else lengths[0] - 3)][1, 5] = bad
+        out, logs = run_attend(q, other, owners, positions, window, 0.125)
+        for i, b in enumerate(owners.tolist()):
+            for h in range(4):
+                score = float(q[i, h, 5]) * bad
+                if b or h < 2:
+                    assert torch.equal(out[i, h], want[i, h]) and torch.equal(logs[i, h], want_logs[i, h])
+                elif score != -INF:
+                    assert bool(out[i, h].isnan().all())
+                    assert float(logs[i, h]) == INF if score == INF else bool(logs[i, h].isnan())
+
+
 @pytest.mark.parametrize("dtype", TYPES[:1], ids=ids_of[:1])
 @pytest.mark.parametrize("queries", [1, 2, 5])
 def test_infinite_values_at_the_end_of_cut_queries(queries, dtype):
