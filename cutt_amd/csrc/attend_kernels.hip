@@ -247,6 +247,10 @@ __device__ __forceinline__ void waitForLoads() {
   asm volatile("" ::: "memory");
 }
 
+// What stands for a weight above 0 where only infinities are wanted: so small that no sum of finite values leaves the range of 32 bits.
+template <typename T>
+constexpr float kSome = std::is_same_v<T, _Float16> ? 1.0f : 0x1p-64f;
+
 constexpr float kLn2 = 0.69314718055994530942f;
 // Scores may exceed what they are taken off from by this much (times log2 e) before it is raised: exponentials stay below 2^8, within the range of half.
 constexpr float kSlack = 8.0f;
@@ -345,8 +349,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
         q[s] = loadChunk(line + d, column ? width - d : 0);
       }
     }
-    float top = -INFINITY, sum = 0;  // of this lane's column: what scores are taken off from (times log2 e), the exponentials of this quarter's tokens
-    Acc acc[VD] = {};
+    float top, sum;  // of this lane's column: what scores are taken off from (times log2 e), the exponentials of this quarter's tokens
+    Acc acc[VD];
+    // An exponential's second part, 0 or below 0 as often as not, makes NaN of an infinite value.  Where the 16-bit types have got NaN, all is done again with one number in place
+    // of all exponentials above 0, in both parts: what is infinite then takes the place of NaN.  (92 requests of up to 97 tokens, two queries each, 32 heads of 192 halves: 156 us; 148
+    // without; 179 where the tiles at queries' ends, and all when done again, have a product of their own for such values.)
+    bool again = false;
+    float limit = INFINITY, twice = 1.0f;  // (again: 0 and 2)
 
     // DIRECT: the wavefront's tiles in LDS.
     Chunk<T>* const keys = reinterpret_cast<Chunk<T>*>(lds + sizeof(PhaseLds) + wave * S::BYTES);
@@ -452,8 +461,9 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
         Chunk<T> high, low;
 #pragma unroll
         for (int t = 0; t < 8; t++) {
-          high[t] = (T)score[t / 4][t % 4];
-          low[t] = (T)(score[t / 4][t % 4] - (float)high[t]);
+          const float e = score[t / 4][t % 4] > limit ? kSome<T> : score[t / 4][t % 4];
+          high[t] = (T)e;
+          low[t] = (T)fmaf(e, twice, -(float)high[t]);
         }
         typedef uint32_t Words __attribute__((ext_vector_type(4)));
         Words keep;
@@ -521,7 +531,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
         top = next;
         sum *= less;
 #pragma unroll
-        for (int j = 0; j < VD; j++) acc[j] *= less;
+        for (int j = 0; j < VD; j++) acc[j] *= again ? 1.0f : less;
       }
       const float base = baseOf(top);
 #pragma unroll
@@ -550,90 +560,116 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
       }
     };
 
-    for (uint32_t phase = seen.first; phase < seen.end; phase += kPhase) {
-      __syncthreads();
-      placeTokens(phase);
-      __syncthreads();
-      askPages(phase + kPhase);
-      // The wavefront's tiles: every kWaves-th of those that have a token.
-      static_assert(kPhase / TILE <= 64, "a lane for every tile");
-      uint32_t there = 0;
-      if (lane < kPhase / TILE) there = (uint32_t)(tokens.there[lane * TILE / 64] >> (lane * TILE % 64)) & ALL;
-      uint64_t left = __ballot(there != 0) & (0x1111111111111111ull << wave);
-      const uint64_t full = __ballot(there == ALL);
-      if (!left) continue;
-      uint32_t tile = __builtin_ctzll(left);
-      loadKeys(tile);
-      loadValues(tile);
-      // The next tile's keys are asked for as soon as this one's have been used, its values likewise; behind the last tile the same ones again, which nobody waits
-      // for: with a condition around loads to registers the compiler, which counts the loads that it waits for, would have to wait for all.
-      for (;;) {
-        if constexpr (DIRECT) waitForLoads<S::LOADS>();  // (the values' loads may be under way)
-        scores();
-        left &= left - 1;
-        const uint32_t next = left ? __builtin_ctzll(left) : tile;
-        if constexpr (DIRECT) {
-          if (left) {
-            loadKeys(next);
-            waitForLoads<S::LOADS>();
+    for (;;) {
+      top = -INFINITY;
+      sum = 0;
+#pragma unroll
+      for (int j = 0; j < VD; j++) acc[j] = Acc(0);
+      for (uint32_t phase = seen.first; phase < seen.end; phase += kPhase) {
+        __syncthreads();
+        placeTokens(phase);
+        __syncthreads();
+        askPages(phase + kPhase);
+        // The wavefront's tiles: every kWaves-th of those that have a token.
+        static_assert(kPhase / TILE <= 64, "a lane for every tile");
+        uint32_t there = 0;
+        if (lane < kPhase / TILE) there = (uint32_t)(tokens.there[lane * TILE / 64] >> (lane * TILE % 64)) & ALL;
+        uint64_t left = __ballot(there != 0) & (0x1111111111111111ull << wave);
+        const uint64_t full = __ballot(there == ALL);
+        if (!left) continue;
+        uint32_t tile = __builtin_ctzll(left);
+        loadKeys(tile);
+        loadValues(tile);
+        // The next tile's keys are asked for as soon as this one's have been used, its values likewise; behind the last tile the same ones again, which nobody waits
+        // for: with a condition around loads to registers the compiler, which counts the loads that it waits for, would have to wait for all.
+        for (;;) {
+          if constexpr (DIRECT) waitForLoads<S::LOADS>();  // (the values' loads may be under way)
+          scores();
+          left &= left - 1;
+          const uint32_t next = left ? __builtin_ctzll(left) : tile;
+          if constexpr (DIRECT) {
+            if (left) {
+              loadKeys(next);
+              waitForLoads<S::LOADS>();
+            } else {
+              waitForLoads<0>();
+            }
           } else {
-            waitForLoads<0>();
+            loadKeys(next);
           }
-        } else {
-          loadKeys(next);
+          addValues(tile, phase + tile * TILE, full >> tile & 1);
+          if (!left) break;
+          loadValues(next);
+          tile = next;
         }
-        addValues(tile, phase + tile * TILE, full >> tile & 1);
-        if (!left) break;
-        loadValues(next);
-        tile = next;
       }
-    }
 
-    // The wavefronts' parts together.
-    sum = overQuarters(sum, [](float x, float y) { return x + y; });
-    __syncthreads();
-    float* const tops = reinterpret_cast<float*>(lds);            // [waves][columns]
-    float* const sums = tops + kWaves * kColumns;
-    float* const parts = sums + kWaves * kColumns;                // [waves][columns][DP + 4]
-    constexpr uint32_t PITCH = DP + 4;
-    if (quarter == 0) {
-      tops[wave * kColumns + l] = top;
-      sums[wave * kColumns + l] = sum;
-    }
-    __syncthreads();
-    float all = -INFINITY;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; w++) all = fmaxf(all, tops[w * kColumns + l]);
-    const float mine = exp2Of(top - baseOf(all));
-    if (column)
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int j = 0; j < VD; j++) parts[(wave * kColumns + l) * PITCH + S::elementOf(j, quarter * 4 + r)] = acc[j][r] * mine;
-    __syncthreads();
-    for (uint32_t c = wave; c < queries * nHeads; c += kWaves) {
-      const uint32_t n = p.most > 1 ? divide(c, p.byHeads) : 0, h = head0 + c - n * nHeads;
-      float m = -INFINITY, of = 0;
-#pragma unroll
-      for (uint32_t w = 0; w < kWaves; w++) m = fmaxf(m, tops[w * kColumns + c]);
-#pragma unroll
-      for (uint32_t w = 0; w < kWaves; w++) of += sums[w * kColumns + c] * exp2Of(tops[w * kColumns + c] - baseOf(m));
-      const bool none = of == 0 && m == -INFINITY;
-      const uint64_t to = range.from.query + n;
-      const uint64_t row = (p.ranges ? (uint64_t)slot * p.most + n : to * p.pieces + (index - range.from.query * p.pieces)) * a.heads + h;
-      for (uint32_t d = lane; d < a.width; d += 64) {
-        float o = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < kWaves; w++) o += parts[(w * kColumns + c) * PITCH + d];
-        if (cut) p.partial[row * a.width + d] = o;
-        else static_cast<T*>(a.out)[to * a.outStride + h * a.outHead + d] = (T)(none ? 0.0f : o / of);
+      // The wavefronts' parts together.
+      sum = overQuarters(sum, [](float x, float y) { return x + y; });
+      __syncthreads();
+      float* const tops = reinterpret_cast<float*>(lds);            // [waves][columns]
+      float* const sums = tops + kWaves * kColumns;
+      uint32_t* const odds = reinterpret_cast<uint32_t*>(sums + kWaves * kColumns);  // [waves]: whether there is NaN
+      float* const parts = sums + kWaves * kColumns + kWaves;       // [waves][columns][DP + 4]
+      constexpr uint32_t PITCH = DP + 4;
+      if (quarter == 0) {
+        tops[wave * kColumns + l] = top;
+        sums[wave * kColumns + l] = sum;
       }
-      if (lane == 0) {
-        if (cut) {
-          p.tops[row * 2] = m;
-          p.tops[row * 2 + 1] = of;
-        } else if (a.logSums) a.logSums[to * a.heads + h] = none ? -INFINITY : (m + __log2f(of)) * kLn2;
+      if constexpr (sizeof(T) == 2) {
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < VD; j++) odd |= __builtin_isunordered(acc[j][0], acc[j][1]) | __builtin_isunordered(acc[j][2], acc[j][3]);
+        odd = __any(odd && column);
+        if (lane == 0) odds[wave] = odd;
       }
+      __syncthreads();
+      uint32_t odd = 0;
+      if constexpr (sizeof(T) == 2)
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) odd |= odds[w];
+      float all = -INFINITY;
+#pragma unroll
+      for (uint32_t w = 0; w < kWaves; w++) all = fmaxf(all, tops[w * kColumns + l]);
+      const float mine = again ? 1.0f : exp2Of(top - baseOf(all));
+      if (column)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int j = 0; j < VD; j++) parts[(wave * kColumns + l) * PITCH + S::elementOf(j, quarter * 4 + r)] = acc[j][r] * mine;
+      __syncthreads();
+      for (uint32_t c = wave; c < queries * nHeads; c += kWaves) {
+        const uint32_t n = p.most > 1 ? divide(c, p.byHeads) : 0, h = head0 + c - n * nHeads;
+        float m = -INFINITY, of = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) m = fmaxf(m, tops[w * kColumns + c]);
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) of += sums[w * kColumns + c] * exp2Of(tops[w * kColumns + c] - baseOf(m));
+        const bool none = of == 0 && m == -INFINITY;
+        const uint64_t to = range.from.query + n;
+        const uint64_t row = (p.ranges ? (uint64_t)slot * p.most + n : to * p.pieces + (index - range.from.query * p.pieces)) * a.heads + h;
+        for (uint32_t d = lane; d < a.width; d += 64) {
+          float o = 0;
+#pragma unroll
+          for (uint32_t w = 0; w < kWaves; w++) o += parts[(w * kColumns + c) * PITCH + d];
+          float* const part = p.partial + (row * a.width + d);
+          T* const out = static_cast<T*>(a.out) + (to * a.outStride + h * a.outHead + d);
+          if (again && (fabsf(o) <= FLT_MAX || (cut ? *part == *part : *out == *out))) continue;  // (this thread has written it before)
+          if (cut) *part = o;
+          else *out = (T)(none ? 0.0f : o / of);
+        }
+        if (lane == 0) {
+          if (cut) {
+            p.tops[row * 2] = m;
+            p.tops[row * 2 + 1] = of;
+          } else if (a.logSums) a.logSums[to * a.heads + h] = none ? -INFINITY : (m + __log2f(of)) * kLn2;
+        }
+      }
+      if (sizeof(T) == 4 || again || !__builtin_amdgcn_readfirstlane(odd)) break;
+      again = true;
+      limit = 0.0f;
+      twice = 2.0f;
+      askPages(seen.first);
     }
 
     if ((p.ranges || p.pieces > 1) && range.from.from == 0 && share == 0 && threadIdx.x < queries) {
@@ -756,7 +792,7 @@ size_t rowsOf(const Attend& p, uint32_t queries) { return p.ranges ? 2 * (size_t
 
 template <typename T, int DP, bool DIRECT>
 int attend(const Attend& p, void* stream) {
-  const size_t space = sizeof(PhaseLds) + kWaves * Tokens<T, DP, DIRECT>::BYTES, join = (2 * kWaves * kColumns + kWaves * kColumns * (DP + 4)) * 4;
+  const size_t space = sizeof(PhaseLds) + kWaves * Tokens<T, DP, DIRECT>::BYTES, join = (2 * kWaves * kColumns + kWaves + kWaves * kColumns * (DP + 4)) * 4;
   const size_t lds = std::max({space, sizeof(ScanLds), join});
   const uint32_t shares = p.a.keyHeads * p.headTiles;
   const uint32_t most = std::max(1u, (1u << 20) / shares) * 8;  // (a launch's lanes stay below 2^32)

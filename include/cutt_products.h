@@ -73,7 +73,8 @@ size_t cuttAttendPagesWorkspace(int queries, int heads, int keyHeads, int width,
  *   logSums[i, h]     log of the sum of exp(s_t)
  *   out[i, h, :]      sum of exp(s_t - logSums[i, h]) * v[t, :]
  * A query that sees nothing (a position below 0, an owner not in 0 .. requests - 1), or whose scores are all -infinity, gets zeros, and -infinity; one with a score of
- * +infinity NaN, and +infinity.  Keys and values that are not seen have no part in it, whatever they hold.
+ * +infinity NaN, and +infinity.  Infinite values that are seen make their element infinite, both signs or NaN make it NaN (so may an infinity whose weight is below 2^-126 of
+ * the largest).  Keys and values that are not seen have no part in it, whatever they hold.
  *
  *   queries, requests, pages >= 0, keyHeads >= 1, heads <= CUTT_MAX_HEADS a multiple of it, queries * heads < 2^31
  *   1 <= width <= CUTT_MAX_HEAD_WIDTH, pageSize, tableWidth >= 1, scale finite

@@ -144,7 +144,22 @@ def test_scores_of_plus_infinity(name, dtype):
                     assert float(logs[i, h]) == INF if score == INF else bool(logs[i, h].isnan())
 
 
-@pytest.mark.parametrize("dtype", TYPES[:1], ids=ids_of[:1])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("width,key_heads", [(64, 2), (128, 2), (200, 1), (77, 2)])
+@pytest.mark.parametrize("name", FORMS)
+def test_infinite_values(name, width, key_heads, dtype):
+    """Infinities in values that are seen make their element infinite, one of either sign or NaN make it no number; all other elements are as they were."""
+    cache, q, owners, positions, window, lengths, g = form(name, dtype, width, key_heads)
+    for b, n in enumerate(lengths):
+        for d, (t, x) in enumerate([(0, INF), (n // 2, -INF), (n - 1, INF), (n // 3, float("nan")), (n // 2, INF), (min(n - 1, 20), -INF), (max(n - 40, 0), INF)]):
+            cache.v[cell(cache, b, t)][:, 3 * d + 1] = x
+        for t, x in ((n // 3, INF), (n - 1, -INF)):
+            cache.v[cell(cache, b, t)][:, 40 + (n == 1)] = x
+    out, logs = run_attend(q, cache, owners, positions, window, 0.125)
+    check(q, cache, owners, positions, window, 0.125, out, logs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 @pytest.mark.parametrize("queries", [1, 2, 5])
 def test_infinite_values_at_the_end_of_cut_queries(queries, dtype):
     """Where the last part of a query's tokens, and of every other part too, holds infinities: as many parts as there are, none of them counts twice or as nothing."""
@@ -160,3 +175,19 @@ def test_infinite_values_at_the_end_of_cut_queries(queries, dtype):
             cache.v[cell(cache, b, n - 1)][0, 9] = -INF
         out, logs = run_attend(q, cache, None, positions, 0, 0.125)
         check(q, cache, None, positions, 0, 0.125, out, logs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("below", [15.0, 30.0, 60.0, 80.0])
+def test_infinite_values_of_small_weights(below, dtype):
+    """As long as a weight is a number of 32 bits above 0, an infinity times it is one, whatever 16 bits would make of the weight."""
+    cache, q, owners, positions, window, lengths, g = form("short", dtype, 64, 1)
+    cache.k.zero_()
+    q.zero_()
+    q[:, :, 0] = 1.0
+    for b, n in enumerate(lengths):
+        cache.k[cell(cache, b, n // 2)][:, 0] = below
+        for t in range(0, n, 7):
+            cache.v[cell(cache, b, t)][:, t % 60] = INF if t % 2 else -INF
+    out, logs = run_attend(q, cache, owners, positions, window, 1.0)
+    check(q, cache, owners, positions, window, 1.0, out, logs)
