@@ -3,7 +3,8 @@
  *
  * With s_t = scale q.k_t, what is wanted is sum exp(s_t) v_t / sum exp(s_t) over the tokens t that a query sees.  It is had in one pass: scores are taken off from a number `top` near
  * the largest so far, and what has been summed is scaled when that is raised.  Parts of a query's tokens, each with its `top`, are joined by the same scaling, first a workgroup's four
- * wavefronts', then, in a second launch, those of the workgroups that share the query.  All of this is in 32 bits; only the products' operands have 16 where the type has.
+ * wavefronts', then, in a second launch, those of the workgroups that share the query.  All of this is in 32 bits; only the products' operands have 16 where the type has, exponentials
+ * twice 16.
  *
  * Every cached element is read once, and takes two operations for each of the query heads that share it: memory bounds it, and where there is little of it the chain
  * offsets -> page -> keys -> scores -> values -> joined parts.  64 requests of up to 8192 tokens, 32 heads on 8 key heads of 128 bfloat16 (1075 MB): 194 us, 5.5 TB/s, where a pure
@@ -249,11 +250,15 @@ __device__ __forceinline__ void waitForLoads() {
 
 // What stands for a weight above 0 where only infinities are wanted: so small that no sum of finite values leaves the range of 32 bits.
 template <typename T>
-constexpr float kSome = std::is_same_v<T, _Float16> ? 1.0f : 0x1p-64f;
+constexpr float kSome = std::is_same_v<T, _Float16> ? 0x1p-15f : 0x1p-64f;
 
 constexpr float kLn2 = 0.69314718055994530942f;
-// Scores may exceed what they are taken off from by this much (times log2 e) before it is raised: exponentials stay below 2^8, within the range of half.
-constexpr float kSlack = 8.0f;
+// Scores may exceed what they are taken off from by kSlack (times log2 e) before it is raised.  Half's exponentials are multiplied by kTimes, so that they use the type's range: they stay
+// below 2^16, and of its smallest step, 2^-24, the half that is lost in both parts of an exponential is 2^-40 of the largest.
+template <typename T>
+constexpr float kSlack = std::is_same_v<T, _Float16> ? 0.9f : 8.0f;
+template <typename T>
+constexpr float kTimes = std::is_same_v<T, _Float16> ? 0x1p15f : 1.0f;
 __device__ __forceinline__ float exp2Of(float x) { return __builtin_amdgcn_exp2f(x); }
 // What scores are taken off from before they are exponents, unless there are only scores of -infinity.  (Finite: a score of +infinity has the exponential +infinity.)
 __device__ __forceinline__ float baseOf(float top) { return top == -INFINITY ? 0.0f : fminf(top, FLT_MAX); }
@@ -355,7 +360,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
     // of all exponentials above 0, in both parts: what is infinite then takes the place of NaN.  (92 requests of up to 97 tokens, two queries each, 32 heads of 192 halves: 156 us; 148
     // without; 179 where the tiles at queries' ends, and all when done again, have a product of their own for such values.)
     bool again = false;
-    float limit = INFINITY, twice = 1.0f;  // (again: 0 and 2)
+    float limit = INFINITY, times = kTimes<T>;  // (again: 0 and twice as much)
 
     // DIRECT: the wavefront's tiles in LDS.
     Chunk<T>* const keys = reinterpret_cast<Chunk<T>*>(lds + sizeof(PhaseLds) + wave * S::BYTES);
@@ -457,13 +462,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
         }
       } else {
         // Exponentials in two parts, what the type rounds and what it leaves, so that they count with 16 bits and more.  (The matrix unit has the time: with the first
-        // part alone a pass takes as long.)
+        // part alone a pass takes as long.  A third part, 24 bits of bfloat16: 64 requests of up to 8192 tokens, 8 key heads of 64, 116 -> 136 us for its registers.)
         Chunk<T> high, low;
 #pragma unroll
         for (int t = 0; t < 8; t++) {
           const float e = score[t / 4][t % 4] > limit ? kSome<T> : score[t / 4][t % 4];
-          high[t] = (T)e;
-          low[t] = (T)fmaf(e, twice, -(float)high[t]);
+          high[t] = (T)(e * kTimes<T>);
+          low[t] = (T)fmaf(e, times, -(float)high[t]);
         }
         typedef uint32_t Words __attribute__((ext_vector_type(4)));
         Words keep;
@@ -525,7 +530,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
       for (int i = 0; i < SUB; i++)
 #pragma unroll
         for (int r = 0; r < 4; r++) most = fmaxf(most, score[i][r]);
-      if (__any(most > top + kSlack)) {
+      if (__any(most > top + kSlack<T>)) {
         most = overQuarters(most, [](float x, float y) { return fmaxf(x, y); });
         const float next = fmaxf(most, top), less = exp2Of(top - baseOf(next));
         top = next;
@@ -631,7 +636,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
       float all = -INFINITY;
 #pragma unroll
       for (uint32_t w = 0; w < kWaves; w++) all = fmaxf(all, tops[w * kColumns + l]);
-      const float mine = again ? 1.0f : exp2Of(top - baseOf(all));
+      const float mine = (again ? 1.0f : exp2Of(top - baseOf(all))) / kTimes<T>;
       if (column)
 #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -668,7 +673,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attendKernel(Atte
       if (sizeof(T) == 4 || again || !__builtin_amdgcn_readfirstlane(odd)) break;
       again = true;
       limit = 0.0f;
-      twice = 2.0f;
+      times = 2 * kTimes<T>;
       askPages(seen.first);
     }
 

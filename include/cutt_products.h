@@ -88,7 +88,9 @@ size_t cuttAttendPagesWorkspace(int queries, int heads, int keyHeads, int width,
  *   logSums           [queries, heads] in 32-bit floating point, or NULL: not wanted.  (Results over two caches can be joined by them.)
  *   workspace         cuttAttendPagesWorkspace bytes, aligned to 4; its contents need no preparation and mean nothing afterwards.  Calls that may overlap
  *                     on the GPU need one each
- * Scores, their exponentials and the sums are in 32 bits.  The strides are host arrays, read during the call.
+ * Scores, their exponentials and the sums are in 32 bits, but that the 16-bit types multiply values with exponentials in two parts of the type: to within 2^-16 of each
+ * (CUTT_BF16), or 2^-22 of each and 2^-40 of the largest (CUTT_F16).  The sums are divided at the end: values have to stay below 2^120 over the number of tokens.  The strides are host
+ * arrays, read during the call.
  */
 cuttResult cuttAttendPages(int queries, int requests, int heads, int keyHeads, int width, cuttRowType type, int pages, int pageSize, int tableWidth,
                            int window, float scale, hipStream_t stream, const int* tables, const int* owners, const int* positions, const void* q,

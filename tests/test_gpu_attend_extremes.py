@@ -191,3 +191,23 @@ def test_infinite_values_of_small_weights(below, dtype):
             cache.v[cell(cache, b, t)][:, t % 60] = INF if t % 2 else -INF
     out, logs = run_attend(q, cache, owners, positions, window, 1.0)
     check(q, cache, owners, positions, window, 1.0, out, logs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("key_heads,requests", [(1, 1), (4, 3), (2, 140)])
+@pytest.mark.parametrize("below", [6.0, 10.0, 14.0, 18.0, 20.0])
+def test_long_tails_of_small_weights(below, key_heads, requests, dtype):
+    """One token of value 0 that outweighs each of 4095 others by e^below: these are all there is in the result."""
+    g, n = generator(71), 4096 if requests < 100 else 700
+    cache = Cache([n] * requests, 64, key_heads, 64, dtype, "slot", g)
+    cache.k.zero_()
+    cache.v.uniform_(20000, 60000, generator=g)
+    q = torch.zeros(requests, 2 * key_heads, 64, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    for b in range(requests):
+        at = cell(cache, b, (b * 997 + 5) % n)
+        cache.k[at][:, 0] = below
+        cache.v[at] = 0
+    positions = ints([n - 1] * requests)
+    out, logs = run_attend(q, cache, None, positions, 0, 1.0)
+    check(q, cache, None, positions, 0, 1.0, out, logs)
