@@ -592,17 +592,17 @@ constexpr uint32_t kFewRows = 4;
 constexpr uint64_t kFew = 176, kFewUnaligned = 768;
 
 template <typename T, typename S>
-int productAs(const cuttHipProductArgs& a, bool transposed, bool ring, void* stream) {
+int productInRings(const cuttHipProductArgs& a, bool transposed, void* stream) {
   const uint64_t items = tilesOf(a, S::BM) * parts(a.outer, S::BN);
-  if (ring) {
-    auto kernel = transposed ? productRingKernel<T, true, S> : productRingKernel<T, false, S>;
-    return launchRows(kernel, ringBlocks(items), S::THREADS, S::LDS, stream, a, ringItems(items), nearOf(items));
-  }
-  if constexpr (S::BM <= 128) {
-    auto kernel = transposed ? productKernel<T, true, S> : productKernel<T, false, S>;
-    return launchRows(kernel, blocksFor(items), S::THREADS, 0, stream, a, items);
-  }
-  return 0;
+  auto kernel = transposed ? productRingKernel<T, true, S> : productRingKernel<T, false, S>;
+  return launchRows(kernel, ringBlocks(items), S::THREADS, S::LDS, stream, a, ringItems(items), nearOf(items));
+}
+template <typename T, typename S>
+int productAs(const cuttHipProductArgs& a, bool transposed, bool ring, void* stream) {
+  if (ring) return productInRings<T, S>(a, transposed, stream);
+  const uint64_t items = tilesOf(a, S::BM) * parts(a.outer, S::BN);
+  auto kernel = transposed ? productKernel<T, true, S> : productKernel<T, false, S>;
+  return launchRows(kernel, blocksFor(items), S::THREADS, 0, stream, a, items);
 }
 
 template <typename T>
@@ -623,7 +623,7 @@ int product(const cuttHipProductArgs& a, bool transposed, void* stream) {
     if (rows <= kRows32) return productAs<T, Shape<32, 128, 1, 4, 4>>(a, transposed, ring, stream);
     if (rows <= (transposed ? kRows64Transposed : kRows64) || items(128, 128) < kFew128) return productAs<T, Shape<64, 128, 2, 2, 3>>(a, transposed, ring, stream);
     if (!ring || rows <= kRows128 || items(256, 256) < kFew256) return productAs<T, Shape<128, 128, 2, 2, 2>>(a, transposed, ring, stream);
-    return productAs<T, Shape<256, 256, 2, 2, 2>>(a, transposed, ring, stream);
+    return productInRings<T, Shape<256, 256, 2, 2, 2>>(a, transposed, stream);
   }
 }
 
