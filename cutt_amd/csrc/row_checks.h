@@ -17,8 +17,8 @@ typedef unsigned __int128 Wide;
 // Byte ranges beyond this are no device buffer's (and keep the kernels' 64-bit offsets exact).
 constexpr Wide kMaxBytes = (Wide)1 << 62;
 
-// A device buffer as a call's arguments describe it: from its first to its last byte, as rows of `row` bytes every `pitch` bytes; one piece (values, a
-// row, a row that is read again and again) has no pitch.
+// A device buffer as a call's arguments describe it: from its first to its last byte, as rows of `row` bytes every `pitch` bytes (the largest stride; a row is what the others reach); one
+// piece (values, a row, a row that is read again and again) has no pitch.
 struct Span {
   uintptr_t at = 0;
   Wide bytes = 0;
@@ -85,9 +85,9 @@ inline bool strided(const void* p, int n, const unsigned long long* extent, cons
     reach += (axes.extent[i] - 1) * axes.stride[i];
   }
   s.bytes = s.row = (last + width) * size;
-  if (n == 1 && extent[0] > 1) {
-    s.row = (Wide)width * size;
-    s.pitch = (Wide)stride[0] * size;
+  if (axes.n) {
+    s.pitch = axes.stride[axes.n - 1] * size;
+    s.row -= (Wide)(axes.extent[axes.n - 1] - 1) * s.pitch;
   }
   return s.bytes <= kMaxBytes;
 }

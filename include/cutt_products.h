@@ -11,7 +11,8 @@
  *     does not synchronise, and can be captured into a HIP graph (make the call once before the capture).  The caller orders
  *     work of other streams;
  *   - buffers are aligned to their elements; any such address and any stride will do, multiples of 16 bytes are fastest.  What a
- *     call writes must not overlap what it reads;
+ *     call writes must not overlap what it reads; columns of one buffer (equal largest strides, all of a buffer's other axes within a
+ *     column) do not;
  *   - no buffer's contents can make a call touch memory outside the buffers as their sizes, strides and counts describe them;
  *   - the results do not depend on timing: equal inputs give equal bits.
  *
