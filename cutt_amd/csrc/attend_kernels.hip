@@ -793,7 +793,7 @@ Attend planAttend(uint32_t queries, uint32_t heads, uint32_t keyHeads, uint32_t 
 }
 
 // Parts of queries that the workspace has room for.
-size_t rowsOf(const Attend& p, uint32_t queries) { return p.ranges ? 2 * (size_t)p.ranges * p.most : p.pieces > 1 ? (size_t)queries * p.pieces : 0; }
+size_t rowsOf(const Attend& p, uint32_t queries) { return !queries ? 0 : p.ranges ? 2 * (size_t)p.ranges * p.most : p.pieces > 1 ? (size_t)queries * p.pieces : 0; }
 
 template <typename T, int DP, bool DIRECT>
 int attend(const Attend& p, void* stream) {

@@ -62,7 +62,8 @@ cuttResult cuttGroupedProductWeights(int rows, int groups, int inner, int outer,
 #define CUTT_MAX_HEAD_WIDTH 256
 #define CUTT_MAX_HEADS 65536
 
-/* Bytes of workspace that cuttAttendPages needs for these sizes (0: none, or arguments out of range). */
+/* Bytes of workspace that cuttAttendPages needs for these sizes (0: none, or arguments out of range).  Fewer queries may need more than many: ask for the sizes of every
+ * call, or take the largest of all that may come. */
 size_t cuttAttendPagesWorkspace(int queries, int heads, int keyHeads, int width, int pageSize, int tableWidth, int window);
 
 /*

@@ -86,6 +86,13 @@ def test_workspace_of_sizes_out_of_range(cutt):
         assert cutt.cuttAttendPagesWorkspace(*bad) == 0
 
 
+def test_no_queries_need_no_workspace(cutt):
+    for sizes in ((8, 2, 16, 16, 8), (64, 8, 128, 64, 2048), (16, 16, 256, 16, 4096)):
+        assert cutt.cuttAttendPagesWorkspace(0, *sizes, 0) == 0
+    nothing = dict(queries=0, table=4096, positions=0, q=0, out=0, logs=0, work=0, space=0)
+    assert cutt.cuttAttendPages(*{**ATTEND, **nothing}.values()) == OK
+
+
 # ---- on a stand-in for the kernels' layer -----------------------------------------
 class ProductArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint32) for n in ("rows", "groups", "inner", "outer")] + [(n, ctypes.c_void_p) for n in ("offsets", "x", "w", "y")] + \
