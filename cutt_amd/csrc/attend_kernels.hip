@@ -7,8 +7,11 @@
  * twice 16.
  *
  * Every cached element is read once, and takes two operations for each of the query heads that share it: memory bounds it, and where there is little of it the chain
- * offsets -> page -> keys -> scores -> values -> joined parts.  64 requests of up to 8192 tokens, 32 heads on 8 key heads of 128 bfloat16 (1075 MB): 194 us, 5.5 TB/s, where a pure
- * read of as much reaches 6.2 (6.9 past the caches); 256 requests of 2048 each: 338 us, 6.4 TB/s; one request of 128 tokens: 7.3 us.
+ * offsets -> page -> keys -> scores -> values -> joined parts.  64 requests of up to 8192 tokens, 32 heads on 8 key heads of 128 bfloat16 (1075 MB): 177 to 197 us by where the pages lie in
+ * memory, 5.5 to 6.1 TB/s, where a pure read of as much reaches 6.2 (6.9 past the caches); 256 requests of 2048 each: 338 us, 6.4 TB/s; one request of 128 tokens: 7.5 us.
+ *
+ * Many queries of one request are right but not fast: a workgroup has 16 columns, and every further 16 / (heads / keyHeads) queries read the keys and values again (4 requests with
+ * 4096 queries for 4096 tokens each, the same heads: 3.57 ms, 0.15 PFLOP/s of what they see).
  */
 #include <algorithm>
 #include <cfloat>

@@ -52,7 +52,7 @@ cuttResult cuttGroupedProduct(int rows, int groups, int inner, int outer, cuttRo
  *   x                 [rows, inner] with row stride xStride         dy  [rows, outer] with row stride dyStride
  *   dw                [groups, inner, outer]
  *   dwStrides[2]      elements from group to group and from row to row of dw: rows must not lie on top of each other
- * For weights that are used transposed, exchange x and dy, inner and outer.
+ * For weights that are used transposed, exchange x and dy, inner and outer.  Fastest where all rows of x, and all of dy, span less than 2^30 bytes.
  */
 cuttResult cuttGroupedProductWeights(int rows, int groups, int inner, int outer, cuttRowType type, hipStream_t stream, const int* offsets, const void* x,
                                      long long xStride, const void* dy, long long dyStride, void* dw, const long long* dwStrides);
@@ -67,7 +67,8 @@ cuttResult cuttGroupedProductWeights(int rows, int groups, int inner, int outer,
 size_t cuttAttendPagesWorkspace(int queries, int heads, int keyHeads, int width, int pageSize, int tableWidth, int window);
 
 /*
- * Queries of new tokens over the cached keys and values of their requests, which lie in pages as in cutt_rows.h (store the new tokens' own first).
+ * Queries of new tokens over the cached keys and values of their requests, which lie in pages as in cutt_rows.h (store the new tokens' own first).  Made for one or a few queries of
+ * a request, which follow each other; prompts are right but not fast, as their queries read the keys and values again, a few queries at a time.
  * Query i belongs to request b = owners[i] and has the position p = positions[i].  It sees the tokens at the positions
  *   first .. p,   first = max(0, p - window + 1), or 0 without a window,
  * as far as they have a page in tables[b]: those beyond the table's width or of a page that is absent (an entry not in 0 .. pages - 1) are not seen.

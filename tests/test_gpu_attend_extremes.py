@@ -211,3 +211,17 @@ def test_long_tails_of_small_weights(below, key_heads, requests, dtype):
     positions = ints([n - 1] * requests)
     out, logs = run_attend(q, cache, None, positions, 0, 1.0)
     check(q, cache, None, positions, 0, 1.0, out, logs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("name", FORMS)
+def test_results_beside_queries(name, dtype):
+    """Queries and results in the columns of one buffer, as a fused projection leaves them: results as into a buffer of their own, everything else as it was."""
+    cache, q, owners, positions, window, lengths, g = form(name, dtype, 64)
+    queries, heads, width = q.shape
+    want, want_logs = run_attend(q, cache, owners, positions, window, 0.125)
+    rows = torch.full((queries, 3 * heads, width), 5.0, dtype=dtype, device="cuda")
+    rows[:, :heads] = q
+    out, logs = run_attend(rows[:, :heads], cache, owners, positions, window, 0.125, out=rows[:, heads:2 * heads])
+    assert torch.equal(out, want) and torch.equal(logs, want_logs)
+    assert torch.equal(rows[:, :heads], q) and bool((rows[:, 2 * heads:] == 5).all())
