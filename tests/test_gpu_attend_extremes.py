@@ -6,8 +6,9 @@ import numpy as np
 import pytest
 import torch
 
+import cutt_amd as cutt
 import product_oracle as oracle
-from test_gpu_products import HALF, LEAST, TYPES, UNIT, Cache, generator, ids_of, ints, np64, run_attend
+from test_gpu_products import CODE, HALF, LEAST, TYPES, UNIT, Cache, generator, ids_of, ints, np64, run_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +226,70 @@ def test_results_beside_queries(name, dtype):
     out, logs = run_attend(rows[:, :heads], cache, owners, positions, window, 0.125, out=rows[:, heads:2 * heads])
     assert torch.equal(out, want) and torch.equal(logs, want_logs)
     assert torch.equal(rows[:, :heads], q) and bool((rows[:, 2 * heads:] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("requests,longest,heads,key_heads,width", [(256, 4500, 16, 1, 64), (2, 55000, 16, 16, 32)])
+def test_infinite_values_of_long_parts(requests, longest, heads, key_heads, width, dtype):
+    """Workgroups whose parts have more tokens than they work out addresses for at a time, one of them without an infinity; others take many queries one after the other."""
+    g = generator(81)
+    lengths = [5] * requests
+    lengths[0], lengths[requests // 2] = longest, longest // 2 + 77
+    cache = Cache(lengths, 32, key_heads, width, dtype, "head", g)
+    q = torch.randn(requests, heads, width, generator=g, device="cuda").to(dtype)
+    for b, n in ((0, longest), (requests - 1, lengths[-1])):
+        for d, t in enumerate((0, 1200, n // 2, n - 1, n - 1030)):
+            if 0 <= t < n:
+                cache.v[cell(cache, b, t)][:, 2 * d] = INF if d % 2 else -INF
+    positions = ints([n - 1 for n in lengths])
+    out, logs = run_attend(q, cache, None, positions, 0, width ** -0.5)
+    check(q, cache, None, positions, 0, width ** -0.5, out, logs)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=ids_of[1:])
+def test_queries_without_numbers(dtype):
+    """A query of NaN gets NaN, whatever infinities its tokens have; the others of its request are as without it."""
+    cache, q, owners, positions, window, lengths, g = form("drafts", dtype, 64)
+    cache.v[cell(cache, 0, lengths[0] - 3)][:, 7] = INF
+    want, want_logs = run_attend(q, cache, owners, positions, window, 0.125)
+    assert bool((want[:3, :, 7] == INF).all())
+    q[1] = float("nan")
+    out, logs = run_attend(q, cache, owners, positions, window, 0.125)
+    assert bool(out[1].isnan().all()) and bool(logs[1].isnan().all())
+    others = [i for i in range(len(owners)) if i != 1]
+    assert torch.equal(out[others], want[others]) and torch.equal(logs[others], want_logs[others])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+def test_infinities_that_come_and_go_between_replays(dtype):
+    """A captured call whose cache gets infinite values and loses them: every replay as the eager call, bit by bit."""
+    cache, q, owners, positions, window, lengths, g = form("long", dtype, 64)
+    out, logs = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    queries, heads, width = q.shape
+    space = cutt.cuttAttendPagesWorkspace(queries, heads, 2, width, cache.page, cache.tables.shape[1], window)
+    work = torch.empty(space, dtype=torch.uint8, device="cuda")
+
+    def call():
+        assert cutt.cuttAttendPages(queries, len(lengths), heads, 2, width, CODE[dtype], cache.pages, cache.page, cache.tables.shape[1], window, 0.125,
+                                    torch.cuda.current_stream().cuda_stream, cache.tables.data_ptr(), owners.data_ptr(), positions.data_ptr(), q.data_ptr(),
+                                    q.stride()[:2], cache.k.data_ptr(), cache.v.data_ptr(), cache.k.stride()[:3], out.data_ptr(), out.stride()[:2], logs.data_ptr(),
+                                    work.data_ptr(), space) == cutt.CUTT_SUCCESS
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    clean = cache.v.clone()
+    for turn in range(5):
+        cache.v.copy_(clean)
+        if turn % 2:
+            cache.v[cell(cache, 0, 1000 * turn)][:, 11] = INF
+            cache.v[cell(cache, 1, 39)][:, 12] = -INF
+        call()
+        want, want_logs = out.clone(), logs.clone()
+        out.fill_(7), logs.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(9), want.nan_to_num(9)) and torch.equal(logs, want_logs)
+        assert bool((out[0, :, 11] == INF).all()) == bool(turn % 2) and not bool(out.isnan().any())
